@@ -42,6 +42,7 @@ extern "C" {
 #define Q4K_TYPE_F16 1
 #define Q4K_TYPE_Q4_K 12
 #define Q4K_TYPE_Q6_K 14
+#define Q4K_TYPE_BF16 30
 
 /* Epilogues of q4k_matmul_ex. */
 #define Q4K_EPI_STORE 0  /* y = W x                                   */
@@ -192,6 +193,97 @@ int q4k_attention_decode_f16_static(const float* qkv, const float* q_gamma, cons
                                     uint16_t* v_cache, int capacity, const int* position_device, int query_heads,
                                     int kv_heads, int head_dim, float epsilon, float rope_base, float* output,
                                     void* stream);
+
+/* ---------------------------------------- paged KV cache and sampling (new) */
+
+/* One layer's K and V in pages of page_size positions: element (page, head,
+ * row, dim) is at page * page_stride + head * head_stride + row * row_stride
+ * + dim, strides in elements (so both [page][head][row][dim] and
+ * [page][row][head][dim] orders, and views of larger buffers, are taken).
+ * type Q4K_TYPE_F16 or Q4K_TYPE_BF16; head_dim 64 or 128; page_size a power
+ * of two from 16 to 256; k and v 16-byte aligned, strides multiples of 8. */
+typedef struct {
+    void* k;
+    void* v;
+    int type;
+    int kv_heads, head_dim, page_size;
+    int64_t pages;
+    int64_t page_stride, head_stride, row_stride;
+} q4k_paged_kv;
+
+/* The sequences of one call. Their new tokens are consecutive rows: sequence
+ * s has rows q_start[s] .. q_start[s + 1] - 1 (possibly none), and kv_len[s]
+ * cached tokens with the new ones, whose last is at position kv_len[s] - 1.
+ * Position p is row p % page_size of page page_table[s * table_stride +
+ * p / page_size]. The arrays are on the device (so a captured call follows
+ * their contents); rows from q_start[sequences] on belong to no sequence and
+ * their outputs are left as they were. max_new is a bound on the new tokens
+ * of any one sequence, known to the host: 1 for a decode step; 0 if unknown.
+ * Rows of a sequence past max_new of them are not attended (their outputs are
+ * unspecified). */
+typedef struct {
+    int sequences;
+    int max_new;
+    const int* q_start;    /* [sequences + 1], ascending */
+    const int* kv_len;     /* [sequences] */
+    const int* page_table; /* [sequences][table_stride] */
+    int64_t table_stride;
+    int table_width; /* entries of a table row that exist (positions below table_width * page_size) */
+} q4k_paged_batch;
+
+/* Appends the batch's new tokens to the cache, as one launch: per query and
+ * key head the RMSNorm (q_gamma, k_gamma: head_dim floats; NULL: no norm) and
+ * RoPE (pair (j, j + head_dim / 2) by position * rope_base^(-2j/head_dim), the
+ * angle taken in fp64), queries to q_out, keys and values to the cache. q, k
+ * and v rows (one per token, heads consecutive) are ld_* elements apart and
+ * `type`: the cache's type, or Q4K_TYPE_F32 with an fp16 cache. q and q_out
+ * may both be NULL (query_heads is then ignored), and may be the same buffer.
+ * A token whose position is negative or past the page table, or whose page is
+ * not one of the cache's (a negative entry marks a page to skip), is not
+ * written to the cache; its query is still rotated. The paged form of
+ * Engine.cpp:87-91. Buffers 16-byte aligned, ld_* whole 16-byte words. */
+int q4k_paged_append(const q4k_paged_kv* cache, const q4k_paged_batch* batch, size_t tokens, int type, const void* q,
+                     int64_t ld_q, int query_heads, const void* k, int64_t ld_k, const void* v, int64_t ld_v,
+                     const float* q_gamma, const float* k_gamma, float epsilon, float rope_base, void* q_out,
+                     int64_t ld_q_out, void* stream);
+
+/* Causal attention of the batch's new tokens over their sequences' pages (the
+ * paged, ragged form of kernels::attention): the token at position p attends
+ * to positions max(0, p - window + 1) .. p (window 0: from 0). query_heads is
+ * a multiple of kv_heads; scale 0: 1 / sqrt(head_dim). q and output rows as
+ * in q4k_paged_append. lse (optional, [tokens][query_heads] floats) receives
+ * the natural logarithm of each row's sum of exponentials. A token that
+ * attends to nothing (position < 0) gets zeros and lse -inf. Table entries
+ * outside the cache read as zero keys and values. fp32 activations keep fp32
+ * accuracy (queries and probabilities enter the tensor cores as fp16 high and
+ * low parts); 16-bit ones round their probabilities to 16 bits, sums are
+ * fp32. workspace: q4k_paged_attention_workspace_bytes of the same call's
+ * numbers, 16-byte aligned, contents irrelevant; calls that may overlap in
+ * time need workspaces of their own. As in q4k_attention_decode_f16, waits on
+ * copies are bounded (2 s); if one gives up, the output is undefined. */
+int q4k_paged_attention(const q4k_paged_kv* cache, const q4k_paged_batch* batch, size_t tokens, int type,
+                        const void* q, int64_t ld_q, int query_heads, float scale, int window, void* output,
+                        int64_t ld_output, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+size_t q4k_paged_attention_workspace_bytes(int query_heads, int kv_heads, int head_dim, int max_new);
+
+/* Draws one token per row of logits (the sampling counterpart of q4k_argmax).
+ * With x_i = (logit_i - max) / temperature and w_i = e^x_i, tokens in order of
+ * logit (ties: lowest index first): top_k keeps the first k (<= 0: all), then
+ * top_p the shortest prefix holding at least top_p of their weight (>= 1: all;
+ * at least one token), then min_p those with w_i >= min_p, i.e. min_p of the
+ * likeliest's (<= 0: all; above 1 as 1). The token is the first in index order
+ * whose running sum of kept weights exceeds uniform * their total, uniform in
+ * [0, 1) being the caller's random number. temperature <= 0 (or NaN): the
+ * argmax. All per row on the device ([rows]); temperature, top_k, top_p and
+ * min_p may be NULL (1, all, all, all). logits of `type` F32, F16 or BF16,
+ * rows ld elements apart; -inf and NaN logits are never drawn, +inf ones share
+ * the row. tokens[r] is -1 (logprob -inf) for a row with no logit above -inf.
+ * logprob (optional) receives the natural logarithm of the token's probability
+ * among the kept. Sums are exact (whole numbers), so results do not depend on
+ * how the work is split. vocab <= 400000. */
+int q4k_sample(const void* logits, int type, int64_t ld, size_t rows, size_t vocab, const float* temperature,
+               const int* top_k, const float* top_p, const float* min_p, const float* uniform, int32_t* tokens,
+               float* logprob, void* stream);
 
 /* ------------------------------------------------------- decode engine */
 

@@ -13,6 +13,7 @@
 #include "gguf.h"
 #include "nccl_api.h"
 #include "ops.h"
+#include "paged.h"
 #include "q4k_format.h"
 #include "q4k_internal.h"
 
@@ -394,6 +395,155 @@ Q4K_API int q4k_matmul_batch(const float* input, const float* norm_gamma, float 
         }
         cudaFreeAsync(ws, s);
         launched(e);
+    });
+}
+
+namespace {
+
+[[noreturn]] void out_of_range(const char* msg) { throw q4k::Error(Q4K_ERANGE, msg); }
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+// Token rows of `heads` heads, `ld` elements apart.
+void check_rows(const void* p, int64_t ld, int heads, int head_dim, bool f32, const char* what) {
+    if (!p || !aligned16(p)) invalid((std::string(what) + " must be a 16-byte aligned device buffer").c_str());
+    if (ld < (int64_t)heads * head_dim || ld % (f32 ? 4 : 8) || ld > (int64_t)1 << 40)
+        invalid((std::string(what) + " rows must hold their heads and start on 16-byte words").c_str());
+}
+
+q4k::PagedCache paged_cache(const q4k_paged_kv* c, int type) {
+    if (!c || !c->k || !c->v || !aligned16(c->k) || !aligned16(c->v))
+        invalid("a paged cache needs 16-byte aligned K and V buffers");
+    if (c->type != Q4K_TYPE_F16 && c->type != Q4K_TYPE_BF16) invalid("a paged cache is F16 or BF16");
+    if (type != c->type && !(type == Q4K_TYPE_F32 && c->type == Q4K_TYPE_F16))
+        invalid("paged activations are of the cache's type, or F32 with an F16 cache");
+    if (c->head_dim != 64 && c->head_dim != 128) invalid("a paged cache has head_dim 64 or 128");
+    if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
+        invalid("page_size must be a power of two from 16 to 256");
+    if (c->kv_heads < 1 || c->kv_heads > 4096 || c->pages < 1) invalid("a paged cache needs heads and pages");
+    if (c->pages > std::numeric_limits<int>::max()) out_of_range("too many pages");
+    for (int64_t s : {c->page_stride, c->head_stride, c->row_stride}) {
+        if (s < c->head_dim || s % 8) invalid("paged cache strides must be multiples of 8 and hold a row");
+        if (s >= (int64_t)1 << 38) out_of_range("paged cache strides are too large");
+    }
+    q4k::PagedCache r;
+    r.k = static_cast<uint16_t*>(c->k);
+    r.v = static_cast<uint16_t*>(c->v);
+    r.bf16 = c->type == Q4K_TYPE_BF16;
+    r.kv_heads = c->kv_heads;
+    r.head_dim = c->head_dim;
+    r.page_size = c->page_size;
+    while ((1 << r.page_shift) < c->page_size) ++r.page_shift;
+    r.pages = c->pages;
+    r.page_stride = c->page_stride;
+    r.head_stride = c->head_stride;
+    r.row_stride = c->row_stride;
+    return r;
+}
+
+q4k::PagedBatch paged_batch(const q4k_paged_batch* b, size_t tokens, int page_size) {
+    if (!b || b->sequences < 0 || b->max_new < 0) invalid("invalid batch of sequences");
+    if (tokens > (1u << 24) || b->sequences > (1 << 20)) out_of_range("too many tokens or sequences");
+    q4k::PagedBatch r;
+    r.sequences = b->sequences;
+    r.tokens = (int)tokens;
+    if (r.sequences == 0 || r.tokens == 0) return r;
+    if (!b->q_start || !b->kv_len || !b->page_table) invalid("a batch needs q_start, kv_len and a page table");
+    if (b->table_width < 1 || b->table_stride < b->table_width) invalid("page table rows must hold table_width entries");
+    if (b->table_width > std::numeric_limits<int>::max() / page_size - 1) out_of_range("the page table is too wide");
+    r.q_start = b->q_start;
+    r.kv_len = b->kv_len;
+    r.page_table = b->page_table;
+    r.table_stride = b->table_stride;
+    r.table_width = b->table_width;
+    r.max_new = b->max_new == 0 || b->max_new > r.tokens ? r.tokens : b->max_new;
+    return r;
+}
+
+}  // namespace
+
+Q4K_API int q4k_paged_append(const q4k_paged_kv* cache, const q4k_paged_batch* batch, size_t tokens, int type,
+                             const void* q, int64_t ld_q, int query_heads, const void* k, int64_t ld_k, const void* v,
+                             int64_t ld_v, const float* q_gamma, const float* k_gamma, float epsilon, float rope_base,
+                             void* q_out, int64_t ld_q_out, void* stream) {
+    return guarded_cuda([&] {
+        q4k::PagedAppendArgs a;
+        a.cache = paged_cache(cache, type);
+        a.batch = paged_batch(batch, tokens, a.cache.page_size);
+        if (!(rope_base > 0.0f) || std::isinf(rope_base)) invalid("RoPE requires a positive frequency base");
+        if ((q_gamma || k_gamma) && !(epsilon > 0.0f)) invalid("RMSNorm requires a positive epsilon");
+        if (!q != !q_out) invalid("q and q_out go together");
+        if (a.batch.sequences == 0 || a.batch.tokens == 0) return;
+        a.f32 = type == Q4K_TYPE_F32;
+        const int d = a.cache.head_dim;
+        if (q) {
+            if (query_heads < 1 || query_heads > (1 << 15)) invalid("invalid number of query heads");
+            check_rows(q, ld_q, query_heads, d, a.f32, "q");
+            check_rows(q_out, ld_q_out, query_heads, d, a.f32, "q_out");
+            a.heads = query_heads;
+        }
+        check_rows(k, ld_k, a.cache.kv_heads, d, a.f32, "k");
+        check_rows(v, ld_v, a.cache.kv_heads, d, a.f32, "v");
+        a.q = q, a.k = k, a.v = v, a.q_out = q_out;
+        a.ld_q = ld_q, a.ld_k = ld_k, a.ld_v = ld_v, a.ld_q_out = ld_q_out;
+        a.q_gamma = q_gamma, a.k_gamma = k_gamma;
+        a.eps = epsilon;
+        a.rope_base = rope_base;
+        launched(q4k::paged_append(a, as_stream(stream)));
+    });
+}
+
+Q4K_API size_t q4k_paged_attention_workspace_bytes(int query_heads, int kv_heads, int head_dim, int max_new) {
+    if (kv_heads < 1 || query_heads < 1 || query_heads % kv_heads || (head_dim != 64 && head_dim != 128) || max_new < 0)
+        return 0;
+    return q4k::paged_attention_workspace_bytes(query_heads, kv_heads, head_dim, max_new);
+}
+
+Q4K_API int q4k_paged_attention(const q4k_paged_kv* cache, const q4k_paged_batch* batch, size_t tokens, int type,
+                                const void* q, int64_t ld_q, int query_heads, float scale, int window, void* output,
+                                int64_t ld_output, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded_cuda([&] {
+        q4k::PagedAttentionArgs a;
+        a.cache = paged_cache(cache, type);
+        a.batch = paged_batch(batch, tokens, a.cache.page_size);
+        if (query_heads < 1 || query_heads > (1 << 15) || query_heads % a.cache.kv_heads)
+            invalid("query_heads must be a multiple of the cache's heads");
+        if (!(scale >= 0.0f) || std::isinf(scale)) invalid("the scale must be positive, or 0 for 1 / sqrt(head_dim)");
+        if (window < 0) invalid("the window must be positive, or 0 for none");
+        if (a.batch.sequences == 0 || a.batch.tokens == 0) return;
+        a.f32 = type == Q4K_TYPE_F32;
+        check_rows(q, ld_q, query_heads, a.cache.head_dim, a.f32, "q");
+        check_rows(output, ld_output, query_heads, a.cache.head_dim, a.f32, "output");
+        const size_t need = q4k::paged_attention_workspace_bytes(query_heads, a.cache.kv_heads, a.cache.head_dim,
+                                                                 batch->max_new);
+        if (need && (!workspace || !aligned16(workspace))) invalid("attention needs a 16-byte aligned workspace");
+        if (workspace_bytes < need) out_of_range("the workspace is smaller than q4k_paged_attention_workspace_bytes");
+        a.q = q, a.out = output, a.lse = lse;
+        a.ld_q = ld_q, a.ld_out = ld_output;
+        a.heads = query_heads;
+        a.scale = scale > 0.0f ? scale : 1.0f / std::sqrt((float)a.cache.head_dim);
+        a.window = window;
+        a.workspace = workspace;
+        launched(q4k::paged_attention(a, as_stream(stream)));
+    });
+}
+
+Q4K_API int q4k_sample(const void* logits, int type, int64_t ld, size_t rows, size_t vocab, const float* temperature,
+                       const int* top_k, const float* top_p, const float* min_p, const float* uniform, int32_t* tokens,
+                       float* logprob, void* stream) {
+    return guarded_cuda([&] {
+        if (type != Q4K_TYPE_F32 && type != Q4K_TYPE_F16 && type != Q4K_TYPE_BF16)
+            invalid("logits are F32, F16 or BF16");
+        if (vocab == 0) invalid("Invalid sampling input");
+        if (vocab > 400000 || rows > (1u << 20)) out_of_range("sampling takes up to 400000 logits a row");
+        if (rows == 0) return;
+        if (!logits || !uniform || !tokens || ld < (int64_t)vocab) invalid("Invalid sampling input");
+        q4k::SampleArgs a;
+        a.logits = logits, a.type = type, a.ld = ld;
+        a.rows = (int)rows, a.vocab = (int)vocab;
+        a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p, a.uniform = uniform;
+        a.tokens = tokens, a.logprob = logprob;
+        launched(q4k::sample(a, as_stream(stream)));
     });
 }
 

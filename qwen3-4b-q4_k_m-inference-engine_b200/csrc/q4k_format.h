@@ -35,6 +35,7 @@
 #define Q4K_TYPE_F16 1
 #define Q4K_TYPE_Q4_K 12
 #define Q4K_TYPE_Q6_K 14
+#define Q4K_TYPE_BF16 30
 #endif
 
 #define Q4K_QK 256

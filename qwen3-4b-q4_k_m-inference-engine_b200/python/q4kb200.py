@@ -17,7 +17,7 @@ PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(PKG_DIR, "lib", "libq4kb200.so")
 
 OK, EINVAL, ERANGE, ECUDA, ETIMEOUT = 0, 1, 2, 3, 4
-F32, F16, Q4_K, Q6_K = 0, 1, 12, 14
+F32, F16, Q4_K, Q6_K, BF16 = 0, 1, 12, 14, 30
 EPI_STORE, EPI_ADD, EPI_SWIGLU, EPI_ARGMAX = 0, 1, 2, 3
 
 # Every symbol the C ABI exports (checked by the CPU tests against the header).
@@ -37,6 +37,7 @@ EXPORTS = (
     "q4k_engine_set_limits",
     "q4k_engine_abort",
     "q4k_tp_sum_parts",
+    "q4k_paged_append", "q4k_paged_attention", "q4k_paged_attention_workspace_bytes", "q4k_sample",
 )
 
 
@@ -68,6 +69,17 @@ class EngineConfig(C.Structure):
 
     def as_dict(self) -> dict:
         return {f: getattr(self, f) for f, _ in self._fields_}
+
+
+class _PagedKV(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("page_size", C.c_int), ("pages", C.c_int64), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("row_stride", C.c_int64)]
+
+
+class _PagedBatch(C.Structure):
+    _fields_ = [("sequences", C.c_int), ("max_new", C.c_int), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
+                ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("table_width", C.c_int)]
 
 
 _lib = None
@@ -104,6 +116,12 @@ def lib():
             "q4k_attention_decode_f16": ([P, P, P, P, P, I, P, I, I, I, C.c_float, C.c_float, P, P, P], I),
             "q4k_attention_decode_f16_static": ([P, P, P, P, P, I, P, I, I, I, C.c_float, C.c_float, P, P], I),
             "q4k_attention_decode_scratch_bytes": ([I, I], S),
+            "q4k_paged_append": ([C.POINTER(_PagedKV), C.POINTER(_PagedBatch), S, I, P, I64, I, P, I64, P, I64, P, P,
+                                  C.c_float, C.c_float, P, I64, P], I),
+            "q4k_paged_attention": ([C.POINTER(_PagedKV), C.POINTER(_PagedBatch), S, I, P, I64, I, C.c_float, I, P, I64,
+                                     P, P, S, P], I),
+            "q4k_paged_attention_workspace_bytes": ([I, I, I, I], S),
+            "q4k_sample": ([P, I, I64, S, S, P, P, P, P, P, P, P, P], I),
             "q4k_engine_config_qwen3_4b": ([C.POINTER(EngineConfig), I], None),
             "q4k_model_tensor": ([C.POINTER(EngineConfig), I, C.c_char_p, S, C.POINTER(I), C.POINTER(I64),
                                   C.POINTER(I64)], I),
@@ -454,6 +472,197 @@ class Engine:
         n = C.c_size_t(0)
         check(lib().q4k_engine_trace(self.h, token, position, hptr(rec), rec.size, C.byref(n)))
         return rec
+
+
+# ------------------------------------- paged KV cache and sampling (torch tensors)
+def _torch_type(dtype) -> int:
+    import torch
+
+    types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+    if dtype not in types:
+        raise InvalidArgument(EINVAL, f"unsupported tensor type {dtype}")
+    return types[dtype]
+
+
+def _on_device(t, what: str, dtype=None, device=None):
+    """t, checked to be a CUDA tensor (of dtype, on device)."""
+    if not t.is_cuda or (device is not None and t.device != device):
+        raise InvalidArgument(EINVAL, f"{what} must be on {device if device is not None else 'a CUDA device'}")
+    if dtype is not None and t.dtype != dtype:
+        raise InvalidArgument(EINVAL, f"{what} must be {dtype}")
+    return t
+
+
+class _on:
+    """The call's device made current, and its stream: `stream`, or torch's
+    current one there."""
+
+    def __init__(self, device, stream):
+        import torch
+
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        self.device, self.stream = device, stream
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        if self.stream is not None:
+            return stream_ptr(self.stream)
+        import torch
+
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+class PagedKV:
+    """One layer's paged K and V (q4k_paged_kv): tensors (possibly views) of
+    shape [pages][kv_heads][page_size][head_dim], fp16 or bf16, of one shape and
+    strides, the last dimension contiguous. A [pages][page_size][kv_heads]
+    [head_dim] cache is passed as its transpose(1, 2)."""
+
+    def __init__(self, k, v):
+        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
+            raise InvalidArgument(EINVAL, "k and v must be alike, [pages][kv_heads][page_size][head_dim]")
+        _on_device(k, "k")
+        _on_device(v, "v", device=k.device)
+        self.k, self.v = k, v
+        pages, heads, rows, d = k.shape
+        s = k.stride()
+        # a dimension of one element has no stride of its own
+        self.c = _PagedKV(k.data_ptr(), v.data_ptr(), _torch_type(k.dtype), heads, d, rows, pages,
+                          s[0] if pages > 1 else max(s[0], d), s[1] if heads > 1 else max(s[1], d), s[2])
+
+
+class PagedBatch:
+    """The sequences of a call (q4k_paged_batch): q_start [n + 1], kv_len [n] and
+    page_table [n][width], int32 on the device. max_new: a bound on the new
+    tokens of any one sequence (1 for a decode step; 0: unknown)."""
+
+    def __init__(self, q_start, kv_len, page_table, max_new: int = 0):
+        import torch
+
+        n = kv_len.numel()
+        for t, what in ((q_start, "q_start"), (kv_len, "kv_len"), (page_table, "page_table")):
+            _on_device(t, what, torch.int32, kv_len.device)
+        if (q_start.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n or not q_start.is_contiguous()
+                or not kv_len.is_contiguous() or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
+            raise InvalidArgument(EINVAL, "q_start [n + 1], kv_len [n] and page_table [n][width] do not fit together")
+        self.tensors = (q_start, kv_len, page_table)
+        width = page_table.shape[1]
+        self.c = _PagedBatch(n, max_new, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
+                             max(page_table.stride(0), width) if n > 1 else width, width)
+
+
+def _token_rows(t, what: str, heads: int | None, head_dim: int, like=None):
+    """(address, elements between token rows) of a [tokens][heads][head_dim] tensor."""
+    if (t.dim() != 3 or t.shape[2] != head_dim or t.stride(2) != 1 or (heads is not None and t.shape[1] != heads)
+            or (t.shape[1] > 1 and t.stride(1) != head_dim)):
+        raise InvalidArgument(EINVAL, f"{what} must be [tokens][heads][head_dim] with contiguous heads")
+    if like is not None:
+        _on_device(t, what, like.dtype, like.device)
+        if t.shape[0] != like.shape[0]:
+            raise InvalidArgument(EINVAL, f"{what} must have as many rows as the others")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * head_dim
+
+
+def _floats(t, what: str, n: int, device, dtype=None):
+    import torch
+
+    if t is None:
+        return None
+    _on_device(t, what, dtype or torch.float32, device)
+    if t.numel() != n or not t.is_contiguous():
+        raise InvalidArgument(EINVAL, f"{what} must hold {n} values")
+    return t.data_ptr()
+
+
+def paged_append(cache: PagedKV, batch: PagedBatch, k, v, q=None, q_out=None, q_gamma=None, k_gamma=None,
+                 epsilon: float = 1e-6, rope_base: float = 1e6, stream=None):
+    """Norm (with a gamma), rotate and append the batch's new tokens
+    (q4k_paged_append). k, v: [tokens][kv_heads][head_dim]; q (optional):
+    [tokens][heads][head_dim]. Returns the rotated queries (q_out, allocated
+    like q if not given), or None without q."""
+    import torch
+
+    d, device = cache.c.head_dim, cache.k.device
+    _on_device(k, "k", device=device)
+    _on_device(batch.tensors[0], "the batch", device=device)
+    pk, lk = _token_rows(k, "k", cache.c.kv_heads, d)
+    pv, lv = _token_rows(v, "v", cache.c.kv_heads, d, k)
+    pq = po = None
+    lq = lo = heads = 0
+    if q is not None:
+        heads = q.shape[1]
+        if q_out is None:
+            q_out = torch.empty((q.shape[0], heads, d), dtype=q.dtype, device=device)
+        pq, lq = _token_rows(q, "q", None, d, k)
+        po, lo = _token_rows(q_out, "q_out", heads, d, k)
+    elif q_out is not None:
+        raise InvalidArgument(EINVAL, "q and q_out go together")
+    qg, kg = _floats(q_gamma, "q_gamma", d, device), _floats(k_gamma, "k_gamma", d, device)
+    with _on(device, stream) as s:
+        check(lib().q4k_paged_append(C.byref(cache.c), C.byref(batch.c), k.shape[0], _torch_type(k.dtype), pq, lq, heads,
+                                     pk, lk, pv, lv, qg, kg, epsilon, rope_base, po, lo, s))
+    return q_out
+
+
+def paged_attention(cache: PagedKV, batch: PagedBatch, q, out=None, lse=None, scale: float = 0.0, window: int = 0,
+                    workspace=None, stream=None):
+    """Causal attention of q [tokens][heads][head_dim] over the batch's pages
+    (q4k_paged_attention). Returns out (allocated like q if not given); lse
+    ([tokens][heads] fp32) is filled if given. The workspace comes from torch's
+    allocator, on its current stream, unless given (uint8)."""
+    import torch
+
+    d, device = cache.c.head_dim, cache.k.device
+    _on_device(q, "q", device=device)
+    _on_device(batch.tensors[0], "the batch", device=device)
+    pq, lq = _token_rows(q, "q", None, d)
+    tokens, heads = q.shape[0], q.shape[1]
+    if out is None:
+        out = torch.empty((tokens, heads, d), dtype=q.dtype, device=device)
+    po, lo = _token_rows(out, "out", heads, d, q)
+    pl = _floats(lse, "lse", tokens * heads, device)
+    with _on(device, stream) as s:
+        need = lib().q4k_paged_attention_workspace_bytes(heads, cache.c.kv_heads, d, batch.c.max_new)
+        if workspace is None and need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+            if stream is not None:
+                # memory of torch's current stream, used on the caller's
+                handle = torch.cuda.ExternalStream(s, device=device) if s else torch.cuda.default_stream(device)
+                workspace.record_stream(handle)
+        size = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        check(lib().q4k_paged_attention(C.byref(cache.c), C.byref(batch.c), tokens, _torch_type(q.dtype), pq, lq, heads,
+                                        scale, window, po, lo, pl, ptr(workspace), size, s))
+    return out
+
+
+def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, logprob=None,
+           stream=None):
+    """One token per row of logits [rows][vocab] (q4k_sample); uniform,
+    temperature, top_p, min_p: [rows] fp32, top_k: [rows] int32, on the device.
+    Returns (tokens int32, logprob fp32), allocated if not given."""
+    import torch
+
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise InvalidArgument(EINVAL, "logits must be [rows][vocab] with contiguous rows")
+    rows, vocab = logits.shape
+    device = _on_device(logits, "logits").device
+    if tokens is None:
+        tokens = torch.empty(rows, dtype=torch.int32, device=device)
+    if logprob is None:
+        logprob = torch.empty(rows, dtype=torch.float32, device=device)
+    args = [_floats(temperature, "temperature", rows, device), _floats(top_k, "top_k", rows, device, torch.int32),
+            _floats(top_p, "top_p", rows, device), _floats(min_p, "min_p", rows, device),
+            _floats(uniform, "uniform", rows, device), _floats(tokens, "tokens", rows, device, torch.int32),
+            _floats(logprob, "logprob", rows, device)]
+    with _on(device, stream) as s:
+        check(lib().q4k_sample(logits.data_ptr(), _torch_type(logits.dtype), logits.stride(0) if rows > 1 else vocab,
+                               rows, vocab, *args, s))
+    return tokens, logprob
 
 
 def nccl_unique_id() -> bytes:
