@@ -510,6 +510,8 @@ Q4K_API int q4k_paged_attention(const q4k_paged_kv* cache, const q4k_paged_batch
             invalid("query_heads must be a multiple of the cache's heads");
         if (!(scale >= 0.0f) || std::isinf(scale)) invalid("the scale must be positive, or 0 for 1 / sqrt(head_dim)");
         if (window < 0) invalid("the window must be positive, or 0 for none");
+        if ((int64_t)a.batch.tokens * query_heads > std::numeric_limits<int>::max() || a.batch.sequences > 8192)
+            out_of_range("attention takes up to 2^31 - 1 query rows and 8192 sequences");
         if (a.batch.sequences == 0 || a.batch.tokens == 0) return;
         a.f32 = type == Q4K_TYPE_F32;
         check_rows(q, ld_q, query_heads, a.cache.head_dim, a.f32, "q");

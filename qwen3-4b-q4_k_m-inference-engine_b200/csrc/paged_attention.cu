@@ -6,98 +6,607 @@
 // with a window of w also k > p - w. A row with no key gets o = 0, lse = -inf.
 #include <math_constants.h>
 
-#include "paged.h"
-#include "paged_device.cuh"
+#include <cstring>
+#include <mutex>
+
+#include "ops.h"
+#include "paged_plan.cuh"
+#include "paged_tc.cuh"
 
 namespace q4k {
 namespace {
 
 using namespace paged_dev;
 
-// One CTA per (row, query head): four warps take every fourth key with an
-// online softmax of their own and are joined at the end.
-template <typename T, typename C, int D>
-__global__ void __launch_bounds__(128) paged_attention_kernel(const __grid_constant__ PagedAttentionArgs a) {
-    constexpr int V = D / 32;
-    const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int s = 0;
-    for (int i = 0; i < a.batch.sequences; i += 128)
-        s += __syncthreads_count(i + tid < a.batch.sequences && __ldg(a.batch.q_start + i + tid + 1) <= t);
-    if (s >= a.batch.sequences) return;
-    const int len = __ldg(a.batch.kv_len + s);
-    const int position = len - __ldg(a.batch.q_start + s + 1) + t;
-    const long long held = (long long)a.batch.table_width << a.cache.page_shift;
-    const int end = (int)min((long long)position + 1, held);
-    const int begin = a.window > 0 ? max(position - a.window + 1, 0) : 0;
-    const int kvh = h / (a.heads / a.cache.kv_heads);
-    const T* q = static_cast<const T*>(a.q) + t * a.ld_q + (size_t)h * D + lane * V;
-    float x[V], o[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        x[i] = to_float<T>(q[i]) * a.scale;
-        o[i] = 0.0f;
-    }
-    float m = -CUDART_INF_F, l = 0.0f;
-    for (int p = begin + warp; p < end; p += 4) {
-        const int page = __ldg(a.batch.page_table + (size_t)s * a.batch.table_stride + (p >> a.cache.page_shift));
-        if (page < 0 || page >= a.cache.pages) continue;
-        const long long at = page * a.cache.page_stride + kvh * a.cache.head_stride +
-                             (p & (a.cache.page_size - 1)) * a.cache.row_stride + lane * V;
-        const C* k = reinterpret_cast<const C*>(a.cache.k) + at;
-        const C* v = reinterpret_cast<const C*>(a.cache.v) + at;
-        float dot = 0.0f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) dot += x[i] * to_float<C>(k[i]);
-        dot = warp_sum(dot);
-        const float mn = fmaxf(m, dot);
-        const float r = expf(m - mn), e = expf(dot - mn);
-        l = l * r + e;
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = o[i] * r + e * to_float<C>(v[i]);
-        m = mn;
-    }
-    __shared__ float wm[4], wl[4], wo[4][D];
-    if (lane == 0) {
-        wm[warp] = m;
-        wl[warp] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) wo[warp][lane * V + i] = o[i];
-    __syncthreads();
-    if (tid >= D) return;
-    float top = wm[0], total = 0.0f, sum = 0.0f;
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, wm[w]);
-    for (int w = 0; w < 4; ++w) {
-        if (!(wl[w] > 0.0f)) continue;
-        const float f = expf(wm[w] - top);
-        total += f * wl[w];
-        sum += f * wo[w][tid];
-    }
-    static_cast<T*>(a.out)[t * a.ld_out + (size_t)h * D + tid] = from_float<T>(total > 0.0f ? sum / total : 0.0f);
-    if (tid == 0 && a.lse) a.lse[(size_t)t * a.heads + h] = total > 0.0f ? top + logf(total) : -CUDART_INF_F;
+enum class Kind { kF32, kF16, kBf16 };
+
+constexpr int kTileRows = 256;   // two MMA tiles of 128 query rows
+constexpr int kBlockKeys = 128;
+constexpr int kTcThreads = 320;  // two softmax warpgroups, TMA warp, MMA warp
+constexpr int kMinUnits = 2;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+// The reference point of a row's exponentials moves only when its maximum
+// has grown by more than 2^8: probabilities stay below 256, far inside
+// fp16, and the accumulator is rescaled a few times per row instead of at
+// every block.
+constexpr float kLazy = 8.0f;
+// fp16 probabilities are kept 2^7 times larger, at most 2^15: fp16 ends at
+// 2^-24, so that one of 2^-32 of the row's largest still has its low part.
+template <Kind K>
+constexpr float kBias = K == Kind::kBf16 ? 0.0f : 7.0f;
+
+template <Kind K>
+struct Types {
+    using Act = __half;
+};
+template <>
+struct Types<Kind::kF32> {
+    using Act = float;
+};
+template <>
+struct Types<Kind::kBf16> {
+    using Act = __nv_bfloat16;
+};
+
+// Shared memory: Q (per MMA tile: the fp16 high and, for fp32 activations,
+// low parts; 64-dim halves of 128 rows x 128 bytes), then the ring of K and V
+// blocks in the same layout.
+template <Kind K, int D>
+struct Layout {
+    static constexpr int kParts = K == Kind::kF32 ? 2 : 1;
+    static constexpr int kHalf = 128 * 128;
+    static constexpr int kMat = D / 64 * kHalf;  // 128 rows of D 16-bit values
+    static constexpr int kStages = D == 64 ? 8 : K == Kind::kF32 ? 3 : 5;
+    static constexpr int kRing = 2 * kParts * kMat;
+    static constexpr int kBars = kRing + kStages * kMat;
+    static constexpr int kBytes = kBars + 512 + 1024;  // barriers and slots, alignment slack
+    static_assert(kBytes <= 227 * 1024, "shared memory of one CTA");
+};
+
+struct TcBars {
+    uint64_t full[8], empty[8];
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
+    uint32_t tmem;
+    int dead;
+    Share share;
+};
+static_assert(sizeof(TcBars) <= 512, "barrier area");
+
+// The workspace: a note per CTA and piece, then per CTA and piece the rows'
+// (m, l) and unnormalised outputs.
+struct Partials {
+    PieceNote* notes;  // [ctas][2]
+    float2* ml;        // [ctas][2][kTileRows]
+    float* o;          // [ctas][2][kTileRows][D]
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
-template <typename T, typename C>
-void launch(const PagedAttentionArgs& a, cudaStream_t s) {
-    const dim3 grid(a.batch.tokens, a.heads);
-    if (a.cache.head_dim == 128)
-        paged_attention_kernel<T, C, 128><<<grid, 128, 0, s>>>(a);
-    else
-        paged_attention_kernel<T, C, 64><<<grid, 128, 0, s>>>(a);
+template <Kind K>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (K == Kind::kBf16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+}
+
+// hi, lo: fp16 parts of (a, b); hi + lo is within 2^-22 of each.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+template <Kind K, int D>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    paged_attention_tc_kernel(const __grid_constant__ PagedAttentionArgs a, const __grid_constant__ CUtensorMap kmap,
+                              const __grid_constant__ CUtensorMap vmap, const Partials part) {
+    using L = Layout<K, D>;
+    using Act = typename Types<K>::Act;
+    constexpr int kStages = L::kStages;
+    constexpr uint32_t kIdescS = idesc_f16(K == Kind::kBf16, 128, kBlockKeys, false);
+    constexpr uint32_t kIdescO = idesc_f16(K == Kind::kBf16, 128, D, true);
+    // TMEM columns: S (its probabilities written over it) and O of each MMA tile
+    constexpr uint32_t kS = 0, kO = 256;
+
+    extern __shared__ uint8_t smem_dyn[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
+    TcBars& bar = *reinterpret_cast<TcBars*>(smem + L::kBars);
+    volatile int* dead = &bar.dead;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int group = a.heads / a.cache.kv_heads;
+    const int held = a.batch.table_width << a.cache.page_shift;
+
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&bar.full[i], 1);
+            mbar_init(&bar.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar.q_full[i], 4);
+            mbar_init(&bar.s_full[i], 1);
+            mbar_init(&bar.p_full[i], 4);
+            mbar_init(&bar.o_full[i], 1);
+        }
+        mbar_init(&bar.done, 1);
+        bar.dead = 0;
+        mbar_fence_init();
+    }
+    if (warp == 9) tmem_alloc(&bar.tmem, 512);
+    tc_fence_before();
+    plan_share<kTileRows, kBlockKeys>(a.batch, group, a.cache.kv_heads, a.window, held, kMinUnits,
+                                      reinterpret_cast<unsigned long long*>(smem + L::kRing), &bar.share);
+    tc_fence_after();
+    const uint32_t tmem = bar.tmem;
+    fence_proxy_async();  // the plan's words, before the ring's copies land on them
+    __syncthreads();
+    Pieces<kTileRows, kBlockKeys> pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
+
+    if (warp == 8) {
+        // ---------------- TMA: K and V blocks, page by page, a lane per (page, half)
+        const int box = min(a.cache.page_size, kBlockKeys);
+        const int boxes = kBlockKeys / box;
+        const int page_in_block = lane / (D / 64), half = lane % (D / 64);
+        const uint32_t box_bytes = (uint32_t)box * D * 2;
+        int n = 0;
+        bool ok = true;
+        for (; pc.valid() && ok; pc.next()) {
+            for (int i = 0; i < pc.count && ok; ++i) {
+                const int key0 = pc.tile.key_begin + (pc.b + i) * kBlockKeys;
+                const int live = min(max((pc.tile.key_end - key0 + box - 1) / box, 0), boxes);
+                int page = -1;
+                if (page_in_block < live)
+                    page = __ldg(a.batch.page_table + (size_t)pc.s * a.batch.table_stride +
+                                 ((key0 + page_in_block * box) >> a.cache.page_shift));
+                for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
+                    const int st = n % kStages;
+                    ok = wait_or_dead(&bar.empty[st], ((n / kStages) & 1) ^ 1, dead);
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) mbar_arrive_expect_tx(&bar.full[st], live * box_bytes);
+                    __syncwarp();
+                    if (page_in_block < live)
+                        tma_load_4d(smem + L::kRing + st * L::kMat + half * L::kHalf + page_in_block * box * 128,
+                                    kv ? &vmap : &kmap, half * 64, key0 & (a.cache.page_size - 1), pc.h, page,
+                                    &bar.full[st]);
+                }
+            }
+        }
+        // every copy issued has landed before the CTA can exit
+        for (int i = max(n - kStages, 0); i < n; ++i) 
+            mbar_wait_bounded(&bar.full[i % kStages], (i / kStages) & 1, nullptr, 0);
+        __syncwarp();
+    } else if (warp == 9) {
+        if (lane == 0) {
+            // ---------------- MMA issue
+            int n = 0;
+            uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+            bool ok = true;
+            const uint32_t q_addr = smem_addr(smem), ring = smem_addr(smem + L::kRing);
+            auto wait_stage = [&](int i) { return wait_or_dead(&bar.full[i % kStages], (i / kStages) & 1, dead); };
+            auto score = [&](int t, int stage) {
+                const uint32_t k = ring + (stage % kStages) * L::kMat;
+#pragma unroll
+                for (int pt = 0; pt < L::kParts; ++pt)
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = (kk / 4) * L::kHalf + (kk % 4) * 32;
+                        mma_ss(tmem + kS + 128 * t, desc_k_major(q_addr + (t * L::kParts + pt) * L::kMat + off),
+                               desc_k_major(k + off), kIdescS, (pt | kk) != 0);
+                    }
+                tc_commit(&bar.s_full[t]);
+            };
+            auto value = [&](int t, int stage, bool accumulate) {
+                const uint32_t v = ring + (stage % kStages) * L::kMat;
+#pragma unroll
+                for (int kk = 0; kk < kBlockKeys / 16; ++kk)
+#pragma unroll
+                    for (int pt = 0; pt < L::kParts; ++pt)
+                        mma_ts(tmem + kO + 128 * t, tmem + kS + 128 * t + 64 * pt + 8 * kk,
+                               desc_mn_major(v + kk * 2048, L::kHalf), kIdescO, accumulate || (pt | kk) != 0);
+            };
+            for (; pc.valid() && ok; pc.next()) {
+                const int tiles = pc.tile.rows > 128 ? 2 : 1;
+                int k_stage = n++;
+                ok = wait_stage(k_stage);
+                for (int t = 0; t < tiles && ok; ++t) {
+                    ok = wait_or_dead(&bar.q_full[t], q_phase[t]++ & 1, dead);
+                    if (!ok) break;
+                    tc_fence_after();
+                    score(t, k_stage);
+                }
+                tc_commit(&bar.empty[k_stage % kStages]);
+                for (int i = 0; i < pc.count && ok; ++i) {
+                    const bool more = i + 1 < pc.count;
+                    const int v_stage = n++;
+                    if (more) k_stage = n++;
+                    for (int t = 0; t < tiles && ok; ++t) {
+                        ok = wait_or_dead(&bar.p_full[t], p_phase[t]++ & 1, dead) && wait_stage(v_stage);
+                        if (!ok) break;
+                        tc_fence_after();
+                        value(t, v_stage, i > 0);
+                        if (more) {
+                            ok = wait_stage(k_stage);
+                            if (!ok) break;
+                            tc_fence_after();
+                            score(t, k_stage);
+                        } else {
+                            tc_commit(&bar.o_full[t]);
+                        }
+                    }
+                    tc_commit(&bar.empty[v_stage % kStages]);
+                    if (more) tc_commit(&bar.empty[k_stage % kStages]);
+                }
+            }
+            if (!ok) {  // the MMAs in flight end before the TMEM is freed
+                tc_commit(&bar.done);
+                mbar_wait_bounded(&bar.done, 0, nullptr, 0);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---------------- softmax: warpgroup t, a thread per query row
+        const int t = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t s_addr = tmem + kS + 128 * t + lanes, o_addr = tmem + kO + 128 * t + lanes;
+        int n = 1;  // ring number of the block's V
+        uint32_t items = 0, phase = 0;
+        bool ok = true, left[2] = {false, false};
+        for (; pc.valid() && ok; pc.next()) {
+            const Tile& tl = pc.tile;
+            const int tile_row = 128 * t + row;
+            if (tl.rows <= 128 * t) {
+                n += 2 * pc.count;
+                continue;
+            }
+            const bool live = tile_row < tl.rows;
+            const int r = tl.row0 + tile_row;
+            const int token = r / group, head = pc.h * group + r % group;
+            const size_t out_row = (size_t)pc.seq.first_row + token;
+            // keys this row sees
+            const int position = pc.seq.position + token;
+            const int last = live ? min(position, held - 1) : -1;
+            const int first = a.window > 0 ? max(position - a.window + 1, 0) : 0;
+            float c = a.scale * kLog2e;
+            {
+                // Q into shared memory; fp32 rows scaled by a power of two to
+                // below 2^8 so that any fp32 query fits the fp16 parts
+                uint8_t* qs = smem + t * L::kParts * L::kMat;
+                const Act* q = static_cast<const Act*>(a.q) + (live ? out_row * a.ld_q + (size_t)head * D : 0);
+                if constexpr (K == Kind::kF32) {
+                    float most = 0.0f;
+                    for (int i = 0; i < D; i += 8) {
+                        float x[8];
+                        load_values<float, 8>(q + i, x);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
+                    }
+                    const int e = min(max((int)(__float_as_uint(most) >> 23) - 126, -100), 127);  // most < 2^e
+                    // 2^(8 - e) in two factors, since 2^-119 and 2^108 only fit together
+                    const float f1 = __uint_as_float((uint32_t)(127 + (8 - e) / 2) << 23);
+                    const float f2 = __uint_as_float((uint32_t)(127 + (8 - e) - (8 - e) / 2) << 23);
+                    c = c / f1 / f2;
+                    for (int i = 0; i < D / 8; ++i) {
+                        float x[8];
+                        load_values<float, 8>(q + 8 * i, x);
+                        uint4 hi, lo;
+                        split2(x[0] * f1 * f2, x[1] * f1 * f2, hi.x, lo.x);
+                        split2(x[2] * f1 * f2, x[3] * f1 * f2, hi.y, lo.y);
+                        split2(x[4] * f1 * f2, x[5] * f1 * f2, hi.z, lo.z);
+                        split2(x[6] * f1 * f2, x[7] * f1 * f2, hi.w, lo.w);
+                        if (!live) hi = lo = make_uint4(0u, 0u, 0u, 0u);
+                        uint8_t* at = qs + (i >> 3) * L::kHalf + swz128(row, i & 7);
+                        *reinterpret_cast<uint4*>(at) = hi;
+                        *reinterpret_cast<uint4*>(at + L::kMat) = lo;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) {
+                        uint4 x = __ldg(reinterpret_cast<const uint4*>(q) + i);
+                        if (!live) x = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4*>(qs + (i >> 3) * L::kHalf + swz128(row, i & 7)) = x;
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.q_full[t]);
+            }
+            float m = -CUDART_INF_F, l = 0.0f;
+            for (int i = 0; i < pc.count && ok; ++i, ++phase, n += 2) {
+                const int key0 = tl.key_begin + (pc.b + i) * kBlockKeys;
+                if (t == 0 && (key0 < tl.key_first || key0 + kBlockKeys > tl.key_end)) {
+                    // rows of V that no query row sees may hold anything (or
+                    // were never loaded): zeros, since 0 times them is not 0
+                    ok = wait_or_dead(&bar.full[n % kStages], (n / kStages) & 1, dead);
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        ok = false;
+                        break;
+                    }
+                    const int key = key0 + row;
+                    if (key < tl.key_first || key >= tl.key_end) {
+                        uint8_t* v = smem + L::kRing + (n % kStages) * L::kMat;
+#pragma unroll
+                        for (int j = 0; j < D / 8; ++j)
+                            *reinterpret_cast<uint4*>(v + (j >> 3) * L::kHalf + swz128(row, j & 7)) =
+                                make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async();
+                }
+                ok = wait_or_dead(&bar.s_full[t], phase & 1, dead);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) tmem_ld32(s_addr + 32 * j, s[j]);
+                tmem_wait_ld();
+                if (__any_sync(0xffffffffu, key0 + kBlockKeys - 1 > last || key0 < first)) {
+                    const int lo = first - key0, hi = last - key0;
+#pragma unroll
+                    for (int j = 0; j < 128; ++j)
+                        if (j < lo || j > hi) s[j >> 5][j & 31] = 0xff800000u;
+                }
+                float mx[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mx[j] = __uint_as_float(s[j][0]);
+#pragma unroll
+                for (int e = 1; e < 32; ++e)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mx[j] = fmaxf(mx[j], __uint_as_float(s[j][e]));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                if (__any_sync(0xffffffffu, top > m + kLazy)) {
+                    const float mn = top > m + kLazy ? top : m;
+                    if (i > 0) {
+                        const float f = mn == m ? 1.0f : exp2_fast(m - mn);
+                        l *= f;
+                        // the score MMAs of this block were committed after the
+                        // last block's value MMAs: O is at rest
+#pragma unroll 1
+                        for (int j = 0; j < D / 32; ++j) {
+                            uint32_t o[32];
+                            tmem_ld32(o_addr + 32 * j, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st32(o_addr + 32 * j, o);
+                        }
+                    }
+                    m = mn;
+                }
+                const float shift = m == -CUDART_INF_F ? 0.0f : m - kBias<K>;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (K == Kind::kF32) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t hi[32];  // 16 high words, then 16 low ones
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float p0 = exp2_fast(fmaf(__uint_as_float(s[j][2 * e]), c, -shift));
+                            const float p1 = exp2_fast(fmaf(__uint_as_float(s[j][2 * e + 1]), c, -shift));
+                            sum[e & 3] += p0 + p1;
+                            split2(p0, p1, hi[e], hi[16 + e]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) s[j][e] = hi[e];
+                    }
+#pragma unroll
+                    for (int pt = 0; pt < 2; ++pt)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            uint32_t w[32];
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) w[e] = s[2 * j + (e >> 4)][16 * pt + (e & 15)];
+                            tmem_st32(s_addr + 64 * pt + 32 * j, w);
+                        }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float p0 =
+                                exp2_fast(fmaf(__uint_as_float(s[2 * j + (e >> 4)][2 * (e & 15)]), c, -shift));
+                            const float p1 =
+                                exp2_fast(fmaf(__uint_as_float(s[2 * j + (e >> 4)][2 * (e & 15) + 1]), c, -shift));
+                            sum[e & 3] += p0 + p1;
+                            w[e] = pack2<K>(p0, p1);
+                        }
+                        tmem_st32(s_addr + 32 * j, w);
+                    }
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.p_full[t]);
+            }
+            if (!ok) break;
+            ok = wait_or_dead(&bar.o_full[t], items & 1, dead);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_fence_after();
+            ++items;
+            const bool whole = pc.whole();
+            const size_t slot = ((size_t)blockIdx.x * 2 + (pc.index > 0)) * kTileRows + tile_row;
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll 1
+            for (int j = 0; j < D / 32; ++j) {
+                uint32_t o[32];
+                tmem_ld32(o_addr + 32 * j, o);
+                tmem_wait_ld();
+                if (!live) continue;
+                float x[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(o[e]);
+                if (whole) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[e] = l > 0.0f ? x[e] * inv : 0.0f;
+                    store_values<Act, 32>(static_cast<Act*>(a.out) + out_row * a.ld_out + (size_t)head * D + 32 * j, x);
+                } else {
+                    store_values<float, 32>(part.o + slot * D + 32 * j, x);
+                }
+            }
+            if (live && whole && a.lse)
+                a.lse[out_row * a.heads + head] = l > 0.0f ? (m - kBias<K> + log2f(l)) * kLn2 : -CUDART_INF_F;
+            if (!whole) {
+                part.ml[slot] = make_float2(m - kBias<K>, l);
+                left[pc.index > 0] = true;
+                if (tid == 0)
+                    part.notes[blockIdx.x * 2 + (pc.index > 0)] = {pc.s, pc.h, pc.r, pc.b, pc.count, tl.blocks};
+            }
+            // O has been read before the next piece's first value MMA
+            tc_fence_before();
+        }
+        if (tid == 0)
+            for (int i = 0; i < 2; ++i)
+                if (!left[i]) part.notes[blockIdx.x * 2 + i] = {0, 0, 0, 0, 0, 0};
+    }
+    pdl_launch_dependents();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// The tiles that several CTAs share: CTA c's block of this grid joins the
+// tile that begins in c's share and ends in a later one's, in the order of
+// the CTAs. One warp per query row.
+template <typename Act, int D, int kRows>
+__global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_constant__ PagedAttentionArgs a,
+                                                                   const Partials part, int rows_per_block) {
+    constexpr int V = D / 32;
+    pdl_wait();
+    const int c0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int own = 1;
+    PieceNote n = part.notes[2 * c0 + 1];
+    if (n.count == 0) {
+        own = 0;
+        n = part.notes[2 * c0];
+    }
+    if (n.count == 0 || n.b != 0) return;
+    int pieces = 1;
+    for (int end = n.count; end < n.blocks && c0 + pieces < (int)gridDim.x; ++pieces)
+        end += part.notes[2 * (c0 + pieces)].count;
+    const int group = a.heads / a.cache.kv_heads;
+    const Sequence q = sequence_of(a.batch, n.s);
+    const int rows = min(q.rows * group - n.r * kRows, kRows);
+    const int begin = blockIdx.y * rows_per_block;
+    auto slot = [&](int i) { return (size_t)2 * (c0 + i) + (i == 0 ? own : 0); };
+    for (int row = begin + warp; row < min(begin + rows_per_block, rows); row += 4) {
+        float m = -CUDART_INF_F;
+        for (int i = lane; i < pieces; i += 32) m = fmaxf(m, part.ml[slot(i) * kRows + row].x);
+        m = warp_max(m);
+        float l = 0.0f, o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = 0.0f;
+        for (int i = 0; i < pieces; ++i) {
+            const size_t at = slot(i) * kRows + row;
+            const float2 ml = part.ml[at];
+            if (!(ml.y != 0.0f)) continue;
+            const float f = exp2_fast(ml.x - m);
+            l += f * ml.y;
+            const float* src = part.o + at * D + lane * V;
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] += f * src[j];
+        }
+        const int r = n.r * kRows + row;
+        const int head = n.h * group + r % group;
+        const size_t out_row = (size_t)q.first_row + r / group;
+        Act* out = static_cast<Act*>(a.out) + out_row * a.ld_out + (size_t)head * D + lane * V;
+#pragma unroll
+        for (int j = 0; j < V; ++j) out[j] = from_float<Act>(l != 0.0f ? o[j] / l : 0.0f);
+        if (lane == 0 && a.lse)
+            a.lse[out_row * a.heads + head] = l != 0.0f ? (m + log2f(l)) * kLn2 : -CUDART_INF_F;
+    }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// K or V pages as (dim, row, head, page): boxes of 64 dims and up to `rows`
+// rows of a page. A page number outside the cache reads as zeros.
+bool page_map(const PagedCache& c, const uint16_t* base, int rows, CUtensorMap* map) {
+    const EncodeTiled encode = reinterpret_cast<EncodeTiled>(tensor_map_encoder());
+    if (!encode) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)c.head_dim, (cuuint64_t)c.page_size, (cuuint64_t)c.kv_heads,
+                                (cuuint64_t)c.pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.row_stride * 2, (cuuint64_t)c.head_stride * 2,
+                                   (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(c.page_size < rows ? c.page_size : rows), 1, 1};
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    return encode(map, c.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                  const_cast<uint16_t*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+size_t partial_bytes(int ctas, int rows, int head_dim) {
+    return (size_t)ctas * 2 * (32 + (size_t)rows * (sizeof(float2) + sizeof(float) * head_dim));
+}
+
+Partials partials(void* workspace, int ctas, int rows) {
+    static_assert(sizeof(PieceNote) <= 32, "notes");
+    Partials p;
+    uint8_t* w = static_cast<uint8_t*>(workspace);
+    p.notes = reinterpret_cast<PieceNote*>(w);
+    p.ml = reinterpret_cast<float2*>(w + (size_t)ctas * 2 * 32);
+    p.o = reinterpret_cast<float*>(w + (size_t)ctas * 2 * (32 + (size_t)rows * sizeof(float2)));
+    return p;
+}
+
+template <Kind K, int D>
+cudaError_t launch_tc(const PagedAttentionArgs& a, cudaStream_t s) {
+    using L = Layout<K, D>;
+    auto kernel = paged_attention_tc_kernel<K, D>;
+    static std::once_flag once;
+    static cudaError_t attr = cudaSuccess;
+    std::call_once(once, [&] {
+        attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    });
+    if (attr != cudaSuccess) return attr;
+    CUtensorMap km, vm;
+    if (!page_map(a.cache, a.cache.k, kBlockKeys, &km) || !page_map(a.cache, a.cache.v, kBlockKeys, &vm))
+        return cudaErrorInvalidValue;
+    const int ctas = sm_count();
+    const Partials part = partials(a.workspace, ctas, kTileRows);
+    kernel<<<ctas, kTcThreads, L::kBytes, s>>>(a, km, vm, part);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    return launch_pdl(paged_attention_join_kernel<typename Types<K>::Act, D, kTileRows>, dim3(ctas, kTileRows / 32),
+                      dim3(128), 0, s, a, part, 32);
+}
+
+template <Kind K>
+cudaError_t launch(const PagedAttentionArgs& a, cudaStream_t s) {
+    return a.cache.head_dim == 128 ? launch_tc<K, 128>(a, s) : launch_tc<K, 64>(a, s);
 }
 
 }  // namespace
 
-size_t paged_attention_workspace_bytes(int, int, int, int) { return 0; }
+size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int max_new) {
+    (void)heads, (void)kv_heads, (void)max_new;
+    return partial_bytes(sm_count(), kTileRows, head_dim);
+}
 
 cudaError_t paged_attention(const PagedAttentionArgs& a, cudaStream_t s) {
-    if (a.f32)
-        launch<float, __half>(a, s);
-    else if (a.cache.bf16)
-        launch<__nv_bfloat16, __nv_bfloat16>(a, s);
-    else
-        launch<__half, __half>(a, s);
-    return cudaGetLastError();
+    if (a.f32) return launch<Kind::kF32>(a, s);
+    return a.cache.bf16 ? launch<Kind::kBf16>(a, s) : launch<Kind::kF16>(a, s);
 }
 
 }  // namespace q4k

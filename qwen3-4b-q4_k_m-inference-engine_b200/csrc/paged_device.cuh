@@ -17,7 +17,6 @@ struct Sequence {
     int first_row;  // of q, k, v and the outputs
     int rows;       // new tokens
     int position;   // of the first new token (negative: rows before the cache's start)
-    int keys;       // cached tokens
 };
 
 __device__ __forceinline__ Sequence sequence_of(const PagedBatch& b, int s) {

@@ -1,0 +1,180 @@
+// How attention's work over a batch of sequences is cut: the same plan is
+// worked out by every CTA from the lengths on the device, so that a captured
+// launch follows them.
+//
+// A tile is kRows query rows (new token x query head of one KV head) of one
+// sequence and KV head; its keys are cut into blocks of kBlock positions. The
+// blocks of all tiles, in the order sequence, KV head, tile, block, are dealt
+// out in equal contiguous shares, one per CTA: lengths of any raggedness keep
+// every CTA busy, long contexts with few rows are split over many CTAs, and
+// a CTA has at most two tiles that it shares with others (its first and its
+// last). Those leave partial sums in the workspace, which a second kernel
+// joins in the order of the CTAs.
+#pragma once
+#include "paged_device.cuh"
+
+namespace q4k {
+namespace paged_dev {
+
+// Rows and keys of tile r of a sequence.
+struct Tile {
+    int row0, rows;        // query rows row0 .. row0 + rows - 1 of the sequence (row = token * group + head)
+    int key_begin;         // first key any row sees, rounded down to a block
+    int key_first;         // first key any row sees
+    int key_end;           // past the last key any row sees
+    int blocks;            // at least 1 (its outputs have to be written)
+};
+
+template <int kRows, int kBlock>
+__device__ __forceinline__ Tile tile_of(const Sequence& q, int r, int group, int window, int held) {
+    Tile t;
+    t.row0 = r * kRows;
+    t.rows = min(q.rows * group - t.row0, kRows);
+    const int first = q.position + t.row0 / group, last = q.position + (t.row0 + t.rows - 1) / group;
+    t.key_end = max(min(last, held - 1) + 1, 0);
+    t.key_first = window > 0 ? max(first - window + 1, 0) : 0;
+    t.key_begin = t.key_first & ~(kBlock - 1);
+    t.blocks = max((t.key_end - t.key_begin + kBlock - 1) / kBlock, 1);
+    return t;
+}
+
+template <int kRows>
+__device__ __forceinline__ int tiles_of(const Sequence& q, int group) {
+    return (q.rows * group + kRows - 1) / kRows;
+}
+
+// Where a CTA's share begins, and how many blocks it is.
+struct Share {
+    int s, h, r, b;
+    int units;
+    int ctas;  // that have a share
+};
+
+// Worked out by all threads; per_seq ([sequences] words of shared memory) and
+// out are free to use and reuse once it returns. Ends with a barrier.
+template <int kRows, int kBlock>
+__device__ __forceinline__ void plan_share(const PagedBatch& b, int group, int kv_heads, int window, int held,
+                                           int min_units, unsigned long long* per_seq, Share* out) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    for (int s = warp; s < b.sequences; s += warps) {
+        const Sequence q = sequence_of(b, s);
+        const int n = tiles_of<kRows>(q, group);
+        unsigned long long sum = 0;
+        for (int r = lane; r < n; r += 32) sum += tile_of<kRows, kBlock>(q, r, group, window, held).blocks;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) per_seq[s] = sum;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        unsigned long long all = 0;
+        for (int s = lane; s < b.sequences; s += 32) all += per_seq[s];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        all *= kv_heads;
+        const unsigned long long want = (all + min_units - 1) / min_units;
+        const int ctas = want < gridDim.x ? (int)want : (int)gridDim.x;
+        Share v = {0, 0, 0, 0, 0, ctas};
+        if ((int)blockIdx.x < ctas) {
+            unsigned long long at = all * blockIdx.x / ctas;
+            v.units = (int)(all * (blockIdx.x + 1) / ctas - at);
+            // the sequence, 32 at a time
+            for (int base = 0; base < b.sequences; base += 32) {
+                const unsigned long long mine = base + lane < b.sequences ? per_seq[base + lane] * kv_heads : 0;
+                unsigned long long run = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned long long u = __shfl_up_sync(0xffffffffu, run, o);
+                    if (lane >= o) run += u;
+                }
+                const unsigned past = __ballot_sync(0xffffffffu, run > at);
+                if (past) {
+                    const int l = __ffs(past) - 1;
+                    at -= __shfl_sync(0xffffffffu, run - mine, l);
+                    v.s = base + l;
+                    break;
+                }
+                at -= __shfl_sync(0xffffffffu, run, 31);
+            }
+            const unsigned long long head = per_seq[v.s];
+            v.h = (int)(at / head);
+            at %= head;
+            // the tile, 32 at a time
+            const Sequence q = sequence_of(b, v.s);
+            const int n = tiles_of<kRows>(q, group);
+            for (int base = 0; base < n; base += 32) {
+                const unsigned long long mine =
+                    base + lane < n ? tile_of<kRows, kBlock>(q, base + lane, group, window, held).blocks : 0;
+                unsigned long long run = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned long long u = __shfl_up_sync(0xffffffffu, run, o);
+                    if (lane >= o) run += u;
+                }
+                const unsigned past = __ballot_sync(0xffffffffu, run > at);
+                if (past) {
+                    const int l = __ffs(past) - 1;
+                    at -= __shfl_sync(0xffffffffu, run - mine, l);
+                    v.r = base + l;
+                    break;
+                }
+                at -= __shfl_sync(0xffffffffu, run, 31);
+            }
+            v.b = (int)at;
+        }
+        if (lane == 0) *out = v;
+    }
+    __syncthreads();
+}
+
+// A share's pieces in turn: piece [b, b + count) of the blocks of `tile`.
+template <int kRows, int kBlock>
+struct Pieces {
+    const PagedBatch& batch;
+    int group, kv_heads, window, held;
+    int s, h, r, b, left, count, index;
+    Sequence seq;
+    Tile tile;
+
+    __device__ __forceinline__ Pieces(const PagedBatch& batch, int group, int kv_heads, int window, int held,
+                                      const Share& share)
+        : batch(batch), group(group), kv_heads(kv_heads), window(window), held(held), s(share.s), h(share.h),
+          r(share.r), b(share.b), left(share.units), count(0), index(0) {
+        if (left > 0) enter();
+    }
+    __device__ __forceinline__ void enter() {
+        seq = sequence_of(batch, s);
+        take();
+    }
+    __device__ __forceinline__ void take() {
+        tile = tile_of<kRows, kBlock>(seq, r, group, window, held);
+        count = min(tile.blocks - b, left);
+    }
+    __device__ __forceinline__ bool valid() const { return left > 0; }
+    __device__ __forceinline__ bool whole() const { return b == 0 && count == tile.blocks; }
+    __device__ __forceinline__ void next() {
+        left -= count;
+        ++index;
+        if (left <= 0) return;
+        b = 0;
+        if (++r < tiles_of<kRows>(seq, group)) return take();
+        r = 0;
+        if (++h < kv_heads) return take();
+        h = 0;
+        do {  // a sequence with work follows, as blocks are left
+            ++s;
+            seq = sequence_of(batch, s);
+        } while (seq.rows == 0 && s + 1 < batch.sequences);
+        take();
+    }
+};
+
+// What a CTA leaves for the joining kernel: of its first and last piece, where
+// they belong. Pieces 0 and 1 are different ones, or only 0 is there.
+struct PieceNote {
+    int s, h, r;
+    int b, count, blocks;  // count 0: nothing left here
+};
+
+}  // namespace paged_dev
+}  // namespace q4k

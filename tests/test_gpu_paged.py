@@ -58,8 +58,8 @@ class Case:
 
     def check(self, out, lse, window=0, scale=None):
         """Per element: 16-bit types round each probability (u of sum p|v|; fp16 also 2^-25 of the row's largest below
-        2^-14) and the output (u |o|); fp32 carries both as fp16 pairs (2^-22 and 2^-25 as above for the low part's
-        own rounding, 2^-36) and adds fp32 sums. Scores are sums of d products in fp32: 1e-5 is 2^-23 for each
+        2^-14) and the output (u |o|); fp32 carries both as fp16 pairs (2^-22, and fp16's last place 2^-25 of 2^7
+        times a probability) and adds fp32 sums. Scores are sums of d products in fp32: 1e-5 is 2^-23 for each
         of 8 blocks of 16 products with |s| up to 10, and moves a probability by as much."""
         scale = self.d ** -0.5 if scale is None else scale
         u, tiny = {"f32": (0.0, 0.0), "f16": (2.0 ** -11, 2.0 ** -25), "bf16": (2.0 ** -8, 0.0)}[self.kind]
@@ -70,7 +70,8 @@ class Case:
             want, want_lse, size, flat = ref.attention(self.q[rows], k, v, c - n, scale, window)
             err = (out[rows].double() - want).abs()
             bound = u * (size + want.abs()) + tiny * (flat + 1) + 2e-5 * size
-            assert torch.isfinite(out[rows]).all() and (err <= bound).all(), (i, n, c, float((err / bound.clamp(min=1e-30)).max()))
+            worst = float((err / bound.clamp(min=1e-30)).max()) if n else 0.0
+            assert bool(torch.isfinite(out[rows]).all()) and worst <= 1.0, (i, n, c, worst)
             if self.kind == "f32" and n and c:
                 assert err.norm() <= 1e-5 * want.norm(), (i, n, c, float(err.norm() / want.norm()))
             none = want_lse == -math.inf
