@@ -219,8 +219,8 @@ typedef struct {
  * their contents); rows from q_start[sequences] on belong to no sequence and
  * their outputs are left as they were. max_new is a bound on the new tokens
  * of any one sequence, known to the host: 1 for a decode step; 0 if unknown.
- * Rows of a sequence past max_new of them are not attended (their outputs are
- * unspecified). */
+ * It only chooses how the work is cut; results do not depend on it beyond
+ * rounding. */
 typedef struct {
     int sequences;
     int max_new;

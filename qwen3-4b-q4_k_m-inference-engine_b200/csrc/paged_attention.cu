@@ -107,6 +107,14 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
+// The power of two, as two factors, that brings a row of largest magnitude
+// `most` to below 2^8 (any fp32 row then fits fp16 parts).
+__device__ __forceinline__ void row_scale(float most, float& f1, float& f2) {
+    const int e = min(max((int)(__float_as_uint(most) >> 23) - 126, -100), 127);  // most < 2^e
+    f1 = __uint_as_float((uint32_t)(127 + (8 - e) / 2) << 23);
+    f2 = __uint_as_float((uint32_t)(127 + (8 - e) - (8 - e) / 2) << 23);
+}
+
 template <Kind K, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
     paged_attention_tc_kernel(const __grid_constant__ PagedAttentionArgs a, const __grid_constant__ CUtensorMap kmap,
@@ -293,10 +301,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                         for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
                     }
-                    const int e = min(max((int)(__float_as_uint(most) >> 23) - 126, -100), 127);  // most < 2^e
-                    // 2^(8 - e) in two factors, since 2^-119 and 2^108 only fit together
-                    const float f1 = __uint_as_float((uint32_t)(127 + (8 - e) / 2) << 23);
-                    const float f2 = __uint_as_float((uint32_t)(127 + (8 - e) - (8 - e) / 2) << 23);
+                    float f1, f2;
+                    row_scale(most, f1, f2);
                     c = c / f1 / f2;
                     for (int i = 0; i < D / 8; ++i) {
                         float x[8];
@@ -483,6 +489,414 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
 }
 
+// ---------------------------------------------------------------------------
+// Few query rows per sequence and KV head (decode steps, draft tokens): the
+// keys and values are read once from HBM and that bounds the call. A producer
+// warp streams 64-key blocks (K and V) through a ring of shared memory; each
+// of kWarps warps takes every kWarps-th block by itself (mma.sync m16n8k16,
+// its own running maximum, sum and output), so no barrier stands in the loop,
+// and the warps are joined once per piece. kWarps divides the ring's stages:
+// all uses of a stage are one warp's, which therefore never waits on a stage
+// whose phase before its own is still another's. fp32 activations: queries and
+// probabilities as fp16 high and low parts, in rows 0-7 and 8-15 of one MMA
+// tile when 8 rows suffice, else in two MMAs.
+// ---------------------------------------------------------------------------
+constexpr int kDecodeKeys = 64;
+constexpr int kDecodeMinUnits = 4;
+
+template <Kind K, int D, int ROWS>
+struct DecodeLayout {
+    static constexpr int kHalf = kDecodeKeys * 128;  // 64 dims of a block
+    static constexpr int kMat = D / 64 * kHalf;
+    static constexpr int kStage = 2 * kMat;
+    static constexpr int kWarps = D == 64 || ROWS == 8 ? 6 : 5;
+    static constexpr int kStages = D == 64 ? 2 * kWarps : kWarps;
+    static constexpr int kThreads = (kWarps + 1) * 32;
+    static_assert(kStages % kWarps == 0, "a stage belongs to one warp");
+    static constexpr int kJoin = kStages * kStage;  // [kWarps][ROWS][D] floats, then (m, l)
+    static constexpr int kBars = kJoin + kWarps * ROWS * (D + 2) * 4;
+    static constexpr int kBytes = kBars + 512 + 1024;
+    static_assert(kBytes <= 227 * 1024, "shared memory of one CTA");
+};
+
+struct DecodeBars {
+    uint64_t full[12], empty[12];
+    int dead;
+    Share share;
+};
+static_assert(sizeof(DecodeBars) <= 512, "barrier area");
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+template <Kind K>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (K == Kind::kBf16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float quad_max(float v) {
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v + __shfl_xor_sync(0xffffffffu, v, 2);
+}
+
+template <Kind K, int D, int ROWS>
+__global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
+    paged_attention_decode_kernel(const __grid_constant__ PagedAttentionArgs a, const __grid_constant__ CUtensorMap kmap,
+                                  const __grid_constant__ CUtensorMap vmap, const Partials part) {
+    using L = DecodeLayout<K, D, ROWS>;
+    using Act = typename Types<K>::Act;
+    constexpr int kStages = L::kStages, kWarps = L::kWarps;
+    constexpr bool kStacked = ROWS == 8;           // fp32: low parts in rows 8-15
+    constexpr bool kSplit = K == Kind::kF32;
+    constexpr int kParts = kSplit && !kStacked ? 2 : 1;
+    static_assert(!kStacked || kSplit, "16-bit rows take all 16 MMA rows");
+    constexpr int kR = kStacked ? 1 : 2;  // query rows of a lane: g (and g + 8)
+
+    extern __shared__ uint8_t smem_dyn[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
+    DecodeBars& bar = *reinterpret_cast<DecodeBars*>(smem + L::kBars);
+    float* join_o = reinterpret_cast<float*>(smem + L::kJoin);
+    float2* join_ml = reinterpret_cast<float2*>(join_o + kWarps * ROWS * D);
+    volatile int* dead = &bar.dead;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int group = a.heads / a.cache.kv_heads;
+    const int held = a.batch.table_width << a.cache.page_shift;
+
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&bar.full[i], 1);
+            mbar_init(&bar.empty[i], 1);
+        }
+        bar.dead = 0;
+        mbar_fence_init();
+    }
+    plan_share<ROWS, kDecodeKeys>(a.batch, group, a.cache.kv_heads, a.window, held, kDecodeMinUnits,
+                                  reinterpret_cast<unsigned long long*>(smem), &bar.share);
+    fence_proxy_async();  // the plan's words, before the ring's copies land on them
+    __syncthreads();
+    Pieces<ROWS, kDecodeKeys> pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
+
+    if (warp == kWarps) {
+        // ---------------- TMA: a lane per (K or V, page, half)
+        const int box = min(a.cache.page_size, kDecodeKeys);
+        const int boxes = kDecodeKeys / box;
+        const int half = lane % (D / 64), kv = lane / (D / 64) & 1, page_in_block = lane / (D / 64 * 2);
+        const uint32_t box_bytes = (uint32_t)box * D * 2 * 2;
+        int n = 0;
+        bool ok = true;
+        for (; pc.valid() && ok; pc.next()) {
+            for (int i = 0; i < pc.count; ++i, ++n) {
+                const int key0 = pc.tile.key_begin + (pc.b + i) * kDecodeKeys;
+                const int live = min(max((pc.tile.key_end - key0 + box - 1) / box, 0), boxes);
+                int page = -1;
+                if (page_in_block < live)
+                    page = __ldg(a.batch.page_table + (size_t)pc.s * a.batch.table_stride +
+                                 ((key0 + page_in_block * box) >> a.cache.page_shift));
+                const int st = n % kStages;
+                ok = wait_or_dead(&bar.empty[st], ((n / kStages) & 1) ^ 1, dead);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) mbar_arrive_expect_tx(&bar.full[st], live * box_bytes);
+                __syncwarp();
+                if (page_in_block < live)
+                    tma_load_4d(smem + st * L::kStage + kv * L::kMat + half * L::kHalf + page_in_block * box * 128,
+                                kv ? &vmap : &kmap, half * 64, key0 & (a.cache.page_size - 1), pc.h, page,
+                                &bar.full[st]);
+            }
+        }
+        for (int i = max(n - kStages, 0); i < n; ++i)
+            mbar_wait_bounded(&bar.full[i % kStages], (i / kStages) & 1, nullptr, 0);
+        __syncwarp();
+    } else {
+        // ---------------- attention
+        const int g = lane >> 2, t = lane & 3;
+        int n0 = 0;  // ring number of the piece's first block
+        bool ok = true, left[2] = {false, false};
+        for (; pc.valid(); pc.next()) {
+            const Tile& tl = pc.tile;
+            // Q: MMA A fragments of every 16-dim step; rows g and g + 8
+            uint32_t qf[D / 16][kParts][4];
+            float c[kR], m[kR], l[kR];
+            int first[kR], last[kR];
+#pragma unroll
+            for (int y = 0; y < kR; ++y) {
+                const int row = g + 8 * y;
+                const bool live = row < tl.rows;
+                const int r = tl.row0 + (live ? row : 0);
+                const int token = r / group, head = pc.h * group + r % group;
+                const int position = pc.seq.position + token;
+                last[y] = live ? min(position, held - 1) : -1;
+                first[y] = a.window > 0 ? max(position - a.window + 1, 0) : 0;
+                c[y] = a.scale * kLog2e;
+                m[y] = -CUDART_INF_F;
+                l[y] = 0.0f;
+                const Act* q = static_cast<const Act*>(a.q) + ((size_t)pc.seq.first_row + token) * a.ld_q + (size_t)head * D;
+                if constexpr (kSplit) {
+                    float2 x[D / 16][2];
+                    float most = 0.0f;
+#pragma unroll
+                    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            x[s][e] = __ldg(reinterpret_cast<const float2*>(q + 16 * s + 8 * e + 2 * t));
+                            most = fmaxf(most, fmaxf(fabsf(x[s][e].x), fabsf(x[s][e].y)));
+                        }
+                    float f1, f2;
+                    row_scale(quad_max(most), f1, f2);
+                    c[y] = c[y] / f1 / f2;
+#pragma unroll
+                    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            uint32_t hi, lo;
+                            split2(x[s][e].x * f1 * f2, x[s][e].y * f1 * f2, hi, lo);
+                            if constexpr (kStacked) {
+                                qf[s][0][2 * e] = hi;
+                                qf[s][0][2 * e + 1] = lo;
+                            } else {
+                                qf[s][0][2 * e + y] = hi;
+                                qf[s][1][2 * e + y] = lo;
+                            }
+                        }
+                } else {
+#pragma unroll
+                    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            qf[s][0][2 * e + y] = __ldg(reinterpret_cast<const uint32_t*>(q + 16 * s + 8 * e + 2 * t));
+                }
+            }
+            float o[D / 8][4];
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+
+            // this warp's blocks of the piece
+            for (int i = (warp - n0 % kWarps + kWarps) % kWarps; i < pc.count && ok; i += kWarps) {
+                const int n = n0 + i, st = n % kStages;
+                ok = wait_or_dead(&bar.full[st], (n / kStages) & 1, dead);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                const int key0 = tl.key_begin + (pc.b + i) * kDecodeKeys;
+                const uint32_t kbase = smem_addr(smem + st * L::kStage), vbase = kbase + L::kMat;
+                const bool edge = key0 < tl.key_first || key0 + kDecodeKeys > tl.key_end;
+                if (edge) {
+                    // rows of V that no query row sees may hold anything (or
+                    // were never loaded): zeros, since 0 times them is not 0
+                    uint8_t* v = smem + st * L::kStage + L::kMat;
+                    for (int row = lane; row < kDecodeKeys; row += 32)
+                        if (key0 + row < tl.key_first || key0 + row >= tl.key_end)
+#pragma unroll
+                            for (int j = 0; j < D / 8; ++j)
+                                *reinterpret_cast<uint4*>(v + (j >> 3) * L::kHalf + swz128(row, j & 7)) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                    __syncwarp();
+                }
+                // S = Q K^T: scores of 8 keys at a time
+                float s[kDecodeKeys / 8][2 * kR];
+#pragma unroll
+                for (int j = 0; j < kDecodeKeys / 8; ++j) {
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int d = 0; d < D / 16; d += 2) {
+                        uint32_t b[4];
+                        const int chunk = 2 * d + (lane >> 3);
+                        ldsm_x4(kbase + (chunk >> 3) * L::kHalf + swz128(8 * j + (lane & 7), chunk & 7), b);
+#pragma unroll
+                        for (int p = 0; p < kParts; ++p) {
+                            mma16816<K>(acc, qf[d][p], b[0], b[1]);
+                            mma16816<K>(acc, qf[d + 1][p], b[2], b[3]);
+                        }
+                    }
+                    if constexpr (kStacked) {
+                        s[j][0] = acc[0] + acc[2];
+                        s[j][1] = acc[1] + acc[3];
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[j][e] = acc[e];
+                    }
+                }
+                float top[kR];
+#pragma unroll
+                for (int y = 0; y < kR; ++y) {
+                    const int lo = first[y] - key0 - 2 * t, hi = last[y] - key0 - 2 * t;
+                    if (__any_sync(0xffffffffu, first[y] > key0 || last[y] < key0 + kDecodeKeys - 1)) {
+#pragma unroll
+                        for (int j = 0; j < kDecodeKeys / 8; ++j)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                if (8 * j + e < lo || 8 * j + e > hi) s[j][2 * y + e] = -CUDART_INF_F;
+                    }
+                    float mx = -CUDART_INF_F;
+#pragma unroll
+                    for (int j = 0; j < kDecodeKeys / 8; ++j) mx = fmaxf(mx, fmaxf(s[j][2 * y], s[j][2 * y + 1]));
+                    top[y] = quad_max(mx) * c[y];
+                }
+                bool moves = false;
+#pragma unroll
+                for (int y = 0; y < kR; ++y) moves |= top[y] > m[y] + kLazy;
+                if (__any_sync(0xffffffffu, moves)) {
+                    float f[kR];
+#pragma unroll
+                    for (int y = 0; y < kR; ++y) {
+                        const float mn = top[y] > m[y] + kLazy ? top[y] : m[y];
+                        f[y] = mn == m[y] ? 1.0f : exp2_fast(m[y] - mn);
+                        l[y] *= f[y];
+                        m[y] = mn;
+                    }
+#pragma unroll
+                    for (int j = 0; j < D / 8; ++j) {
+                        o[j][0] *= f[0];
+                        o[j][1] *= f[0];
+                        o[j][2] *= f[kR - 1];
+                        o[j][3] *= f[kR - 1];
+                    }
+                }
+                // probabilities, straight into the A fragments of P V
+                uint32_t pf[kDecodeKeys / 16][kParts][4];
+#pragma unroll
+                for (int y = 0; y < kR; ++y) {
+                    const float shift = m[y] == -CUDART_INF_F ? 0.0f : m[y] - kBias<K>;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < kDecodeKeys / 8; ++j) {
+                        const float p0 = exp2_fast(fmaf(s[j][2 * y], c[y], -shift));
+                        const float p1 = exp2_fast(fmaf(s[j][2 * y + 1], c[y], -shift));
+                        sum += p0 + p1;
+                        // keys 8j .. of step j / 2: fragment words 0, 1 (low half of 16 keys) or 2, 3
+                        const int w = 2 * (j & 1);
+                        if constexpr (kSplit) {
+                            uint32_t hi, lo;
+                            split2(p0, p1, hi, lo);
+                            if constexpr (kStacked) {
+                                pf[j / 2][0][w] = hi;
+                                pf[j / 2][0][w + 1] = lo;
+                            } else {
+                                pf[j / 2][0][w + y] = hi;
+                                pf[j / 2][1][w + y] = lo;
+                            }
+                        } else {
+                            pf[j / 2][0][w + y] = pack2<K>(p0, p1);
+                        }
+                    }
+                    l[y] += sum;  // this lane's keys; the quad's are added at the end
+                }
+                // O += P V, 16 keys at a time
+#pragma unroll
+                for (int kk = 0; kk < kDecodeKeys / 16; ++kk)
+#pragma unroll
+                    for (int j = 0; j < D / 8; j += 2) {
+                        uint32_t b[4];
+                        const int row = 16 * kk + (lane & 15), chunk = j + (lane >> 4);
+                        ldsm_x4_t(vbase + (chunk >> 3) * L::kHalf + swz128(row, chunk & 7), b);
+#pragma unroll
+                        for (int p = 0; p < kParts; ++p) {
+                            mma16816<K>(o[j], pf[kk][p], b[0], b[1]);
+                            mma16816<K>(o[j + 1], pf[kk][p], b[2], b[3]);
+                        }
+                    }
+                if (edge) fence_proxy_async();  // the zeros, before the next copy into this stage
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.empty[st]);
+            }
+            n0 += pc.count;
+
+            // join the warps
+#pragma unroll
+            for (int y = 0; y < kR; ++y) {
+                const int row = g + 8 * y;
+                l[y] = quad_sum(l[y]);
+                float* dst = join_o + (warp * ROWS + row) * D + 2 * t;
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) {
+                    float2 v;
+                    if constexpr (kStacked)
+                        v = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
+                    else
+                        v = make_float2(o[j][2 * y], o[j][2 * y + 1]);
+                    *reinterpret_cast<float2*>(dst + 8 * j) = v;
+                }
+                if (t == 0) join_ml[warp * ROWS + row] = make_float2(m[y], l[y]);
+            }
+            if (named_barrier_or(1, kWarps * 32, !ok)) {
+                ok = false;
+                break;
+            }
+            const bool whole = pc.whole();
+            const size_t slot = ((size_t)blockIdx.x * 2 + (pc.index > 0)) * ROWS;
+            for (int x = tid; x < tl.rows * (D / 4); x += kWarps * 32) {
+                const int row = x / (D / 4), d = x % (D / 4) * 4;
+                float mx = -CUDART_INF_F;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, join_ml[w * ROWS + row].x);
+                float sum = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float2 ml = join_ml[w * ROWS + row];
+                    if (!(ml.y != 0.0f)) continue;
+                    const float f = exp2_fast(ml.x - mx);
+                    const float4 u = *reinterpret_cast<const float4*>(join_o + (w * ROWS + row) * D + d);
+                    sum += f * ml.y;
+                    v[0] += f * u.x;
+                    v[1] += f * u.y;
+                    v[2] += f * u.z;
+                    v[3] += f * u.w;
+                }
+                const int r = tl.row0 + row;
+                const int head = pc.h * group + r % group;
+                const size_t out_row = (size_t)pc.seq.first_row + r / group;
+                if (whole) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = sum != 0.0f ? v[e] / sum : 0.0f;
+                    store_values<Act, 4>(static_cast<Act*>(a.out) + out_row * a.ld_out + (size_t)head * D + d, v);
+                    if (d == 0 && a.lse)
+                        a.lse[out_row * a.heads + head] = sum != 0.0f ? (mx - kBias<K> + log2f(sum)) * kLn2 : -CUDART_INF_F;
+                } else {
+                    store_values<float, 4>(part.o + (slot + row) * D + d, v);
+                    if (d == 0) part.ml[slot + row] = make_float2(mx - kBias<K>, sum);
+                }
+            }
+            if (!whole) {
+                left[pc.index > 0] = true;
+                if (tid == 0)
+                    part.notes[blockIdx.x * 2 + (pc.index > 0)] = {pc.s, pc.h, pc.r, pc.b, pc.count, tl.blocks};
+            }
+            named_barrier(1, kWarps * 32);  // the join area may be written again
+        }
+        if (tid == 0)
+            for (int i = 0; i < 2; ++i)
+                if (!left[i]) part.notes[blockIdx.x * 2 + i] = {0, 0, 0, 0, 0, 0};
+    }
+    pdl_launch_dependents();
+}
+
 // The tiles that several CTAs share: CTA c's block of this grid joins the
 // tile that begins in c's share and ends in a later one's, in the order of
 // the CTAs. One warp per query row.
@@ -592,16 +1006,51 @@ cudaError_t launch_tc(const PagedAttentionArgs& a, cudaStream_t s) {
                       dim3(128), 0, s, a, part, 32);
 }
 
+template <Kind K, int D, int ROWS>
+cudaError_t launch_decode(const PagedAttentionArgs& a, cudaStream_t s) {
+    using L = DecodeLayout<K, D, ROWS>;
+    auto kernel = paged_attention_decode_kernel<K, D, ROWS>;
+    static std::once_flag once;
+    static cudaError_t attr = cudaSuccess;
+    std::call_once(once, [&] {
+        attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+    });
+    if (attr != cudaSuccess) return attr;
+    CUtensorMap km, vm;
+    if (!page_map(a.cache, a.cache.k, kDecodeKeys, &km) || !page_map(a.cache, a.cache.v, kDecodeKeys, &vm))
+        return cudaErrorInvalidValue;
+    const int ctas = sm_count();
+    const Partials part = partials(a.workspace, ctas, ROWS);
+    kernel<<<ctas, L::kThreads, L::kBytes, s>>>(a, km, vm, part);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    return launch_pdl(paged_attention_join_kernel<typename Types<K>::Act, D, ROWS>, dim3(ctas, 1), dim3(128), 0, s, a,
+                      part, ROWS);
+}
+
+// Query rows per sequence and KV head up to which the decode kernel is used:
+// its 16 MMA rows.
+constexpr int kDecodeRows = 16;
+
+template <Kind K, int D>
+cudaError_t launch_dim(const PagedAttentionArgs& a, cudaStream_t s) {
+    const long long rows = (long long)a.batch.max_new * (a.heads / a.cache.kv_heads);
+    if (rows > kDecodeRows) return launch_tc<K, D>(a, s);
+    if constexpr (K == Kind::kF32)
+        if (rows <= 8) return launch_decode<K, D, 8>(a, s);
+    return launch_decode<K, D, 16>(a, s);
+}
+
 template <Kind K>
 cudaError_t launch(const PagedAttentionArgs& a, cudaStream_t s) {
-    return a.cache.head_dim == 128 ? launch_tc<K, 128>(a, s) : launch_tc<K, 64>(a, s);
+    return a.cache.head_dim == 128 ? launch_dim<K, 128>(a, s) : launch_dim<K, 64>(a, s);
 }
 
 }  // namespace
 
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim, int max_new) {
-    (void)heads, (void)kv_heads, (void)max_new;
-    return partial_bytes(sm_count(), kTileRows, head_dim);
+    const bool few = max_new > 0 && (long long)max_new * (heads / kv_heads) <= kDecodeRows;
+    return partial_bytes(sm_count(), few ? kDecodeRows : kTileRows, head_dim);
 }
 
 cudaError_t paged_attention(const PagedAttentionArgs& a, cudaStream_t s) {
