@@ -138,7 +138,10 @@ void launch(const PagedAppendArgs& a, const Frequencies& f, dim3 grid, cudaStrea
 cudaError_t paged_append(const PagedAppendArgs& a, cudaStream_t s) {
     const int d = a.cache.head_dim, half = d / 2;
     Frequencies f = {};
-    for (int j = 0; j < half; ++j) f.turns[j] = std::pow(a.rope_base, -2.0 * j / d) / 6.283185307179586476925;
+    // powers by products: 64 roundings of 2^-53 are 1e-7 of a turn at position 2^30
+    const double ratio = std::pow(a.rope_base, -2.0 / d);
+    f.turns[0] = 1.0 / 6.283185307179586476925;
+    for (int j = 1; j < half; ++j) f.turns[j] = f.turns[j - 1] * ratio;
     const int rows = a.heads + 2 * a.cache.kv_heads;
     const int held = kAppendThreads / (half / (a.f32 ? 4 : 8));
     const dim3 grid(a.batch.tokens, (rows + held - 1) / held);

@@ -475,46 +475,47 @@ class Engine:
 
 
 # ------------------------------------- paged KV cache and sampling (torch tensors)
-def _torch_type(dtype) -> int:
-    import torch
-
-    types = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    if dtype not in types:
-        raise InvalidArgument(EINVAL, f"unsupported tensor type {dtype}")
-    return types[dtype]
+# These calls are a few microseconds of GPU work at their smallest, so their
+# checks read each tensor's attributes once and make no objects on the way.
+_torch = None
+_TYPE_OF: dict = {}  # torch dtype -> type id
 
 
-def _on_device(t, what: str, dtype=None, device=None):
-    """t, checked to be a CUDA tensor (of dtype, on device)."""
-    if not t.is_cuda or (device is not None and t.device != device):
-        raise InvalidArgument(EINVAL, f"{what} must be on {device if device is not None else 'a CUDA device'}")
-    if dtype is not None and t.dtype != dtype:
-        raise InvalidArgument(EINVAL, f"{what} must be {dtype}")
-    return t
-
-
-class _on:
-    """The call's device made current, and its stream: `stream`, or torch's
-    current one there."""
-
-    def __init__(self, device, stream):
+def _load_torch():
+    global _torch
+    if _torch is None:
         import torch
 
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-        self.device, self.stream = device, stream
+        _TYPE_OF.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+        _torch = torch
+    return _torch
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        if self.stream is not None:
-            return stream_ptr(self.stream)
-        import torch
 
-        return torch.cuda.current_stream(self.device).cuda_stream
+def _refuse(message: str):
+    raise InvalidArgument(EINVAL, message)
 
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+
+def _type_of(dtype) -> int:
+    code = _TYPE_OF.get(dtype)
+    if code is None:
+        _refuse(f"unsupported tensor type {dtype}")
+    return code
+
+
+def _call(index: int, fn, *args):
+    """fn(*args) with device `index` current."""
+    if _torch._C._cuda_getDevice() == index:
+        status = fn(*args)
+    else:
+        with _torch.cuda.device(index):
+            status = fn(*args)
+    if status != OK:
+        check(status)
+
+
+def _stream_of(stream, index: int):
+    """`stream`, or torch's current one on device `index`."""
+    return stream_ptr(stream) if stream is not None else _torch._C._cuda_getCurrentRawStream(index)
 
 
 class PagedKV:
@@ -524,16 +525,20 @@ class PagedKV:
     [head_dim] cache is passed as its transpose(1, 2)."""
 
     def __init__(self, k, v):
-        if k.dim() != 4 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(3) != 1:
-            raise InvalidArgument(EINVAL, "k and v must be alike, [pages][kv_heads][page_size][head_dim]")
-        _on_device(k, "k")
-        _on_device(v, "v", device=k.device)
-        self.k, self.v = k, v
-        pages, heads, rows, d = k.shape
+        _load_torch()
         s = k.stride()
+        if k.dim() != 4 or k.shape != v.shape or s != v.stride() or k.dtype != v.dtype or s[3] != 1:
+            _refuse("k and v must be alike, [pages][kv_heads][page_size][head_dim]")
+        self.index = k.get_device()
+        if self.index < 0 or v.get_device() != self.index:
+            _refuse("k and v must be on one CUDA device")
+        self.k, self.v = k, v
+        pages, self.heads, rows, d = k.shape
+        self.head_dim = d
         # a dimension of one element has no stride of its own
-        self.c = _PagedKV(k.data_ptr(), v.data_ptr(), _torch_type(k.dtype), heads, d, rows, pages,
-                          s[0] if pages > 1 else max(s[0], d), s[1] if heads > 1 else max(s[1], d), s[2])
+        self.c = _PagedKV(k.data_ptr(), v.data_ptr(), _type_of(k.dtype), self.heads, d, rows, pages,
+                          s[0] if pages > 1 else max(s[0], d), s[1] if self.heads > 1 else max(s[1], d), s[2])
+        self.ref = C.byref(self.c)
 
 
 class PagedBatch:
@@ -542,40 +547,46 @@ class PagedBatch:
     tokens of any one sequence (1 for a decode step; 0: unknown)."""
 
     def __init__(self, q_start, kv_len, page_table, max_new: int = 0):
-        import torch
-
-        n = kv_len.numel()
-        for t, what in ((q_start, "q_start"), (kv_len, "kv_len"), (page_table, "page_table")):
-            _on_device(t, what, torch.int32, kv_len.device)
-        if (q_start.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n or not q_start.is_contiguous()
-                or not kv_len.is_contiguous() or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
-            raise InvalidArgument(EINVAL, "q_start [n + 1], kv_len [n] and page_table [n][width] do not fit together")
-        self.tensors = (q_start, kv_len, page_table)
+        int32 = _load_torch().int32
+        self.index = index = kv_len.get_device()
+        if index < 0 or q_start.get_device() != index or page_table.get_device() != index:
+            _refuse("q_start, kv_len and page_table must be on one CUDA device")
+        n, s = kv_len.numel(), page_table.stride()
+        if (q_start.dtype is not int32 or kv_len.dtype is not int32 or page_table.dtype is not int32
+                or q_start.numel() != n + 1 or len(s) != 2 or page_table.shape[0] != n
+                or not q_start.is_contiguous() or not kv_len.is_contiguous()):
+            _refuse("q_start [n + 1], kv_len [n] and page_table [n][width] must be int32 and fit together")
         width = page_table.shape[1]
+        if width > 1 and s[1] != 1:
+            _refuse("page_table rows must be contiguous")
+        self.tensors = (q_start, kv_len, page_table)
+        self.max_new = max_new
         self.c = _PagedBatch(n, max_new, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
-                             max(page_table.stride(0), width) if n > 1 else width, width)
+                             max(s[0], width) if n > 1 else width, width)
+        self.ref = C.byref(self.c)
 
 
-def _token_rows(t, what: str, heads: int | None, head_dim: int, like=None):
-    """(address, elements between token rows) of a [tokens][heads][head_dim] tensor."""
-    if (t.dim() != 3 or t.shape[2] != head_dim or t.stride(2) != 1 or (heads is not None and t.shape[1] != heads)
-            or (t.shape[1] > 1 and t.stride(1) != head_dim)):
-        raise InvalidArgument(EINVAL, f"{what} must be [tokens][heads][head_dim] with contiguous heads")
-    if like is not None:
-        _on_device(t, what, like.dtype, like.device)
-        if t.shape[0] != like.shape[0]:
-            raise InvalidArgument(EINVAL, f"{what} must have as many rows as the others")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1] * head_dim
+def _token_rows(t, what: str, head_dim: int, index: int, like=None, heads: int = 0) -> int:
+    """Elements between the token rows of t, a [tokens][heads][head_dim] tensor
+    on device `index` with contiguous heads (of like's type and row count)."""
+    shape, s = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != head_dim or s[2] != 1 or (shape[1] > 1 and s[1] != head_dim):
+        _refuse(f"{what} must be [tokens][heads][head_dim] with contiguous heads")
+    if heads and shape[1] != heads:
+        _refuse(f"{what} must have {heads} heads")
+    if t.get_device() != index:
+        _refuse(f"{what} must be on the cache's device")
+    if like is not None and (shape[0] != like.shape[0] or t.dtype is not like.dtype):
+        _refuse(f"{what} must have the others' type and number of rows")
+    return s[0] if shape[0] > 1 else shape[1] * head_dim
 
 
-def _floats(t, what: str, n: int, device, dtype=None):
-    import torch
-
+def _values(t, what: str, n: int, index: int, dtype):
+    """Address of n contiguous values (None passes through)."""
     if t is None:
         return None
-    _on_device(t, what, dtype or torch.float32, device)
-    if t.numel() != n or not t.is_contiguous():
-        raise InvalidArgument(EINVAL, f"{what} must hold {n} values")
+    if t.dtype is not dtype or t.numel() != n or t.get_device() != index or not t.is_contiguous():
+        _refuse(f"{what} must hold {n} contiguous {dtype} values on the call's device")
     return t.data_ptr()
 
 
@@ -585,28 +596,29 @@ def paged_append(cache: PagedKV, batch: PagedBatch, k, v, q=None, q_out=None, q_
     (q4k_paged_append). k, v: [tokens][kv_heads][head_dim]; q (optional):
     [tokens][heads][head_dim]. Returns the rotated queries (q_out, allocated
     like q if not given), or None without q."""
-    import torch
-
-    d, device = cache.c.head_dim, cache.k.device
-    _on_device(k, "k", device=device)
-    _on_device(batch.tensors[0], "the batch", device=device)
-    pk, lk = _token_rows(k, "k", cache.c.kv_heads, d)
-    pv, lv = _token_rows(v, "v", cache.c.kv_heads, d, k)
+    d, index, f32 = cache.head_dim, cache.index, _torch.float32
+    if batch.index != index:
+        _refuse("the batch must be on the cache's device")
+    lk = _token_rows(k, "k", d, index, None, cache.heads)
+    lv = _token_rows(v, "v", d, index, k, cache.heads)
     pq = po = None
     lq = lo = heads = 0
     if q is not None:
+        lq = _token_rows(q, "q", d, index, k)
         heads = q.shape[1]
         if q_out is None:
-            q_out = torch.empty((q.shape[0], heads, d), dtype=q.dtype, device=device)
-        pq, lq = _token_rows(q, "q", None, d, k)
-        po, lo = _token_rows(q_out, "q_out", heads, d, k)
+            q_out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lo = _token_rows(q_out, "q_out", d, index, k, heads)
+        pq, po = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
-        raise InvalidArgument(EINVAL, "q and q_out go together")
-    qg, kg = _floats(q_gamma, "q_gamma", d, device), _floats(k_gamma, "k_gamma", d, device)
-    with _on(device, stream) as s:
-        check(lib().q4k_paged_append(C.byref(cache.c), C.byref(batch.c), k.shape[0], _torch_type(k.dtype), pq, lq, heads,
-                                     pk, lk, pv, lv, qg, kg, epsilon, rope_base, po, lo, s))
+        _refuse("q and q_out go together")
+    _call(index, lib().q4k_paged_append, cache.ref, batch.ref, k.shape[0], _type_of(k.dtype), pq, lq, heads,
+          k.data_ptr(), lk, v.data_ptr(), lv, _values(q_gamma, "q_gamma", d, index, f32),
+          _values(k_gamma, "k_gamma", d, index, f32), epsilon, rope_base, po, lo, _stream_of(stream, index))
     return q_out
+
+
+_workspace_bytes: dict = {}
 
 
 def paged_attention(cache: PagedKV, batch: PagedBatch, q, out=None, lse=None, scale: float = 0.0, window: int = 0,
@@ -615,28 +627,34 @@ def paged_attention(cache: PagedKV, batch: PagedBatch, q, out=None, lse=None, sc
     (q4k_paged_attention). Returns out (allocated like q if not given); lse
     ([tokens][heads] fp32) is filled if given. The workspace comes from torch's
     allocator, on its current stream, unless given (uint8)."""
-    import torch
-
-    d, device = cache.c.head_dim, cache.k.device
-    _on_device(q, "q", device=device)
-    _on_device(batch.tensors[0], "the batch", device=device)
-    pq, lq = _token_rows(q, "q", None, d)
+    d, index = cache.head_dim, cache.index
+    if batch.index != index:
+        _refuse("the batch must be on the cache's device")
+    lq = _token_rows(q, "q", d, index)
     tokens, heads = q.shape[0], q.shape[1]
     if out is None:
-        out = torch.empty((tokens, heads, d), dtype=q.dtype, device=device)
-    po, lo = _token_rows(out, "out", heads, d, q)
-    pl = _floats(lse, "lse", tokens * heads, device)
-    with _on(device, stream) as s:
-        need = lib().q4k_paged_attention_workspace_bytes(heads, cache.c.kv_heads, d, batch.c.max_new)
-        if workspace is None and need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=device)
-            if stream is not None:
-                # memory of torch's current stream, used on the caller's
-                handle = torch.cuda.ExternalStream(s, device=device) if s else torch.cuda.default_stream(device)
-                workspace.record_stream(handle)
-        size = 0 if workspace is None else workspace.numel() * workspace.element_size()
-        check(lib().q4k_paged_attention(C.byref(cache.c), C.byref(batch.c), tokens, _torch_type(q.dtype), pq, lq, heads,
-                                        scale, window, po, lo, pl, ptr(workspace), size, s))
+        out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lo = _token_rows(out, "out", d, index, q, heads)
+    pl = _values(lse, "lse", tokens * heads, index, _torch.float32)
+    s = _stream_of(stream, index)
+    if workspace is None:
+        key = (heads, cache.heads, d, batch.max_new, index)
+        size = _workspace_bytes.get(key)
+        if size is None:
+            with _torch.cuda.device(index):
+                size = _workspace_bytes[key] = lib().q4k_paged_attention_workspace_bytes(heads, cache.heads, d,
+                                                                                         batch.max_new)
+        workspace = _torch.empty(size, dtype=_torch.uint8, device=q.device)
+        if stream is not None:
+            # memory of torch's current stream, used on the caller's
+            workspace.record_stream(_torch.cuda.ExternalStream(s, device=index) if s
+                                    else _torch.cuda.default_stream(index))
+    else:
+        if workspace.get_device() != index or not workspace.is_contiguous():
+            _refuse("the workspace must be contiguous, on the cache's device")
+        size = workspace.numel() * workspace.element_size()
+    _call(index, lib().q4k_paged_attention, cache.ref, batch.ref, tokens, _type_of(q.dtype), q.data_ptr(), lq, heads,
+          scale, window, out.data_ptr(), lo, pl, workspace.data_ptr(), size, s)
     return out
 
 
@@ -645,23 +663,24 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
     """One token per row of logits [rows][vocab] (q4k_sample); uniform,
     temperature, top_p, min_p: [rows] fp32, top_k: [rows] int32, on the device.
     Returns (tokens int32, logprob fp32), allocated if not given."""
-    import torch
-
-    if logits.dim() != 2 or logits.stride(1) != 1:
-        raise InvalidArgument(EINVAL, "logits must be [rows][vocab] with contiguous rows")
+    torch = _torch or _load_torch()
+    s = logits.stride()
+    if len(s) != 2 or s[1] != 1:
+        _refuse("logits must be [rows][vocab] with contiguous rows")
+    index = logits.get_device()
+    if index < 0:
+        _refuse("logits must be on a CUDA device")
     rows, vocab = logits.shape
-    device = _on_device(logits, "logits").device
+    f32, i32 = torch.float32, torch.int32
     if tokens is None:
-        tokens = torch.empty(rows, dtype=torch.int32, device=device)
+        tokens = torch.empty(rows, dtype=i32, device=logits.device)
     if logprob is None:
-        logprob = torch.empty(rows, dtype=torch.float32, device=device)
-    args = [_floats(temperature, "temperature", rows, device), _floats(top_k, "top_k", rows, device, torch.int32),
-            _floats(top_p, "top_p", rows, device), _floats(min_p, "min_p", rows, device),
-            _floats(uniform, "uniform", rows, device), _floats(tokens, "tokens", rows, device, torch.int32),
-            _floats(logprob, "logprob", rows, device)]
-    with _on(device, stream) as s:
-        check(lib().q4k_sample(logits.data_ptr(), _torch_type(logits.dtype), logits.stride(0) if rows > 1 else vocab,
-                               rows, vocab, *args, s))
+        logprob = torch.empty(rows, dtype=f32, device=logits.device)
+    _call(index, lib().q4k_sample, logits.data_ptr(), _type_of(logits.dtype), s[0] if rows > 1 else vocab, rows, vocab,
+          _values(temperature, "temperature", rows, index, f32), _values(top_k, "top_k", rows, index, i32),
+          _values(top_p, "top_p", rows, index, f32), _values(min_p, "min_p", rows, index, f32),
+          _values(uniform, "uniform", rows, index, f32), _values(tokens, "tokens", rows, index, i32),
+          _values(logprob, "logprob", rows, index, f32), _stream_of(stream, index))
     return tokens, logprob
 
 
