@@ -8,16 +8,20 @@
 // Weights are whole numbers, round(w 2^S), so that every sum is exact: it
 // does not depend on the order of atomics or on how a row is cut, and two
 // calls (or two launch shapes) give the same token. S leaves room for a
-// vocabulary of ones in 62 bits (44 for 2^18 tokens); a weight's rounding,
+// vocabulary of ones in 62 bits (44 up to 2^18 tokens); a weight's rounding,
 // 2^-(S+1) of the largest, moves the draw's boundaries by about 1e-12.
 //
 // No sorting: a row's threshold is found by histograms. A cluster of 1 to 16
 // CTAs holds the row in shared memory, each CTA a slice, so that the logits
-// are read from HBM once; the passes over them (maximum, 2048 equal bins of
-// the distance to the maximum, 2048 bins of the bin where the running total
-// passes, the draw) run from there, and only bins and totals cross the
-// cluster. Equal keys in the last bin end the search; otherwise (values
-// closer than 2^-22 of the range) their bits are gone through, 11 at a time.
+// are read from HBM once; the passes over them run from there, and only bins,
+// totals and candidates cross the cluster. The first pass takes the maximum,
+// the second 2048 equal bins of the distance to it: of counts (top-k) or of
+// weights (top-p). The tokens down to the bin where the running total reaches
+// what is wanted are the candidates. Up to kList of them (the usual case) are
+// brought to one CTA, which ranks them by comparing all with all, applies the
+// filters in turn and draws. More of them stay where they are: the bin is cut
+// into 2048 again, then by the keys' bits, 11 at a time, until equal logits
+// are left, of which the lowest indexes are kept.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -36,14 +40,14 @@ constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 16;
-constexpr int kVec = 4;                               // consecutive logits of a thread
-constexpr int kStride = kSampleThreads * kVec;        // logits of one step of the CTA
-// Logits of one CTA: 80 KB of them, so that two CTAs fit an SM; 25000 fp32 ones
-// of a vocabulary of 400000 in 16 CTAs (one to an SM).
+constexpr int kVec = 4;  // consecutive logits of a lane
+constexpr int kStep = 32 * kVec;
+constexpr int kList = kSampleThreads;
+// Logits of one CTA: 80 KB of them, so that two CTAs fit an SM; 25088 fp32
+// ones of a vocabulary of 400000 in 16 CTAs (one to an SM).
 constexpr int kSliceBytes = 80 * 1024;
 template <typename T>
 constexpr int kMaxSlice = kSliceBytes / sizeof(T) > 25600 ? kSliceBytes / sizeof(T) : 25600;
-constexpr int kMaxSteps = (kMaxSlice<uint16_t> + kStride - 1) / kStride;
 constexpr int kTable = 64;
 
 // Whole numbers in the order of the floats.
@@ -56,56 +60,49 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
 }
 
 struct Crossing {
-    u64 above, inside;  // the total above the bin, and in it
+    u64 above, inside, all;  // the total above the bin, in it, and of every bin
     int bin;
 };
 
 struct alignas(16) SampleShared {
     uint32_t lo[kBins], hi[kBins];  // a histogram of 64-bit sums
+    u64 list_key[kList];            // candidates: key, then the complement of the index
+    u64 list_w[kList];
     double table[kTable];           // 2^(j/64)
-    u64 chunk[kMaxSteps * kSampleWarps];
     u64 warp_sum[kSampleWarps];
     u64 total[kMaxCluster];  // one word from every CTA of the cluster
     float bound[2][kMaxCluster];
     Crossing crossing;
-    int place;
+    int place, listed;
 };
 
-// w(l) = round(2^(S + (l - top) log2(e) / T)). The exponent t is taken as a
-// sum of two floats (the subtraction's and the product's own roundings kept),
-// 2^-46 of it; 2^frac(t) is 2^(j/64) times a Taylor polynomial in fp64 where w
-// needs the bits, ex2.approx (2^-22) below 2^-26, where 2^-48 of the largest
-// weight is all that is lost.
+// w(l) = round(2^(S + t)), t = (l - top) log2(e) / T, in fp64: l - top is exact,
+// 64 t = i + r with i whole, 2^t = 2^(i/64) (the table, its exponent moved) times
+// the Taylor polynomial of e^(r ln 2 / 64), |r| <= 1/2, whose fifth term is below
+// 4e-14. Whole numbers are split off by adding 1.5 2^52 and w is read from the
+// mantissa after adding 2^52 (w < 2^45): conversion instructions would cost
+// more than all the arithmetic.
 struct Weights {
-    float top, c_hi, c_lo, cutoff;
+    float top, c, cutoff;
+    double top64, c64;  // 64 log2(e) / T
     int S;
     const double* table;
 
     __device__ __forceinline__ u64 operator()(float l) const {
-        if (l == top) return 1ull << S;
-        const float d = l - top, bb = d - l;
-        const float err = (l - (d - bb)) - (top + bb);
-        const float t = d * c_hi;
-        if (!(t > cutoff)) return 0;
-        const float t_lo = fmaf(d, c_hi, -t) + fmaf(d, c_lo, err * c_hi);
-        const float n = rintf(t), f = t - n;
-        if (t < -26.0f) {
-            float p;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(f + t_lo));
-            return __float2ull_rn(p * __uint_as_float((uint32_t)(127 + (int)n + S) << 23));
-        }
-        // f = j / 64 + r
-        const float j = rintf(f * 64.0f);
-        const double r = ((double)fmaf(j, -1.0f / 64.0f, f) + (double)t_lo) * 0.693147180559945309417;
-        const int ji = (int)j;
-        double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-        p = fma(p, r, 1.0 / 6.0);
-        p = fma(p, r, 0.5);
+        if (!((l - top) * c > cutoff)) return l == top ? 1ull << S : 0;  // top itself where inf - inf or 0 inf is NaN
+        constexpr double kWhole = 6755399441055744.0;  // 1.5 2^52
+        const double d = (double)l - top64;
+        const double z = fma(d, c64, kWhole);
+        const double r = fma(d, c64, kWhole - z);
+        constexpr double k = 0.693147180559945309417 / 64.0;
+        double p = fma(r, k * k * k * k / 24.0, k * k * k / 6.0);
+        p = fma(p, r, k * k / 2.0);
+        p = fma(p, r, k);
         p = fma(p, r, 1.0);
-        p = fma(p, r, 1.0);
-        const int e = (int)n + S + (ji >> 6);  // ji in [-32, 32]
-        const double scale = __hiloint2double((1023 + e) << 20, 0);
-        return (u64)__double2ll_rn(p * table[ji & 63] * scale);
+        const int i = __double2loint(z);
+        const double v = table[i & 63];
+        const double w = p * __hiloint2double(__double2hiint(v) + (((i >> 6) + S) << 20), __double2loint(v));
+        return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
     }
 };
 
@@ -119,9 +116,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int row = blockIdx.x / ranks;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int base = min(rank * slice, a.vocab);         // this CTA's logits: base .. base + count - 1
+    const int base = min(rank * slice, a.vocab);  // this CTA's logits: base .. base + count - 1
     const int count = min(slice, a.vocab - base);
-    const int steps = (count + kStride - 1) / kStride;
     const T* src = static_cast<const T*>(a.logits) + row * a.ld + base;
 
     if (tid < kTable) sh.table[tid] = exp2(tid / 64.0);
@@ -149,8 +145,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
             most = fmaxf(most, to_float<T>(v));
         }
     }
-    // what lies behind the slice, up to a whole step, is never drawn
-    for (int i = count + tid; i < steps * kStride; i += kSampleThreads) held[i] = from_float<T>(-CUDART_INF_F);
+    // what lies behind the vocabulary is never drawn
+    for (int i = count + tid; i < slice; i += kSampleThreads) held[i] = from_float<T>(-CUDART_INF_F);
 
     // The largest and smallest of a value over the cluster.
     auto cluster_bounds = [&](float high, float low) {
@@ -180,25 +176,26 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     const float temperature = a.temperature ? a.temperature[row] : 1.0f;
     const bool greedy = !(temperature > 0.0f);
     const double c = 1.44269504088896340736 / (double)(greedy ? 1.0f : temperature);
-    const float c_hi = (float)c;
-    const Weights weight = {top, c_hi, (float)(c - (double)c_hi), -(float)S - 1.0f, S, sh.table};
+    const Weights weight = {top, (float)c, -(float)S - 1.0f, (double)top, 64.0 * c, S, sh.table};
 
     // kept: logits above cut, and those equal to it up to index cut_index
     float cut = -CUDART_INF_F;
     int cut_index = -1;
     auto kept = [&](float l, int i) { return l > cut || (l == cut && i <= cut_index); };
 
-    // f(logit, index) for all of the CTA's logits, four at a time
+    // f(logit, index) for all of the CTA's logits, four at a time; a warp's are
+    // consecutive, so that its sums are of one stretch of the index order
+    const int stretch = slice / kSampleWarps;  // a multiple of kVec
     auto for_each = [&](auto&& f) {
-        for (int s = 0; s < steps; ++s) {
-            const int at = s * kStride + tid * kVec;
+        for (int s = lane * kVec; s < stretch; s += kStep) {
+            const int at = warp * stretch + s;
             T v[kVec];
             if constexpr (sizeof(T) == 4)
                 *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(held + at);
             else
                 *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(held + at);
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) f(to_float<T>(v[j]), base + at + j, s);
+            for (int j = 0; j < kVec; ++j) f(to_float<T>(v[j]), base + at + j);
         }
     };
 
@@ -211,27 +208,32 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         const uint32_t high = (uint32_t)(v >> 32) + (old + low < old);
         if (high) atomicAdd(&sh.hi[bin], high);
     };
-    // The inclusive running sum over the CTA's threads, and the CTA's total.
-    auto block_scan = [&](u64 v, u64& all) {
+    auto warp_total = [&](u64 v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    };
+    auto warp_scan = [&](u64 v) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const u64 u = __shfl_up_sync(0xffffffffu, v, o);
             if (lane >= o) v += u;
         }
+        return v;
+    };
+    auto block_total = [&](u64 v) {
+        v = warp_total(v);
         __syncthreads();
-        if (lane == 31) sh.warp_sum[warp] = v;
+        if (lane == 0) sh.warp_sum[warp] = v;
         __syncthreads();
-        all = 0;
-        u64 before = 0;
-        for (int w = 0; w < kSampleWarps; ++w) {
-            if (w < warp) before += sh.warp_sum[w];
-            all += sh.warp_sum[w];
-        }
-        return v + before;
+        v = 0;
+        for (int w = 0; w < kSampleWarps; ++w) v += sh.warp_sum[w];
+        return v;
     };
     // Of the cluster's histograms together: the bin where the running total,
-    // from `above`, first reaches `want`. Each CTA adds up a share of the bins.
-    auto cross = [&](u64 above, u64 want) {
+    // from `above`, first reaches want(total of all bins). Each CTA adds up a
+    // share of the bins.
+    auto cross = [&](u64 above, auto&& wanted) {
         cluster.sync();
         const int per = kBins / ranks, q = (per + kSampleThreads - 1) / kSampleThreads;
         u64 mine[kBins / kSampleThreads], sum = 0;
@@ -245,17 +247,28 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
                 sum += mine[j];
             }
         }
-        u64 all;
-        const u64 run = block_scan(sum, all) - sum;
+        const u64 run = warp_scan(sum);
+        __syncthreads();
+        if (lane == 31) sh.warp_sum[warp] = run;
+        __syncthreads();
+        u64 before = above + run - sum, all = 0;
+        for (int w = 0; w < kSampleWarps; ++w) {
+            if (w < warp) before += sh.warp_sum[w];
+            all += sh.warp_sum[w];
+        }
         if (tid < ranks) cluster.map_shared_rank(sh.total, tid)[rank] = all;
         cluster.sync();
-        u64 before = above + run;
-        for (int r = 0; r < rank; ++r) before += sh.total[r];
+        all = 0;
+        for (int r = 0; r < ranks; ++r) {
+            if (r < rank) before += sh.total[r];
+            all += sh.total[r];
+        }
+        const u64 want = wanted(all);
         if (before < want && want <= before + sum) {
 #pragma unroll
             for (int j = 0; j < kBins / kSampleThreads; ++j) {
                 if (before < want && want <= before + mine[j]) {
-                    const Crossing found = {before, mine[j], rank * per + tid * q + j};
+                    const Crossing found = {before, mine[j], all, rank * per + tid * q + j};
                     for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&sh.crossing, r) = found;
                 }
                 before += mine[j];
@@ -267,119 +280,205 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     // Index of the first logit, in index order, at which the running sum of
     // value(logit, index) over the row exceeds target(total); -1 if none does.
     auto locate = [&](auto&& value, auto&& target, u64& total) {
-        u64 mine = 0, step_sum = 0;
-        int step = 0;
-        auto close = [&] {
-            u64 v = step_sum;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0) sh.chunk[step * kSampleWarps + warp] = v;
-            mine += step_sum;
-            step_sum = 0;
-        };
-        for_each([&](float l, int i, int s) {
-            if (s != step) {
-                close();
-                step = s;
-            }
-            step_sum += value(l, i);
-        });
-        if (steps > 0) close();
-        u64 all;
-        block_scan(mine, all);
+        u64 mine = 0;
+        for_each([&](float l, int i) { mine += value(l, i); });
+        mine = warp_total(mine);
+        __syncthreads();
+        if (lane == 0) sh.warp_sum[warp] = mine;
+        __syncthreads();
+        u64 before = 0, all = 0;
+        for (int w = 0; w < kSampleWarps; ++w) {
+            if (w < warp) before += sh.warp_sum[w];
+            all += sh.warp_sum[w];
+        }
         if (tid == 0) sh.place = -1;
         if (tid < ranks) cluster.map_shared_rank(sh.total, tid)[rank] = all;
         cluster.sync();
         total = 0;
-        u64 before = 0;
         for (int r = 0; r < ranks; ++r) {
             if (r < rank) before += sh.total[r];
             total += sh.total[r];
         }
         const u64 goal = target(total);
-        if (warp == 0 && before <= goal && goal < before + all) {
-            // the chunk of 128 logits, 32 chunks at a time, then the logit
-            u64 at = goal - before;
-            int chunk = 0;
-            for (int b = 0; b < steps * kSampleWarps; b += 32) {
-                const u64 v = b + lane < steps * kSampleWarps ? sh.chunk[b + lane] : 0;
-                u64 run = v;
+        if (before <= goal && goal < before + mine) {
+            // this warp's stretch again, a step at a time
+            for (int s = 0; s < stretch; s += kStep) {
+                const int at = warp * stretch + s + lane * kVec;
+                u64 v[kVec], sum = 0;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const u64 u = __shfl_up_sync(0xffffffffu, run, o);
-                    if (lane >= o) run += u;
+                for (int j = 0; j < kVec; ++j) {
+                    v[j] = s + lane * kVec < stretch ? value(to_float<T>(held[at + j]), base + at + j) : 0;
+                    sum += v[j];
                 }
-                const unsigned past = __ballot_sync(0xffffffffu, run > at);
-                if (past) {
-                    const int first = __ffs(past) - 1;
-                    at -= __shfl_sync(0xffffffffu, run - v, first);
-                    chunk = b + first;
-                    break;
+                if (!__any_sync(0xffffffffu, sum != 0)) continue;
+                u64 run = warp_scan(sum);
+                const u64 step = __shfl_sync(0xffffffffu, run, 31);
+                if (goal >= before + step) {
+                    before += step;
+                    continue;
                 }
-                at -= __shfl_sync(0xffffffffu, run, 31);
-            }
-            const int i0 = chunk / kSampleWarps * kStride + chunk % kSampleWarps * 32 * kVec + lane * kVec;
-            u64 v[kVec], sum = 0;
+                run += before - sum;
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) sum += v[j] = value(to_float<T>(held[i0 + j]), base + i0 + j);
-            u64 run = sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 u = __shfl_up_sync(0xffffffffu, run, o);
-                if (lane >= o) run += u;
-            }
-            run -= sum;
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-                if (run <= at && at < run + v[j])
-                    for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&sh.place, r) = base + i0 + j;
-                run += v[j];
+                for (int j = 0; j < kVec; ++j) {
+                    if (run <= goal && goal < run + v[j])
+                        for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&sh.place, r) = base + at + j;
+                    run += v[j];
+                }
+                break;
             }
         }
         cluster.sync();
         return sh.place;
     };
 
-    // Moves the cut to the shortest prefix of the kept that has `want` of
-    // value(logit), `range` being the distance from the top that the first
-    // bins resolve.
-    auto narrow = [&](auto&& value, u64 want, float range) {
-        const float scale = (float)kBins / range;
-        auto bin_of = [&](float l) { return l == top ? 0 : (int)fminf((top - l) * scale, (float)(kBins - 1)); };
+    const double u = (double)a.uniform[row];
+    // the first running sum above floor(u total) is the first above u total
+    auto goal_of = [&](u64 all) {
+        const u64 t = u > 0.0 ? (u64)fmin(u * (double)all, 9e18) : 0ull;
+        return t < all ? t : all - 1;
+    };
+    auto answer = [&](int token, float l, u64 total) {
+        a.tokens[row] = token;
+        if (a.logprob) {
+            const double x = l == top ? 0.0 : ((double)l - (double)top) / (double)temperature;
+            a.logprob[row] = (float)(x - log((double)total / (double)(1ull << S)));
+        }
+    };
+
+    if (top == -CUDART_INF_F || greedy) {
+        u64 total;
+        const int i = locate([&](float l, int) -> u64 { return l == top && l > -CUDART_INF_F; },
+                             [](u64) { return 0ull; }, total);
+        if (rank == 0 && tid == 0) {
+            a.tokens[row] = i;
+            if (a.logprob) a.logprob[row] = i < 0 ? -CUDART_INF_F : 0.0f;
+        }
+        return;  // the last cluster.sync is behind every access of another CTA's memory
+    }
+    int top_k = a.top_k ? a.top_k[row] : 0;
+    if (top_k <= 0 || top_k > a.vocab) top_k = a.vocab;
+    const float top_p = a.top_p ? a.top_p[row] : 1.0f;
+    const bool by_weight = top_p < 1.0f;
+    const float min_p = a.min_p ? a.min_p[row] : 0.0f;
+    const u64 least = min_p > 0.0f ? (u64)ceil(fmin((double)min_p, 1.0) * (double)(1ull << S)) : 0ull;
+    auto share_of = [&](u64 all) {
+        const double want = ceil((double)top_p * (double)all);
+        return want >= 1.0 ? (u64)want : 1ull;
+    };
+    // distances from the top that the first bins resolve: logits of language
+    // models lie within 64 of their largest; weights end 2^-(S+1) below theirs
+    const float count_range = 64.0f, weight_range = fminf(fmaxf(32.0f * temperature, 1e-30f), 1e30f);
+
+    // the distance from the top in bins, 0 for the top itself (also where inf -
+    // inf is NaN), and the nearest whole number of one below 2^22
+    auto distance = [&](float l, float scale) { return fminf(fmaxf((top - l) * scale, 0.0f), (float)(kBins - 1)); };
+    auto whole = [](float x) { return (int)(__float_as_uint(x + 8388608.0f) & 0x3fffffu); };
+    auto bin_in = [&](float l, float scale) { return whole(distance(l, scale)); };
+
+    // The first bins: of counts where top_k cuts, else of weights
+    const bool counting = top_k < a.vocab;
+    Crossing first = {0, 0, 0, kBins - 1};
+    const float first_scale = (float)kBins / (counting ? count_range : weight_range);
+    if (counting || by_weight) {
         clear();
-        for_each([&](float l, int i, int) {
-            if (kept(l, i)) add(bin_of(l), value(l));
+        if (counting)
+            for_each([&](float l, int) {
+                if (l > -CUDART_INF_F) atomicAdd(&sh.lo[bin_in(l, first_scale)], 1u);
+            });
+        else
+            for_each([&](float l, int) {
+                if (l > -CUDART_INF_F) add(bin_in(l, first_scale), weight(l));
+            });
+        if (tid == 0) sh.listed = 0;
+        // fewer tokens than top_k: the last of them ends the prefix
+        first = cross(0, [&](u64 all) { return counting ? min((u64)top_k, all) : share_of(all); });
+        // the candidates, to CTA 0 if they are few
+        for_each([&](float l, int i) {
+            if (l > -CUDART_INF_F && bin_in(l, first_scale) <= first.bin) {
+                const int n = atomicAdd(&sh.listed, 1);
+                if (n < kList) sh.list_key[n] = (u64)key_of(l) << 32 | (uint32_t)~i;
+            }
         });
-        Crossing x = cross(0, want);
+        __syncthreads();
+        if (tid < ranks) cluster.map_shared_rank(sh.total, tid)[rank] = (u64)sh.listed;
+        cluster.sync();
+        int before = 0, n = 0;
+        for (int r = 0; r < ranks; ++r) {
+            if (r < rank) before += (int)sh.total[r];
+            n += (int)sh.total[r];
+        }
+        if (n <= kList) {
+            const u64 mine = tid < sh.listed ? sh.list_key[tid] : 0;
+            cluster.sync();
+            if (tid < sh.listed) cluster.map_shared_rank(sh.list_key, 0)[before + tid] = mine;
+            cluster.sync();
+            if (rank != 0) return;
+            const u64 key = tid < n ? sh.list_key[tid] : 0;
+            const float l = logit_of((uint32_t)(key >> 32));
+            const int index = (int)~(uint32_t)key;
+            u64 w = tid < n ? weight(l) : 0;
+            sh.list_w[tid] = w;
+            __syncthreads();
+            // rank and weight of those before it
+            int ahead = 0;
+            u64 ahead_w = 0;
+            if (tid < n)
+                for (int j = 0; j < n; ++j)
+                    if (sh.list_key[j] > key) {
+                        ++ahead;
+                        ahead_w += sh.list_w[j];
+                    }
+            if (ahead >= top_k) w = 0;
+            const u64 all = counting ? block_total(w) : first.all;
+            if ((by_weight && ahead_w >= share_of(all)) || w < least) w = 0;
+            const u64 total = block_total(w);  // its barriers end the loop above
+            sh.list_w[tid] = w;
+            __syncthreads();
+            const u64 goal = goal_of(total);
+            if (w) {
+                u64 run = 0;
+                for (int j = 0; j < n; ++j)
+                    if ((uint32_t)sh.list_key[j] > (uint32_t)key) run += sh.list_w[j];  // lower indexes
+                if (run <= goal && goal < run + w) answer(index, l, total);
+            }
+            return;
+        }
+    }
+
+    // Moves the cut to the shortest prefix of the kept that has wanted(total)
+    // of value(logit); x: the crossing of the first bins.
+    auto narrow = [&](auto&& value, Crossing x, float scale, u64 want) {
         const int bin = x.bin;
+        const float low_edge = (float)bin - 0.5f;
         auto fine = [&](float l) {
-            return (int)fminf(fmaxf(((top - l) * scale - (float)bin) * (float)kBins, 0.0f), (float)(kBins - 1));
+            return whole(fminf(fmaxf((distance(l, scale) - low_edge) * (float)kBins, 0.0f), (float)(kBins - 1)));
         };
+        auto level = [&](u64) { return want; };
         clear();
-        for_each([&](float l, int i, int) {
-            if (kept(l, i) && bin_of(l) == bin) add(fine(l), value(l));
+        for_each([&](float l, int i) {
+            if (bin_in(l, scale) == bin && kept(l, i)) add(fine(l), value(l));
         });
-        x = cross(x.above, want);
+        x = cross(x.above, level);
         const int sub = x.bin;
         float high = -CUDART_INF_F, low = CUDART_INF_F;
-        for_each([&](float l, int i, int) {
-            if (kept(l, i) && bin_of(l) == bin && fine(l) == sub) high = fmaxf(high, l), low = fminf(low, l);
+        for_each([&](float l, int i) {
+            if (bin_in(l, scale) == bin && fine(l) == sub && kept(l, i)) high = fmaxf(high, l), low = fminf(low, l);
         });
         const float2 ends = cluster_bounds(high, low);
         float key = ends.x;
         if (ends.x != ends.y) {
             uint32_t prefix = 0;
 #pragma unroll 1
-            for (int level = 0; level < 3; ++level) {
-                const int down = level == 0 ? 21 : level == 1 ? 10 : 0, bits = level == 2 ? 10 : 11;
+            for (int step = 0; step < 3; ++step) {
+                const int down = step == 0 ? 21 : step == 1 ? 10 : 0, bits = step == 2 ? 10 : 11;
                 const uint32_t mask = (1u << bits) - 1u;
                 clear();
-                for_each([&](float l, int i, int) {
-                    if (!(kept(l, i) && bin_of(l) == bin && fine(l) == sub)) return;
+                for_each([&](float l, int i) {
+                    if (!(bin_in(l, scale) == bin && fine(l) == sub && kept(l, i))) return;
                     const uint32_t k = key_of(l);
-                    if (level == 0 || k >> (down + bits) == prefix) add((int)(mask - (k >> down & mask)), value(l));
+                    if (step == 0 || k >> (down + bits) == prefix) add((int)(mask - (k >> down & mask)), value(l));
                 });
-                x = cross(x.above, want);
+                x = cross(x.above, level);
                 prefix = prefix << bits | (mask - (uint32_t)x.bin);
             }
             key = logit_of(prefix);
@@ -399,36 +498,20 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
             cut_index = old_index;
         }
     };
-
-    if (top == -CUDART_INF_F || greedy) {
-        u64 total;
-        const int i = locate([&](float l, int) -> u64 { return l == top && l > -CUDART_INF_F; },
-                             [](u64) { return 0ull; }, total);
-        if (rank == 0 && tid == 0) {
-            a.tokens[row] = i;
-            if (a.logprob) a.logprob[row] = i < 0 ? -CUDART_INF_F : 0.0f;
+    if (counting) {
+        narrow([](float) -> u64 { return 1; }, first, first_scale, min((u64)top_k, first.all));
+        if (by_weight) {
+            const float scale = (float)kBins / weight_range;
+            clear();
+            for_each([&](float l, int i) {
+                if (kept(l, i)) add(bin_in(l, scale), weight(l));
+            });
+            first = cross(0, share_of);
+            narrow(weight, first, scale, share_of(first.all));
         }
-        return;  // the last cluster.sync is behind every access of another CTA's memory
+    } else if (by_weight) {
+        narrow(weight, first, first_scale, share_of(first.all));
     }
-    const int top_k = a.top_k ? a.top_k[row] : 0;
-    if (top_k > 0 && top_k < a.vocab) {
-        u64 tokens;
-        const float none = -CUDART_INF_F;
-        locate([&](float l, int) -> u64 { return l > none; }, [](u64) { return ~0ull; }, tokens);
-        // logits of language models lie within 64 of their largest
-        if ((u64)top_k < tokens) narrow([](float) -> u64 { return 1; }, (u64)top_k, 64.0f);
-    }
-    const float top_p = a.top_p ? a.top_p[row] : 1.0f;
-    if (top_p < 1.0f) {
-        u64 all;
-        locate([&](float l, int i) -> u64 { return kept(l, i) ? weight(l) : 0; }, [](u64) { return ~0ull; }, all);
-        const double want = ceil((double)top_p * (double)all);
-        // weights end 2^-(S + 1) below the largest
-        narrow(weight, want >= 1.0 ? (u64)want : 1ull, fminf(fmaxf(32.0f * temperature, 1e-30f), 1e30f));
-    }
-    const float min_p = a.min_p ? a.min_p[row] : 0.0f;
-    const u64 least = min_p > 0.0f ? (u64)ceil(fmin((double)min_p, 1.0) * (double)(1ull << S)) : 0ull;
-    const double u = (double)a.uniform[row];
     u64 total;
     const int token = locate(
         [&](float l, int i) -> u64 {
@@ -436,20 +519,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
             const u64 w = weight(l);
             return w >= least ? w : 0;
         },
-        [&](u64 all) {
-            // the first running sum above floor(u total) is the first above u total
-            const u64 t = u > 0.0 ? (u64)fmin(u * (double)all, 9e18) : 0ull;
-            return t < all ? t : all - 1;
-        },
-        total);
-    if (rank == 0 && tid == 0) {
-        a.tokens[row] = token;
-        if (a.logprob) {
-            const float l = to_float<T>(static_cast<const T*>(a.logits)[row * a.ld + token]);
-            const double x = l == top ? 0.0 : ((double)l - (double)top) / (double)temperature;
-            a.logprob[row] = (float)(x - log((double)total / (double)(1ull << S)));
-        }
-    }
+        goal_of, total);
+    if (rank == 0 && tid == 0)
+        answer(token, to_float<T>(static_cast<const T*>(a.logits)[row * a.ld + token]), total);
 }
 
 template <typename T>
@@ -457,27 +529,27 @@ cudaError_t launch(const SampleArgs& a, cudaStream_t s) {
     static std::once_flag once;
     static cudaError_t attr = cudaSuccess;
     auto kernel = sample_kernel<T>;
-    constexpr int kMost = (int)sizeof(SampleShared) +
-                          (kMaxSlice<T> + kStride - 1) / kStride * kStride * (int)sizeof(T);
+    constexpr int kMost = (int)sizeof(SampleShared) + kMaxSlice<T> * (int)sizeof(T);
     static_assert(kMost <= 227 * 1024, "shared memory of one CTA");
     std::call_once(once, [&] {
         attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
         if (attr == cudaSuccess) attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     });
     if (attr != cudaSuccess) return attr;
-    // CTAs per row: as few as leave two CTAs to an SM (80 KB of logits each),
-    // more while the rows leave SMs idle and a CTA has a step of its own
+    // CTAs per row: as few as leave two CTAs to an SM, more while the rows
+    // leave SMs idle and a CTA has 2048 logits of its own
     int ranks = 1;
     while (ranks < kMaxCluster && (long long)ranks * (kSliceBytes / (int)sizeof(T)) < a.vocab) ranks *= 2;
-    while (ranks < kMaxCluster && 2ll * ranks * a.rows <= sm_count() && ranks * kStride < a.vocab) ranks *= 2;
-    const int slice = ((a.vocab + ranks - 1) / ranks + 7) / 8 * 8;  // whole 16-byte words
+    while (ranks < kMaxCluster && 2ll * ranks * a.rows <= sm_count() && ranks * 2048 < a.vocab) ranks *= 2;
+    constexpr int kUnit = 8 * kSampleWarps;  // whole 16-byte words, for every warp
+    const int slice = (a.vocab + ranks * kUnit - 1) / (ranks * kUnit) * kUnit;
     if (slice > kMaxSlice<T>) return cudaErrorInvalidValue;
-    int bits = 1;  // vocab < 2^bits
+    int bits = 18;  // vocab < 2^bits
     while ((1ll << bits) <= a.vocab) ++bits;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(a.rows * ranks);
     cfg.blockDim = dim3(kSampleThreads);
-    cfg.dynamicSmemBytes = sizeof(SampleShared) + (size_t)((slice + kStride - 1) / kStride) * kStride * sizeof(T);
+    cfg.dynamicSmemBytes = sizeof(SampleShared) + (size_t)slice * sizeof(T);
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
