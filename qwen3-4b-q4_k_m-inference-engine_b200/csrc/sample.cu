@@ -25,6 +25,7 @@
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
+#include <cmath>
 #include <mutex>
 
 #include "paged_device.cuh"
@@ -49,6 +50,7 @@ constexpr int kSliceBytes = 80 * 1024;
 template <typename T>
 constexpr int kMaxSlice = kSliceBytes / sizeof(T) > 25600 ? kSliceBytes / sizeof(T) : 25600;
 constexpr int kTable = 64;
+constexpr int kCopies = 4;  // a slice's copies, each of a quarter of the warps' stretches
 
 // Whole numbers in the order of the floats.
 __device__ __forceinline__ uint32_t key_of(float l) {
@@ -58,6 +60,11 @@ __device__ __forceinline__ uint32_t key_of(float l) {
 __device__ __forceinline__ float logit_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
+
+// 2^(j/64), from the host.
+struct ExpTable {
+    double v[kTable];
+};
 
 struct Crossing {
     u64 above, inside, all;  // the total above the bin, in it, and of every bin
@@ -74,6 +81,7 @@ struct alignas(16) SampleShared {
     float bound[2][kMaxCluster];
     Crossing crossing;
     int place, listed;
+    uint64_t landed[kCopies];
 };
 
 // w(l) = round(2^(S + t)), t = (l - top) log2(e) / T, in fp64: l - top is exact,
@@ -89,7 +97,6 @@ struct Weights {
     const double* table;
 
     __device__ __forceinline__ u64 operator()(float l) const {
-        if (!((l - top) * c > cutoff)) return l == top ? 1ull << S : 0;  // top itself where inf - inf or 0 inf is NaN
         constexpr double kWhole = 6755399441055744.0;  // 1.5 2^52
         const double d = (double)l - top64;
         const double z = fma(d, c64, kWhole);
@@ -102,13 +109,16 @@ struct Weights {
         const int i = __double2loint(z);
         const double v = table[i & 63];
         const double w = p * __hiloint2double(__double2hiint(v) + (((i >> 6) + S) << 20), __double2loint(v));
-        return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+        const u64 n = (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
+        // selects, not a branch: four of these run side by side. top itself
+        // where inf - inf or 0 inf is NaN
+        return (l - top) * c > cutoff ? n : l == top ? 1ull << S : 0;
     }
 };
 
 template <typename T>
 __global__ void __launch_bounds__(kSampleThreads, 2)
-    sample_kernel(const __grid_constant__ SampleArgs a, int S, int slice) {
+    sample_kernel(const __grid_constant__ SampleArgs a, const __grid_constant__ ExpTable table, int S, int slice) {
     extern __shared__ __align__(16) uint8_t smem[];
     SampleShared& sh = *reinterpret_cast<SampleShared*>(smem);
     T* held = reinterpret_cast<T*>(smem + sizeof(SampleShared));
@@ -120,33 +130,55 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     const int count = min(slice, a.vocab - base);
     const T* src = static_cast<const T*>(a.logits) + row * a.ld + base;
 
-    if (tid < kTable) sh.table[tid] = exp2(tid / 64.0);
-    float most = -CUDART_INF_F;
-    if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
-        constexpr int kWide = 16 / sizeof(T);
-#pragma unroll 4
-        for (int i = tid * kWide; i + kWide <= count; i += kSampleThreads * kWide) {
-            const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + i));
-            *reinterpret_cast<uint4*>(held + i) = w;
-            const T* t = reinterpret_cast<const T*>(&w);
-#pragma unroll
-            for (int j = 0; j < kWide; ++j) most = fmaxf(most, to_float<T>(t[j]));
-        }
-        const int i = count / kWide * kWide + tid;
-        if (i < count) {
-            held[i] = src[i];
-            most = fmaxf(most, to_float<T>(src[i]));
-        }
-    } else {
-#pragma unroll 4
-        for (int i = tid; i < count; i += kSampleThreads) {
-            const T v = src[i];
-            held[i] = v;
-            most = fmaxf(most, to_float<T>(v));
+    // The slice into shared memory: bulk copies where rows start on 16-byte
+    // words, all in flight at once.
+    const int stretch = slice / kSampleWarps;  // a warp's logits, a multiple of 8
+    if (tid == 0) {
+        for (int i = 0; i < kCopies; ++i) mbar_init(&sh.landed[i], 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
+    const bool aligned = reinterpret_cast<uintptr_t>(src) % 16 == 0;
+    constexpr int kWide = 16 / sizeof(T);
+    const int copied = aligned ? count / kWide * kWide : 0;
+    if (tid == 0) {
+        const int part = slice / kCopies;
+        for (int i = 0; i < kCopies; ++i) {
+            const int n = min(max(copied - i * part, 0), part);
+            mbar_arrive_expect_tx(&sh.landed[i], n * (int)sizeof(T));
+            if (n > 0) bulk_g2s(held + i * part, src + i * part, n * (int)sizeof(T), &sh.landed[i]);
         }
     }
+    if (tid < kTable) sh.table[tid] = table.v[tid];
+#pragma unroll 4
+    for (int i = copied + tid; i < count; i += kSampleThreads) held[i] = src[i];
     // what lies behind the vocabulary is never drawn
     for (int i = count + tid; i < slice; i += kSampleThreads) held[i] = from_float<T>(-CUDART_INF_F);
+
+    // f(logits, index of the first) for all of the CTA's logits, kVec at a time;
+    // a warp's are consecutive, so that its sums are of one stretch of the
+    // index order
+    auto for_each = [&](auto&& f) {
+        for (int s = lane * kVec; s < stretch; s += kStep) {
+            const int at = warp * stretch + s;
+            T v[kVec];
+            if constexpr (sizeof(T) == 4)
+                *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(held + at);
+            else
+                *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(held + at);
+            float l[kVec];
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) l[j] = to_float<T>(v[j]);
+            f(l, base + at);
+        }
+    };
+    __syncthreads();
+    mbar_wait_bounded(&sh.landed[warp / (kSampleWarps / kCopies)], 0, nullptr, 0);
+    float most = -CUDART_INF_F;
+    for_each([&](const float(&l)[kVec], int) {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) most = fmaxf(most, l[j]);
+    });
 
     // The largest and smallest of a value over the cluster.
     auto cluster_bounds = [&](float high, float low) {
@@ -182,22 +214,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     float cut = -CUDART_INF_F;
     int cut_index = -1;
     auto kept = [&](float l, int i) { return l > cut || (l == cut && i <= cut_index); };
-
-    // f(logit, index) for all of the CTA's logits, four at a time; a warp's are
-    // consecutive, so that its sums are of one stretch of the index order
-    const int stretch = slice / kSampleWarps;  // a multiple of kVec
-    auto for_each = [&](auto&& f) {
-        for (int s = lane * kVec; s < stretch; s += kStep) {
-            const int at = warp * stretch + s;
-            T v[kVec];
-            if constexpr (sizeof(T) == 4)
-                *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(held + at);
-            else
-                *reinterpret_cast<uint2*>(v) = *reinterpret_cast<const uint2*>(held + at);
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) f(to_float<T>(v[j]), base + at + j);
-        }
-    };
 
     auto clear = [&] {
         for (int i = tid; i < kBins; i += kSampleThreads) sh.lo[i] = sh.hi[i] = 0;
@@ -277,11 +293,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         cluster.sync();
         return sh.crossing;
     };
-    // Index of the first logit, in index order, at which the running sum of
-    // value(logit, index) over the row exceeds target(total); -1 if none does.
+    // Index of the first logit, in index order, at which the running sum of the
+    // values (value(logits, index of the first, values); 0 for -inf) over the
+    // row exceeds target(total); -1 if none does.
     auto locate = [&](auto&& value, auto&& target, u64& total) {
         u64 mine = 0;
-        for_each([&](float l, int i) { mine += value(l, i); });
+        for_each([&](const float(&l)[kVec], int i) {
+            u64 v[kVec];
+            value(l, i, v);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) mine += v[j];
+        });
         mine = warp_total(mine);
         __syncthreads();
         if (lane == 0) sh.warp_sum[warp] = mine;
@@ -304,12 +326,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
             // this warp's stretch again, a step at a time
             for (int s = 0; s < stretch; s += kStep) {
                 const int at = warp * stretch + s + lane * kVec;
+                const bool there = s + lane * kVec < stretch;
+                float l[kVec];
                 u64 v[kVec], sum = 0;
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) {
-                    v[j] = s + lane * kVec < stretch ? value(to_float<T>(held[at + j]), base + at + j) : 0;
-                    sum += v[j];
-                }
+                for (int j = 0; j < kVec; ++j) l[j] = there ? to_float<T>(held[at + j]) : -CUDART_INF_F;
+                value(l, base + at, v);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) sum += v[j];
                 if (!__any_sync(0xffffffffu, sum != 0)) continue;
                 u64 run = warp_scan(sum);
                 const u64 step = __shfl_sync(0xffffffffu, run, 31);
@@ -347,8 +371,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
 
     if (top == -CUDART_INF_F || greedy) {
         u64 total;
-        const int i = locate([&](float l, int) -> u64 { return l == top && l > -CUDART_INF_F; },
-                             [](u64) { return 0ull; }, total);
+        const int i = locate(
+            [&](const float(&l)[kVec], int, u64(&v)[kVec]) {
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) v[j] = l[j] == top && l[j] > -CUDART_INF_F;
+            },
+            [](u64) { return 0ull; }, total);
         if (rank == 0 && tid == 0) {
             a.tokens[row] = i;
             if (a.logprob) a.logprob[row] = i < 0 ? -CUDART_INF_F : 0.0f;
@@ -382,22 +410,31 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     if (counting || by_weight) {
         clear();
         if (counting)
-            for_each([&](float l, int) {
-                if (l > -CUDART_INF_F) atomicAdd(&sh.lo[bin_in(l, first_scale)], 1u);
+            for_each([&](const float(&l)[kVec], int) {
+#pragma unroll
+                for (int j = 0; j < kVec; ++j)
+                    if (l[j] > -CUDART_INF_F) atomicAdd(&sh.lo[bin_in(l[j], first_scale)], 1u);
             });
         else
-            for_each([&](float l, int) {
-                if (l > -CUDART_INF_F) add(bin_in(l, first_scale), weight(l));
+            for_each([&](const float(&l)[kVec], int) {
+                u64 w[kVec];
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) w[j] = weight(l[j]);
+#pragma unroll
+                for (int j = 0; j < kVec; ++j)
+                    if (w[j]) add(bin_in(l[j], first_scale), w[j]);
             });
         if (tid == 0) sh.listed = 0;
         // fewer tokens than top_k: the last of them ends the prefix
         first = cross(0, [&](u64 all) { return counting ? min((u64)top_k, all) : share_of(all); });
         // the candidates, to CTA 0 if they are few
-        for_each([&](float l, int i) {
-            if (l > -CUDART_INF_F && bin_in(l, first_scale) <= first.bin) {
-                const int n = atomicAdd(&sh.listed, 1);
-                if (n < kList) sh.list_key[n] = (u64)key_of(l) << 32 | (uint32_t)~i;
-            }
+        for_each([&](const float(&l)[kVec], int i) {
+#pragma unroll
+            for (int j = 0; j < kVec; ++j)
+                if (l[j] > -CUDART_INF_F && bin_in(l[j], first_scale) <= first.bin) {
+                    const int n = atomicAdd(&sh.listed, 1);
+                    if (n < kList) sh.list_key[n] = (u64)key_of(l[j]) << 32 | (uint32_t)~(i + j);
+                }
         });
         __syncthreads();
         if (tid < ranks) cluster.map_shared_rank(sh.total, tid)[rank] = (u64)sh.listed;
@@ -455,14 +492,21 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         };
         auto level = [&](u64) { return want; };
         clear();
-        for_each([&](float l, int i) {
-            if (bin_in(l, scale) == bin && kept(l, i)) add(fine(l), value(l));
+        for_each([&](const float(&l)[kVec], int i) {
+#pragma unroll
+            for (int j = 0; j < kVec; ++j)
+                if (bin_in(l[j], scale) == bin && kept(l[j], i + j)) add(fine(l[j]), value(l[j]));
         });
         x = cross(x.above, level);
         const int sub = x.bin;
         float high = -CUDART_INF_F, low = CUDART_INF_F;
-        for_each([&](float l, int i) {
-            if (bin_in(l, scale) == bin && fine(l) == sub && kept(l, i)) high = fmaxf(high, l), low = fminf(low, l);
+        for_each([&](const float(&l)[kVec], int i) {
+#pragma unroll
+            for (int j = 0; j < kVec; ++j)
+                if (bin_in(l[j], scale) == bin && fine(l[j]) == sub && kept(l[j], i + j)) {
+                    high = fmaxf(high, l[j]);
+                    low = fminf(low, l[j]);
+                }
         });
         const float2 ends = cluster_bounds(high, low);
         float key = ends.x;
@@ -473,10 +517,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
                 const int down = step == 0 ? 21 : step == 1 ? 10 : 0, bits = step == 2 ? 10 : 11;
                 const uint32_t mask = (1u << bits) - 1u;
                 clear();
-                for_each([&](float l, int i) {
-                    if (!(bin_in(l, scale) == bin && fine(l) == sub && kept(l, i))) return;
-                    const uint32_t k = key_of(l);
-                    if (step == 0 || k >> (down + bits) == prefix) add((int)(mask - (k >> down & mask)), value(l));
+                for_each([&](const float(&l)[kVec], int i) {
+#pragma unroll 1
+                    for (int j = 0; j < kVec; ++j) {
+                        if (!(bin_in(l[j], scale) == bin && fine(l[j]) == sub && kept(l[j], i + j))) continue;
+                        const uint32_t k = key_of(l[j]);
+                        if (step == 0 || k >> (down + bits) == prefix)
+                            add((int)(mask - (k >> down & mask)), value(l[j]));
+                    }
                 });
                 x = cross(x.above, level);
                 prefix = prefix << bits | (mask - (uint32_t)x.bin);
@@ -492,7 +540,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         if (n * each < x.inside) {
             u64 total;
             cut_index = locate(
-                [&](float l, int i) -> u64 { return l == key && (l > old || (l == old && i <= old_index)); },
+                [&](const float(&l)[kVec], int i, u64(&v)[kVec]) {
+#pragma unroll
+                    for (int j = 0; j < kVec; ++j)
+                        v[j] = l[j] == key && (key > old || (key == old && i + j <= old_index));
+                },
                 [&](u64) { return n - 1; }, total);
         } else if (key == old) {
             cut_index = old_index;
@@ -503,8 +555,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         if (by_weight) {
             const float scale = (float)kBins / weight_range;
             clear();
-            for_each([&](float l, int i) {
-                if (kept(l, i)) add(bin_in(l, scale), weight(l));
+            for_each([&](const float(&l)[kVec], int i) {
+#pragma unroll
+                for (int j = 0; j < kVec; ++j)
+                    if (kept(l[j], i + j)) add(bin_in(l[j], scale), weight(l[j]));
             });
             first = cross(0, share_of);
             narrow(weight, first, scale, share_of(first.all));
@@ -514,10 +568,20 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     }
     u64 total;
     const int token = locate(
-        [&](float l, int i) -> u64 {
-            if (!kept(l, i)) return 0;
-            const u64 w = weight(l);
-            return w >= least ? w : 0;
+        [&](const float(&l)[kVec], int i, u64(&v)[kVec]) {
+            bool in[kVec], any = false;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+                in[j] = kept(l[j], i + j);
+                any |= in[j];
+                v[j] = 0;
+            }
+            if (!any) return;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+                const u64 w = weight(l[j]);
+                v[j] = in[j] && w >= least ? w : 0;
+            }
         },
         goal_of, total);
     if (rank == 0 && tid == 0)
@@ -557,7 +621,9 @@ cudaError_t launch(const SampleArgs& a, cudaStream_t s) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a, 62 - bits, slice);
+    ExpTable table;
+    for (int j = 0; j < kTable; ++j) table.v[j] = std::exp2(j / (double)kTable);
+    return cudaLaunchKernelEx(&cfg, kernel, a, table, 62 - bits, slice);
 }
 
 }  // namespace
