@@ -22,7 +22,11 @@ enum class Kind { kF32, kF16, kBf16 };
 
 constexpr int kTileRows = 256;   // two MMA tiles of 128 query rows
 constexpr int kBlockKeys = 128;
-constexpr int kTcThreads = 320;  // two softmax warpgroups, TMA warp, MMA warp
+constexpr int kTcThreads = 384;  // two softmax warpgroups, and one of the TMA and MMA warps
+// Registers: 168 a thread at launch (384 x 168 = 64512), then 200 for the softmax
+// warpgroups, which hold a row of 128 scores, and 104 for the third:
+// 256 x 200 + 128 x 104 = 64512.
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
 constexpr int kMinUnits = 2;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -55,6 +59,9 @@ struct Types<Kind::kBf16> {
 template <Kind K, int D>
 struct Layout {
     static constexpr int kParts = K == Kind::kF32 ? 2 : 1;
+    // TMEM columns of 32 probabilities, written over their scores: 16 (two to a
+    // column), for fp32 the low parts 16 on
+    static constexpr int kPStep = 16 * kParts;
     static constexpr int kHalf = 128 * 128;
     static constexpr int kMat = D / 64 * kHalf;  // 128 rows of D 16-bit values
     static constexpr int kStages = D == 64 ? 8 : K == Kind::kF32 ? 3 : 5;
@@ -158,114 +165,124 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t tmem = bar.tmem;
     fence_proxy_async();  // the plan's words, before the ring's copies land on them
     __syncthreads();
-    Pieces<kTileRows, kBlockKeys> pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
 
-    if (warp == 8) {
-        // ---------------- TMA: K and V blocks, page by page, a lane per (page, half)
-        const int box = min(a.cache.page_size, kBlockKeys);
-        const int boxes = kBlockKeys / box;
-        const int page_in_block = lane / (D / 64), half = lane % (D / 64);
-        const uint32_t box_bytes = (uint32_t)box * D * 2;
-        int n = 0;
-        bool ok = true;
-        for (; pc.valid() && ok; pc.next()) {
-            for (int i = 0; i < pc.count && ok; ++i) {
-                const int key0 = pc.tile.key_begin + (pc.b + i) * kBlockKeys;
-                const int live = min(max((pc.tile.key_end - key0 + box - 1) / box, 0), boxes);
-                int page = -1;
-                if (page_in_block < live)
-                    page = __ldg(a.batch.page_table + (size_t)pc.s * a.batch.table_stride +
-                                 ((key0 + page_in_block * box) >> a.cache.page_shift));
-                for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
-                    const int st = n % kStages;
-                    ok = wait_or_dead(&bar.empty[st], ((n / kStages) & 1) ^ 1, dead);
-                    if (!__all_sync(0xffffffffu, ok)) {
-                        ok = false;
-                        break;
-                    }
-                    if (lane == 0) mbar_arrive_expect_tx(&bar.full[st], live * box_bytes);
-                    __syncwarp();
+    using Walk = Pieces<kTileRows, kBlockKeys>;
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == 8) {
+            Walk pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
+            // ---------------- TMA: K and V blocks, page by page, a lane per (page, half)
+            const int box = min(a.cache.page_size, kBlockKeys);
+            const int boxes = kBlockKeys / box;
+            const int page_in_block = lane / (D / 64), half = lane % (D / 64);
+            const uint32_t box_bytes = (uint32_t)box * D * 2;
+            int n = 0;
+            bool ok = true;
+            for (; pc.valid() && ok; pc.next()) {
+                for (int i = 0; i < pc.count && ok; ++i) {
+                    const int key0 = pc.tile.key_begin + (pc.b + i) * kBlockKeys;
+                    const int live = min(max((pc.tile.key_end - key0 + box - 1) / box, 0), boxes);
+                    int page = -1;
                     if (page_in_block < live)
-                        tma_load_4d(smem + L::kRing + st * L::kMat + half * L::kHalf + page_in_block * box * 128,
-                                    kv ? &vmap : &kmap, half * 64, key0 & (a.cache.page_size - 1), pc.h, page,
-                                    &bar.full[st]);
+                        page = __ldg(a.batch.page_table + (size_t)pc.s * a.batch.table_stride +
+                                     ((key0 + page_in_block * box) >> a.cache.page_shift));
+                    for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
+                        const int st = n % kStages;
+                        ok = wait_or_dead(&bar.empty[st], ((n / kStages) & 1) ^ 1, dead);
+                        if (!__all_sync(0xffffffffu, ok)) {
+                            ok = false;
+                            break;
+                        }
+                        if (lane == 0) mbar_arrive_expect_tx(&bar.full[st], live * box_bytes);
+                        __syncwarp();
+                        if (page_in_block < live)
+                            tma_load_4d(smem + L::kRing + st * L::kMat + half * L::kHalf + page_in_block * box * 128,
+                                        kv ? &vmap : &kmap, half * 64, key0 & (a.cache.page_size - 1), pc.h, page,
+                                        &bar.full[st]);
+                    }
                 }
             }
-        }
-        // every copy issued has landed before the CTA can exit
-        for (int i = max(n - kStages, 0); i < n; ++i) 
-            mbar_wait_bounded(&bar.full[i % kStages], (i / kStages) & 1, nullptr, 0);
-        __syncwarp();
-    } else if (warp == 9) {
-        if (lane == 0) {
-            // ---------------- MMA issue
-            int n = 0;
-            uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-            bool ok = true;
-            const uint32_t q_addr = smem_addr(smem), ring = smem_addr(smem + L::kRing);
-            auto wait_stage = [&](int i) { return wait_or_dead(&bar.full[i % kStages], (i / kStages) & 1, dead); };
-            auto score = [&](int t, int stage) {
-                const uint32_t k = ring + (stage % kStages) * L::kMat;
+            // every copy issued has landed before the CTA can exit
+            for (int i = max(n - kStages, 0); i < n; ++i) 
+                mbar_wait_bounded(&bar.full[i % kStages], (i / kStages) & 1, nullptr, 0);
+            __syncwarp();
+        } else if (warp == 9) {
+            if (lane == 0) {
+                // ---------------- MMA issue
+                Walk pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
+                int n = 0;
+                uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+                bool ok = true;
+                const uint32_t q_addr = smem_addr(smem), ring = smem_addr(smem + L::kRing);
+                auto wait_stage = [&](int i) { return wait_or_dead(&bar.full[i % kStages], (i / kStages) & 1, dead); };
+                const uint64_t q_desc = desc_k_major(q_addr), k_desc = desc_k_major(ring);
+                const uint64_t v_desc = desc_mn_major(ring, L::kHalf);
+                auto score = [&](int t, int stage) {
+                    const uint64_t k = k_desc + (stage % kStages) * (L::kMat >> 4);
+                    uint64_t q = q_desc + t * L::kParts * (L::kMat >> 4);
 #pragma unroll
-                for (int pt = 0; pt < L::kParts; ++pt)
+                    for (int pt = 0; pt < L::kParts; ++pt, q += L::kMat >> 4)
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint32_t off = (kk / 4) * L::kHalf + (kk % 4) * 32;
-                        mma_ss(tmem + kS + 128 * t, desc_k_major(q_addr + (t * L::kParts + pt) * L::kMat + off),
-                               desc_k_major(k + off), kIdescS, (pt | kk) != 0);
-                    }
-                tc_commit(&bar.s_full[t]);
-            };
-            auto value = [&](int t, int stage, bool accumulate) {
-                const uint32_t v = ring + (stage % kStages) * L::kMat;
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            const uint32_t off = ((kk / 4) * L::kHalf + (kk % 4) * 32) >> 4;
+                            mma_ss(tmem + kS + 128 * t, q + off, k + off, kIdescS, (pt | kk) != 0);
+                        }
+                    tc_commit(&bar.s_full[t]);
+                };
+                auto value = [&](int t, int stage, bool accumulate) {
+                    const uint64_t v = v_desc + (stage % kStages) * (L::kMat >> 4);
+                    const uint32_t p = tmem + kS + 128 * t;
 #pragma unroll
-                for (int kk = 0; kk < kBlockKeys / 16; ++kk)
+                    for (int kk = 0; kk < kBlockKeys / 16; ++kk)
 #pragma unroll
-                    for (int pt = 0; pt < L::kParts; ++pt)
-                        mma_ts(tmem + kO + 128 * t, tmem + kS + 128 * t + 64 * pt + 8 * kk,
-                               desc_mn_major(v + kk * 2048, L::kHalf), kIdescO, accumulate || (pt | kk) != 0);
-            };
-            for (; pc.valid() && ok; pc.next()) {
-                const int tiles = pc.tile.rows > 128 ? 2 : 1;
-                int k_stage = n++;
-                ok = wait_stage(k_stage);
-                for (int t = 0; t < tiles && ok; ++t) {
-                    ok = wait_or_dead(&bar.q_full[t], q_phase[t]++ & 1, dead);
-                    if (!ok) break;
-                    tc_fence_after();
-                    score(t, k_stage);
-                }
-                tc_commit(&bar.empty[k_stage % kStages]);
-                for (int i = 0; i < pc.count && ok; ++i) {
-                    const bool more = i + 1 < pc.count;
-                    const int v_stage = n++;
-                    if (more) k_stage = n++;
+                        for (int pt = 0; pt < L::kParts; ++pt)
+                            mma_ts(tmem + kO + 128 * t, p + L::kPStep * (kk / 2) + 16 * pt + 8 * (kk & 1),
+                                   v + kk * (2048 >> 4), kIdescO, accumulate || (pt | kk) != 0);
+                };
+                for (; pc.valid() && ok; pc.next()) {
+                    const int tiles = pc.tile.rows > 128 ? 2 : 1;
+                    int k_stage = n++;
+                    ok = wait_stage(k_stage);
                     for (int t = 0; t < tiles && ok; ++t) {
-                        ok = wait_or_dead(&bar.p_full[t], p_phase[t]++ & 1, dead) && wait_stage(v_stage);
+                        ok = wait_or_dead(&bar.q_full[t], q_phase[t]++ & 1, dead);
                         if (!ok) break;
                         tc_fence_after();
-                        value(t, v_stage, i > 0);
-                        if (more) {
-                            ok = wait_stage(k_stage);
+                        score(t, k_stage);
+                    }
+                    tc_commit(&bar.empty[k_stage % kStages]);
+                    for (int i = 0; i < pc.count && ok; ++i) {
+                        const bool more = i + 1 < pc.count;
+                        const int v_stage = n++;
+                        if (more) k_stage = n++;
+                        for (int t = 0; t < tiles && ok; ++t) {
+                            ok = wait_or_dead(&bar.p_full[t], p_phase[t]++ & 1, dead) && wait_stage(v_stage);
                             if (!ok) break;
                             tc_fence_after();
-                            score(t, k_stage);
-                        } else {
-                            tc_commit(&bar.o_full[t]);
+                            value(t, v_stage, i > 0);
+                            if (more) {
+                                ok = wait_stage(k_stage);
+                                if (!ok) break;
+                                tc_fence_after();
+                                score(t, k_stage);
+                            } else {
+                                tc_commit(&bar.o_full[t]);
+                            }
                         }
+                        tc_commit(&bar.empty[v_stage % kStages]);
+                        if (more) tc_commit(&bar.empty[k_stage % kStages]);
                     }
-                    tc_commit(&bar.empty[v_stage % kStages]);
-                    if (more) tc_commit(&bar.empty[k_stage % kStages]);
+                }
+                if (!ok) {  // the MMAs in flight end before the TMEM is freed
+                    tc_commit(&bar.done);
+                    mbar_wait_bounded(&bar.done, 0, nullptr, 0);
                 }
             }
-            if (!ok) {  // the MMAs in flight end before the TMEM is freed
-                tc_commit(&bar.done);
-                mbar_wait_bounded(&bar.done, 0, nullptr, 0);
-            }
+            __syncwarp();
         }
-        __syncwarp();
     } else {
         // ---------------- softmax: warpgroup t, a thread per query row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        Walk pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
         const int t = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t s_addr = tmem + kS + 128 * t + lanes, o_addr = tmem + kO + 128 * t + lanes;
@@ -394,47 +411,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     m = mn;
                 }
                 const float shift = m == -CUDART_INF_F ? 0.0f : m - kBias<K>;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (K == Kind::kF32) {
+                const uint64_t c2 = pack_f32x2(c, c), shift2 = pack_f32x2(-shift, -shift);
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t hi[32];  // 16 high words, then 16 low ones
+                for (int j = 0; j < 4; ++j) {
+                    // 32 probabilities: 16 words (and 16 of low parts)
+                    uint32_t w[16], low[16];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float p0 = exp2_fast(fmaf(__uint_as_float(s[j][2 * e]), c, -shift));
-                            const float p1 = exp2_fast(fmaf(__uint_as_float(s[j][2 * e + 1]), c, -shift));
-                            sum[e & 3] += p0 + p1;
-                            split2(p0, p1, hi[e], hi[16 + e]);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) s[j][e] = hi[e];
-                    }
-#pragma unroll
-                    for (int pt = 0; pt < 2; ++pt)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            uint32_t w[32];
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) w[e] = s[2 * j + (e >> 4)][16 * pt + (e & 15)];
-                            tmem_st32(s_addr + 64 * pt + 32 * j, w);
-                        }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        uint32_t w[32];
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const float p0 =
-                                exp2_fast(fmaf(__uint_as_float(s[2 * j + (e >> 4)][2 * (e & 15)]), c, -shift));
-                            const float p1 =
-                                exp2_fast(fmaf(__uint_as_float(s[2 * j + (e >> 4)][2 * (e & 15) + 1]), c, -shift));
-                            sum[e & 3] += p0 + p1;
+                    for (int e = 0; e < 16; ++e) {
+                        const uint64_t x = fma_f32x2(
+                            pack_f32x2(__uint_as_float(s[j][2 * e]), __uint_as_float(s[j][2 * e + 1])), c2, shift2);
+                        float p0, p1;
+                        unpack_f32x2(x, p0, p1);
+                        p0 = exp2_fast(p0);
+                        p1 = exp2_fast(p1);
+                        sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(p0, p1));
+                        if constexpr (K == Kind::kF32)
+                            split2(p0, p1, w[e], low[e]);
+                        else
                             w[e] = pack2<K>(p0, p1);
-                        }
-                        tmem_st32(s_addr + 32 * j, w);
                     }
+                    tmem_st16(s_addr + L::kPStep * j, w);
+                    if constexpr (K == Kind::kF32) tmem_st16(s_addr + L::kPStep * j + 16, low);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                float sum0, sum1;
+                unpack_f32x2(add_f32x2(sum[0], sum[1]), sum0, sum1);
+                l += sum0 + sum1;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();

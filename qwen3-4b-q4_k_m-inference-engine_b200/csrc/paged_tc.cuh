@@ -91,6 +91,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int x, int y, int z, int w,
@@ -111,18 +119,43 @@ __device__ __forceinline__ uint32_t swz128(int r, int c) {
 }
 
 // Bounded wait on a barrier phase; a wait that gives up (2 s) marks `dead`,
-// which makes every other wait of the CTA give up at its next poll.
+// which makes every other wait of the CTA give up. The clock is read once in
+// 64 polls, each of which sleeps until the phase completes or 20 us have
+// passed: reading it first would delay a wait that is about to end.
 __device__ __forceinline__ bool wait_or_dead(uint64_t* bar, uint32_t parity, volatile int* dead) {
     if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t start = global_timer_ns();
-    for (;;) {
+    uint64_t start = 0;
+#pragma unroll 1
+    for (uint32_t i = 1;; ++i) {
         if (mbar_try_wait_suspend(bar, parity)) return true;
+        if (i % 64) continue;
+        if (start == 0) start = global_timer_ns();
         if (*dead) return false;
         if (global_timer_ns() - start > kWaitLimitNs) {
             *dead = 1;
             return false;
         }
     }
+}
+
+// Two fp32 operations at a time.
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 }  // namespace paged_dev
