@@ -20,14 +20,12 @@ using namespace paged_dev;
 
 enum class Kind { kF32, kF16, kBf16 };
 
-constexpr int kTileRows = 256;   // two MMA tiles of 128 query rows
+constexpr int kTileRows = 256;  // two MMA tiles of 128 query rows
 constexpr int kBlockKeys = 128;
-constexpr int kTcThreads = 384;  // two softmax warpgroups, and one of the TMA and MMA warps
-// Registers: 168 a thread at launch (384 x 168 = 64512), then 200 for the softmax
-// warpgroups, which hold a row of 128 scores, and 104 for the third:
-// 256 x 200 + 128 x 104 = 64512.
-constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
-constexpr int kMinUnits = 2;
+constexpr int kSoftmaxWarps = 16;  // two warpgroups per MMA tile, a thread per row and half of its keys
+constexpr int kTcThreads = (kSoftmaxWarps + 2) * 32;  // and a TMA and an MMA warp
+constexpr int kTileCost = 2;
+constexpr int kMinUnits = 4;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 // The reference point of a row's exponentials moves only when its maximum
@@ -39,7 +37,6 @@ constexpr float kLazy = 8.0f;
 // 2^-24, so that one of 2^-32 of the row's largest still has its low part.
 template <Kind K>
 constexpr float kBias = K == Kind::kBf16 ? 0.0f : 7.0f;
-
 template <Kind K>
 struct Types {
     using Act = __half;
@@ -53,9 +50,21 @@ struct Types<Kind::kBf16> {
     using Act = __nv_bfloat16;
 };
 
+struct TcBars {
+    uint64_t full[6], empty[6];
+    uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], done;
+    uint32_t tmem;
+    int dead;
+    Share share;
+    int run[2][128];  // per row of each tile: what its two threads tell each other
+};
+constexpr int kBarBytes = 1024 + 256;
+static_assert(sizeof(TcBars) <= kBarBytes, "barrier area");
+
 // Shared memory: Q (per MMA tile: the fp16 high and, for fp32 activations,
-// low parts; 64-dim halves of 128 rows x 128 bytes), then the ring of K and V
-// blocks in the same layout.
+// low parts; 64-dim halves of 128 rows x 128 bytes), the ring of K and V
+// blocks in the same layout, and where Q is too small for them the outputs on
+// their way out (4 KB a softmax warp).
 template <Kind K, int D>
 struct Layout {
     static constexpr int kParts = K == Kind::kF32 ? 2 : 1;
@@ -64,21 +73,15 @@ struct Layout {
     static constexpr int kPStep = 16 * kParts;
     static constexpr int kHalf = 128 * 128;
     static constexpr int kMat = D / 64 * kHalf;  // 128 rows of D 16-bit values
-    static constexpr int kStages = D == 64 ? 8 : K == Kind::kF32 ? 3 : 5;
+    static constexpr int kStages = D == 64 ? 6 : K == Kind::kF32 ? 3 : 5;
     static constexpr int kRing = 2 * kParts * kMat;
-    static constexpr int kBars = kRing + kStages * kMat;
-    static constexpr int kBytes = kBars + 512 + 1024;  // barriers and slots, alignment slack
+    static constexpr bool kOutInQ = kParts * kMat >= 8 * 4096;
+    static constexpr int kOut = kOutInQ ? 0 : kRing + kStages * kMat;
+    static constexpr int kOutTile = kOutInQ ? kParts * kMat : 8 * 4096;
+    static constexpr int kBars = kRing + kStages * kMat + (kOutInQ ? 0 : 2 * kOutTile);
+    static constexpr int kBytes = kBars + kBarBytes + 1024;  // alignment slack
     static_assert(kBytes <= 227 * 1024, "shared memory of one CTA");
 };
-
-struct TcBars {
-    uint64_t full[8], empty[8];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
-    uint32_t tmem;
-    int dead;
-    Share share;
-};
-static_assert(sizeof(TcBars) <= 512, "barrier area");
 
 // The workspace: a note per CTA and piece, then per CTA and piece the rows'
 // (m, l) and unnormalised outputs.
@@ -122,19 +125,39 @@ __device__ __forceinline__ void row_scale(float most, float& f1, float& f2) {
     f2 = __uint_as_float((uint32_t)(127 + (8 - e) - (8 - e) / 2) << 23);
 }
 
+// Signed whole numbers in the order of the floats.
+__device__ __forceinline__ int ordered(float v) {
+    const int b = __float_as_int(v);
+    return b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float from_ordered(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
+
+// ---------------------------------------------------------------------------
+// Many query rows (prompt chunks): bound by the tensor cores (4 x 512 cycles per
+// block of 256 rows x 128 keys x 128 dims) and as much by the exponentials (2048
+// cycles at 16 per cycle and SM). One MMA-issuing thread alternates between two
+// tiles of 128 rows, so that one tile's products run under the other's
+// softmax: S = Q K^T from shared memory into TMEM, probabilities back over S
+// as 16-bit values, O += P V with P from TMEM. Two threads share a row, each
+// with half of a block's keys and half of the row's output: with one thread to
+// a row the two warps of an SM sub-partition could not hide their own latencies
+// (2300 cycles for a softmax of 1024 cycles of exponentials).
+// ---------------------------------------------------------------------------
 template <Kind K, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
     paged_attention_tc_kernel(const __grid_constant__ PagedAttentionArgs a, const __grid_constant__ CUtensorMap kmap,
                               const __grid_constant__ CUtensorMap vmap, const Partials part) {
     using L = Layout<K, D>;
     using Act = typename Types<K>::Act;
+    using Walk = Pieces<kTileRows, kBlockKeys, kTileCost>;
     constexpr int kStages = L::kStages;
     constexpr uint32_t kIdescS = idesc_f16(K == Kind::kBf16, 128, kBlockKeys, false);
     constexpr uint32_t kIdescO = idesc_f16(K == Kind::kBf16, 128, D, true);
     // TMEM columns: S (its probabilities written over it) and O of each MMA tile
     constexpr uint32_t kS = 0, kO = 256;
+    constexpr int kTmaWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1;
 
-    extern __shared__ uint8_t smem_dyn[];
+    extern __shared__ __align__(1024) uint8_t smem_dyn[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
     TcBars& bar = *reinterpret_cast<TcBars*>(smem + L::kBars);
     volatile int* dead = &bar.dead;
@@ -148,249 +171,273 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&bar.empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&bar.q_full[i], 4);
+            mbar_init(&bar.q_full[i], kSoftmaxWarps / 2);
             mbar_init(&bar.s_full[i], 1);
-            mbar_init(&bar.p_full[i], 4);
+            mbar_init(&bar.p_full[i][0], kSoftmaxWarps / 4);
+            mbar_init(&bar.p_full[i][1], kSoftmaxWarps / 4);
             mbar_init(&bar.o_full[i], 1);
         }
         mbar_init(&bar.done, 1);
         bar.dead = 0;
         mbar_fence_init();
     }
-    if (warp == 9) tmem_alloc(&bar.tmem, 512);
+    if (warp == kMmaWarp) tmem_alloc(&bar.tmem, 512);
     tc_fence_before();
-    plan_share<kTileRows, kBlockKeys>(a.batch, group, a.cache.kv_heads, a.window, held, kMinUnits,
-                                      reinterpret_cast<unsigned long long*>(smem + L::kRing), &bar.share);
+    plan_share<kTileRows, kBlockKeys, kTileCost>(a.batch, group, a.cache.kv_heads, a.window, held, kMinUnits,
+                                                 reinterpret_cast<unsigned long long*>(smem + L::kRing), &bar.share);
     tc_fence_after();
     const uint32_t tmem = bar.tmem;
     fence_proxy_async();  // the plan's words, before the ring's copies land on them
     __syncthreads();
 
-    using Walk = Pieces<kTileRows, kBlockKeys>;
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-        if (warp == 8) {
-            Walk pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
-            // ---------------- TMA: K and V blocks, page by page, a lane per (page, half)
-            const int box = min(a.cache.page_size, kBlockKeys);
-            const int boxes = kBlockKeys / box;
-            const int page_in_block = lane / (D / 64), half = lane % (D / 64);
-            const uint32_t box_bytes = (uint32_t)box * D * 2;
-            int n = 0;
-            bool ok = true;
-            for (; pc.valid() && ok; pc.next()) {
-                for (int i = 0; i < pc.count && ok; ++i) {
-                    const int key0 = pc.tile.key_begin + (pc.b + i) * kBlockKeys;
-                    const int live = min(max((pc.tile.key_end - key0 + box - 1) / box, 0), boxes);
-                    int page = -1;
-                    if (page_in_block < live)
-                        page = __ldg(a.batch.page_table + (size_t)pc.s * a.batch.table_stride +
-                                     ((key0 + page_in_block * box) >> a.cache.page_shift));
-                    for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
-                        const int st = n % kStages;
-                        ok = wait_or_dead(&bar.empty[st], ((n / kStages) & 1) ^ 1, dead);
-                        if (!__all_sync(0xffffffffu, ok)) {
-                            ok = false;
-                            break;
-                        }
-                        if (lane == 0) mbar_arrive_expect_tx(&bar.full[st], live * box_bytes);
-                        __syncwarp();
-                        if (page_in_block < live)
-                            tma_load_4d(smem + L::kRing + st * L::kMat + half * L::kHalf + page_in_block * box * 128,
-                                        kv ? &vmap : &kmap, half * 64, key0 & (a.cache.page_size - 1), pc.h, page,
-                                        &bar.full[st]);
+    if (warp == kTmaWarp) {
+        // ---------------- TMA: K and V blocks, page by page, a lane per (page, half)
+        Walk pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
+        const int box = min(a.cache.page_size, kBlockKeys);
+        const int boxes = kBlockKeys / box;
+        const int page_in_block = lane / (D / 64), half = lane % (D / 64);
+        const uint32_t box_bytes = (uint32_t)box * D * 2;
+        int n = 0;
+        bool ok = true;
+        for (; pc.valid() && ok; pc.next()) {
+            for (int i = 0; i < pc.count && ok; ++i) {
+                const int key0 = pc.tile.key_begin + (pc.b + i) * kBlockKeys;
+                const int live = min(max((pc.tile.key_end - key0 + box - 1) / box, 0), boxes);
+                int page = -1;
+                if (page_in_block < live)
+                    page = __ldg(a.batch.page_table + (size_t)pc.s * a.batch.table_stride +
+                                 ((key0 + page_in_block * box) >> a.cache.page_shift));
+                for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
+                    const int st = n % kStages;
+                    ok = wait_or_dead(&bar.empty[st], ((n / kStages) & 1) ^ 1, dead);
+                    if (!__all_sync(0xffffffffu, ok)) {
+                        ok = false;
+                        break;
                     }
+                    if (lane == 0) mbar_arrive_expect_tx(&bar.full[st], live * box_bytes);
+                    __syncwarp();
+                    if (page_in_block < live)
+                        tma_load_4d(smem + L::kRing + st * L::kMat + half * L::kHalf + page_in_block * box * 128,
+                                    kv ? &vmap : &kmap, half * 64, key0 & (a.cache.page_size - 1), pc.h, page,
+                                    &bar.full[st]);
                 }
             }
-            // every copy issued has landed before the CTA can exit
-            for (int i = max(n - kStages, 0); i < n; ++i) 
-                mbar_wait_bounded(&bar.full[i % kStages], (i / kStages) & 1, nullptr, 0);
-            __syncwarp();
-        } else if (warp == 9) {
-            if (lane == 0) {
-                // ---------------- MMA issue
-                Walk pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
-                int n = 0;
-                uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-                bool ok = true;
-                const uint32_t q_addr = smem_addr(smem), ring = smem_addr(smem + L::kRing);
-                auto wait_stage = [&](int i) { return wait_or_dead(&bar.full[i % kStages], (i / kStages) & 1, dead); };
-                const uint64_t q_desc = desc_k_major(q_addr), k_desc = desc_k_major(ring);
-                const uint64_t v_desc = desc_mn_major(ring, L::kHalf);
-                auto score = [&](int t, int stage) {
-                    const uint64_t k = k_desc + (stage % kStages) * (L::kMat >> 4);
-                    uint64_t q = q_desc + t * L::kParts * (L::kMat >> 4);
+        }
+        // every copy issued has landed before the CTA can exit
+        for (int i = max(n - kStages, 0); i < n; ++i)
+            mbar_wait_bounded(&bar.full[i % kStages], (i / kStages) & 1, nullptr, 0);
+        __syncwarp();
+    } else if (warp == kMmaWarp) {
+        if (lane == 0) {
+            // ---------------- MMA issue
+            Walk pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
+            int n = 0;
+            uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+            bool ok = true;
+            const uint32_t ring = smem_addr(smem + L::kRing);
+            const uint64_t q_desc = desc_k_major(smem_addr(smem)), k_desc = desc_k_major(ring);
+            const uint64_t v_desc = desc_mn_major(ring, L::kHalf);
+            auto wait_stage = [&](int i) { return wait_or_dead(&bar.full[i % kStages], (i / kStages) & 1, dead); };
+            auto score = [&](int t, int stage) {
+                const uint64_t k = k_desc + (stage % kStages) * (L::kMat >> 4);
+                uint64_t q = q_desc + t * L::kParts * (L::kMat >> 4);
 #pragma unroll
-                    for (int pt = 0; pt < L::kParts; ++pt, q += L::kMat >> 4)
+                for (int pt = 0; pt < L::kParts; ++pt, q += L::kMat >> 4)
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk) {
-                            const uint32_t off = ((kk / 4) * L::kHalf + (kk % 4) * 32) >> 4;
-                            mma_ss(tmem + kS + 128 * t, q + off, k + off, kIdescS, (pt | kk) != 0);
-                        }
-                    tc_commit(&bar.s_full[t]);
-                };
-                auto value = [&](int t, int stage, bool accumulate) {
-                    const uint64_t v = v_desc + (stage % kStages) * (L::kMat >> 4);
-                    const uint32_t p = tmem + kS + 128 * t;
-#pragma unroll
-                    for (int kk = 0; kk < kBlockKeys / 16; ++kk)
-#pragma unroll
-                        for (int pt = 0; pt < L::kParts; ++pt)
-                            mma_ts(tmem + kO + 128 * t, p + L::kPStep * (kk / 2) + 16 * pt + 8 * (kk & 1),
-                                   v + kk * (2048 >> 4), kIdescO, accumulate || (pt | kk) != 0);
-                };
-                for (; pc.valid() && ok; pc.next()) {
-                    const int tiles = pc.tile.rows > 128 ? 2 : 1;
-                    int k_stage = n++;
-                    ok = wait_stage(k_stage);
-                    for (int t = 0; t < tiles && ok; ++t) {
-                        ok = wait_or_dead(&bar.q_full[t], q_phase[t]++ & 1, dead);
-                        if (!ok) break;
-                        tc_fence_after();
-                        score(t, k_stage);
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = ((kk / 4) * L::kHalf + (kk % 4) * 32) >> 4;
+                        mma_ss(tmem + kS + 128 * t, q + off, k + off, kIdescS, (pt | kk) != 0);
                     }
-                    tc_commit(&bar.empty[k_stage % kStages]);
-                    for (int i = 0; i < pc.count && ok; ++i) {
-                        const bool more = i + 1 < pc.count;
-                        const int v_stage = n++;
-                        if (more) k_stage = n++;
-                        for (int t = 0; t < tiles && ok; ++t) {
-                            ok = wait_or_dead(&bar.p_full[t], p_phase[t]++ & 1, dead) && wait_stage(v_stage);
+                tc_commit(&bar.s_full[t]);
+            };
+            // O += P V over one half of the block's keys
+            auto value = [&](int t, int stage, int half, bool accumulate) {
+                const uint64_t v = v_desc + (stage % kStages) * (L::kMat >> 4) + half * 4 * (2048 >> 4);
+                const uint32_t p = tmem + kS + 128 * t + L::kPStep * 2 * half;
+#pragma unroll
+                for (int kk = 0; kk < kBlockKeys / 32; ++kk)
+#pragma unroll
+                    for (int pt = 0; pt < L::kParts; ++pt)
+                        mma_ts(tmem + kO + 128 * t, p + L::kPStep * (kk / 2) + 16 * pt + 8 * (kk & 1),
+                               v + kk * (2048 >> 4), kIdescO, accumulate || (pt | kk) != 0);
+            };
+            for (; pc.valid() && ok; pc.next()) {
+                const int tiles = pc.tile.rows > 128 ? 2 : 1;
+                int k_stage = n++;
+                ok = wait_stage(k_stage);
+                for (int t = 0; t < tiles && ok; ++t) {
+                    ok = wait_or_dead(&bar.q_full[t], q_phase[t]++ & 1, dead);
+                    if (!ok) break;
+                    tc_fence_after();
+                    score(t, k_stage);
+                }
+                tc_commit(&bar.empty[k_stage % kStages]);
+                for (int i = 0; i < pc.count && ok; ++i) {
+                    const bool more = i + 1 < pc.count;
+                    const int v_stage = n++;
+                    if (more) k_stage = n++;
+                    for (int t = 0; t < tiles && ok; ++t) {
+                        const uint32_t phase = p_phase[t]++ & 1;
+                        ok = wait_stage(v_stage);
+                        for (int half = 0; half < 2 && ok; ++half) {
+                            ok = wait_or_dead(&bar.p_full[t][half], phase, dead);
                             if (!ok) break;
                             tc_fence_after();
-                            value(t, v_stage, i > 0);
-                            if (more) {
-                                ok = wait_stage(k_stage);
-                                if (!ok) break;
-                                tc_fence_after();
-                                score(t, k_stage);
-                            } else {
-                                tc_commit(&bar.o_full[t]);
-                            }
+                            value(t, v_stage, half, i > 0 || half > 0);
                         }
-                        tc_commit(&bar.empty[v_stage % kStages]);
-                        if (more) tc_commit(&bar.empty[k_stage % kStages]);
+                        if (!ok) break;
+                        if (more) {
+                            ok = wait_stage(k_stage);
+                            if (!ok) break;
+                            tc_fence_after();
+                            score(t, k_stage);
+                        } else {
+                            tc_commit(&bar.o_full[t]);
+                        }
                     }
-                }
-                if (!ok) {  // the MMAs in flight end before the TMEM is freed
-                    tc_commit(&bar.done);
-                    mbar_wait_bounded(&bar.done, 0, nullptr, 0);
+                    tc_commit(&bar.empty[v_stage % kStages]);
+                    if (more) tc_commit(&bar.empty[k_stage % kStages]);
                 }
             }
-            __syncwarp();
+            if (!ok) {  // the MMAs in flight end before the TMEM is freed
+                tc_commit(&bar.done);
+                mbar_wait_bounded(&bar.done, 0, nullptr, 0);
+            }
         }
+        __syncwarp();
     } else {
-        // ---------------- softmax: warpgroup t, a thread per query row
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        // ---------------- softmax: MMA tile t, half h of a block's keys, a thread per query row
         Walk pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
-        const int t = warp >> 2, row = tid & 127;
-        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t s_addr = tmem + kS + 128 * t + lanes, o_addr = tmem + kO + 128 * t + lanes;
+        const int t = warp >> 3, h = warp >> 2 & 1, quad = warp & 3, row = 32 * quad + lane;
+        const int pair_barrier = 1 + 4 * t + quad, tile_barrier = 9 + t;
+        const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+        const uint32_t s_addr = tmem + kS + 128 * t + lanes, o_addr = tmem + kO + 128 * t + lanes + h * (D / 2);
+        int* run = &bar.run[t][row];  // the row's largest score so far, ordered()
+        uint8_t* const qs = smem + t * L::kParts * L::kMat;
+        uint8_t* const out_stage =
+            smem + (L::kOutInQ ? t * L::kParts * L::kMat : L::kOut + t * L::kOutTile) + (warp & 7) * 4096;
         int n = 1;  // ring number of the block's V
         uint32_t items = 0, phase = 0;
-        bool ok = true, left[2] = {false, false};
-        for (; pc.valid() && ok; pc.next()) {
+        bool left[2] = {false, false};
+        // (a wait that gives up is not acted on here: every warp goes through the
+        // same barriers, and once one wait has given up the others return at once)
+        for (; pc.valid(); pc.next()) {
             const Tile& tl = pc.tile;
-            const int tile_row = 128 * t + row;
             if (tl.rows <= 128 * t) {
                 n += 2 * pc.count;
                 continue;
             }
-            const bool live = tile_row < tl.rows;
-            const int r = tl.row0 + tile_row;
+            const int r = tl.row0 + 128 * t + row;
+            const bool live = 128 * t + row < tl.rows;
             const int token = r / group, head = pc.h * group + r % group;
             const size_t out_row = (size_t)pc.seq.first_row + token;
-            // keys this row sees
-            const int position = pc.seq.position + token;
-            const int last = live ? min(position, held - 1) : -1;
-            const int first = a.window > 0 ? max(position - a.window + 1, 0) : 0;
             float c = a.scale * kLog2e;
+            named_barrier(tile_barrier, 256);  // the last piece's outputs have left the shared memory
             {
-                // Q into shared memory; fp32 rows scaled by a power of two to
-                // below 2^8 so that any fp32 query fits the fp16 parts
-                uint8_t* qs = smem + t * L::kParts * L::kMat;
-                const Act* q = static_cast<const Act*>(a.q) + (live ? out_row * a.ld_q + (size_t)head * D : 0);
-                if constexpr (K == Kind::kF32) {
-                    float most = 0.0f;
-                    for (int i = 0; i < D; i += 8) {
-                        float x[8];
-                        load_values<float, 8>(q + i, x);
+                // Q into shared memory, 16 rows a warp, whole rows at a time
+                constexpr int kChunks = D * (int)sizeof(Act) / 16;  // 16-byte words of a row
+                constexpr int kAtOnce = 32 / kChunks;               // rows of one load
+                constexpr int kBatch = 4;
+                const int chunk = lane % kChunks;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[j]));
-                    }
-                    float f1, f2;
-                    row_scale(most, f1, f2);
-                    c = c / f1 / f2;
-                    for (int i = 0; i < D / 8; ++i) {
-                        float x[8];
-                        load_values<float, 8>(q + 8 * i, x);
-                        uint4 hi, lo;
-                        split2(x[0] * f1 * f2, x[1] * f1 * f2, hi.x, lo.x);
-                        split2(x[2] * f1 * f2, x[3] * f1 * f2, hi.y, lo.y);
-                        split2(x[4] * f1 * f2, x[5] * f1 * f2, hi.z, lo.z);
-                        split2(x[6] * f1 * f2, x[7] * f1 * f2, hi.w, lo.w);
-                        if (!live) hi = lo = make_uint4(0u, 0u, 0u, 0u);
-                        uint8_t* at = qs + (i >> 3) * L::kHalf + swz128(row, i & 7);
-                        *reinterpret_cast<uint4*>(at) = hi;
-                        *reinterpret_cast<uint4*>(at + L::kMat) = lo;
-                    }
-                } else {
+                for (int it = 0; it < 16 / kAtOnce; it += kBatch) {
+                    uint4 x[kBatch];
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i) {
-                        uint4 x = __ldg(reinterpret_cast<const uint4*>(q) + i);
-                        if (!live) x = make_uint4(0u, 0u, 0u, 0u);
-                        *reinterpret_cast<uint4*>(qs + (i >> 3) * L::kHalf + swz128(row, i & 7)) = x;
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int rr = 128 * t + 16 * (warp & 7) + (it + j) * kAtOnce + lane / kChunks;
+                        const int rq = tl.row0 + rr;
+                        const Act* q = static_cast<const Act*>(a.q) + ((size_t)pc.seq.first_row + rq / group) * a.ld_q +
+                                       (size_t)(pc.h * group + rq % group) * D;
+                        x[j] = make_uint4(0u, 0u, 0u, 0u);
+                        if (rr < tl.rows) x[j] = __ldg(reinterpret_cast<const uint4*>(q) + chunk);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int rr = 16 * (warp & 7) + (it + j) * kAtOnce + lane / kChunks;
+                        if constexpr (K == Kind::kF32) {
+                            // scaled by a power of two to below 2^8, as high and low parts
+                            float v[4] = {__uint_as_float(x[j].x), __uint_as_float(x[j].y), __uint_as_float(x[j].z),
+                                          __uint_as_float(x[j].w)};
+                            float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+                            for (int o = kChunks / 2; o > 0; o >>= 1)
+                                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                            float f1, f2;
+                            row_scale(most, f1, f2);
+                            uint2 hi, lo;
+                            split2(v[0] * f1 * f2, v[1] * f1 * f2, hi.x, lo.x);
+                            split2(v[2] * f1 * f2, v[3] * f1 * f2, hi.y, lo.y);
+                            uint8_t* at = qs + (chunk >> 4) * L::kHalf + swz128(rr, chunk >> 1 & 7) + (chunk & 1) * 8;
+                            *reinterpret_cast<uint2*>(at) = hi;
+                            *reinterpret_cast<uint2*>(at + L::kMat) = lo;
+                            if (chunk == 0) bar.run[t][rr] = __float_as_int(c / f1 / f2);
+                        } else {
+                            *reinterpret_cast<uint4*>(qs + (chunk >> 3) * L::kHalf + swz128(rr, chunk & 7)) = x[j];
+                        }
                     }
                 }
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar.q_full[t]);
+                if constexpr (K == Kind::kF32) {
+                    named_barrier(tile_barrier, 256);
+                    c = __int_as_float(*run);
+                    named_barrier(pair_barrier, 64);
+                }
+                if (h == 0) *run = ordered(-CUDART_INF_F);
+                named_barrier(pair_barrier, 64);
             }
+            // keys this row sees, from this thread's first key of the piece on
+            const int position = pc.seq.position + token;
+            const int begin = tl.key_begin + pc.b * kBlockKeys;
+            int hi = (live ? min(position, held - 1) : -1) - begin - 64 * h;
+            int lo = (a.window > 0 ? max(position - a.window + 1, 0) : 0) - begin - 64 * h;
             float m = -CUDART_INF_F, l = 0.0f;
-            for (int i = 0; i < pc.count && ok; ++i, ++phase, n += 2) {
-                const int key0 = tl.key_begin + (pc.b + i) * kBlockKeys;
-                if (t == 0 && (key0 < tl.key_first || key0 + kBlockKeys > tl.key_end)) {
-                    // rows of V that no query row sees may hold anything (or
-                    // were never loaded): zeros, since 0 times them is not 0
-                    ok = wait_or_dead(&bar.full[n % kStages], (n / kStages) & 1, dead);
-                    if (!__all_sync(0xffffffffu, ok)) {
-                        ok = false;
-                        break;
-                    }
-                    const int key = key0 + row;
-                    if (key < tl.key_first || key >= tl.key_end) {
-                        uint8_t* v = smem + L::kRing + (n % kStages) * L::kMat;
+            for (int i = 0; i < pc.count; ++i, ++phase, n += 2, hi -= kBlockKeys, lo -= kBlockKeys) {
+                if (t == 0 && h == 0) {
+                    const int key0 = begin + i * kBlockKeys;
+                    if (key0 < tl.key_first || key0 + kBlockKeys > tl.key_end) {
+                        // rows of V that no query row sees may hold anything
+                        // (or were never loaded): zeros, since 0 times them is not 0
+                        wait_or_dead(&bar.full[n % kStages], (n / kStages) & 1, dead);
+                        const int key = key0 + row;
+                        if (key < tl.key_first || key >= tl.key_end) {
+                            uint8_t* v = smem + L::kRing + (n % kStages) * L::kMat;
 #pragma unroll
-                        for (int j = 0; j < D / 8; ++j)
-                            *reinterpret_cast<uint4*>(v + (j >> 3) * L::kHalf + swz128(row, j & 7)) =
-                                make_uint4(0u, 0u, 0u, 0u);
+                            for (int j = 0; j < D / 8; ++j)
+                                *reinterpret_cast<uint4*>(v + (j >> 3) * L::kHalf + swz128(row, j & 7)) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        fence_proxy_async();
                     }
-                    fence_proxy_async();
                 }
-                ok = wait_or_dead(&bar.s_full[t], phase & 1, dead);
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    break;
-                }
+                wait_or_dead(&bar.s_full[t], phase & 1, dead);
+                __syncwarp();
                 tc_fence_after();
-                uint32_t s[4][32];
+                uint32_t s[2][32];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) tmem_ld32(s_addr + 32 * j, s[j]);
+                for (int j = 0; j < 2; ++j) tmem_ld32(s_addr + 64 * h + 32 * j, s[j]);
                 tmem_wait_ld();
-                if (__any_sync(0xffffffffu, key0 + kBlockKeys - 1 > last || key0 < first)) {
-                    const int lo = first - key0, hi = last - key0;
+                if (__any_sync(0xffffffffu, hi < 63 || lo > 0)) {
 #pragma unroll
-                    for (int j = 0; j < 128; ++j)
+                    for (int j = 0; j < 64; ++j)
                         if (j < lo || j > hi) s[j >> 5][j & 31] = 0xff800000u;
                 }
                 float mx[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mx[j] = __uint_as_float(s[j][0]);
+                for (int j = 0; j < 4; ++j) mx[j] = __uint_as_float(s[j >> 1][16 * (j & 1)]);
 #pragma unroll
-                for (int e = 1; e < 32; ++e)
+                for (int e = 1; e < 15; e += 2)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) mx[j] = fmaxf(mx[j], __uint_as_float(s[j][e]));
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c;
+                    for (int j = 0; j < 4; ++j)
+                        mx[j] = max3(mx[j], __uint_as_float(s[j >> 1][16 * (j & 1) + e]),
+                                     __uint_as_float(s[j >> 1][16 * (j & 1) + e + 1]));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mx[j] = fmaxf(mx[j], __uint_as_float(s[j >> 1][16 * (j & 1) + 15]));
+                // both halves' largest, and so far
+                atomicMax(run, ordered(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c));
+                named_barrier(pair_barrier, 64);
+                const float top = from_ordered(*reinterpret_cast<volatile int*>(run));
                 if (__any_sync(0xffffffffu, top > m + kLazy)) {
                     const float mn = top > m + kLazy ? top : m;
                     if (i > 0) {
@@ -399,13 +446,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         // the score MMAs of this block were committed after the
                         // last block's value MMAs: O is at rest
 #pragma unroll 1
-                        for (int j = 0; j < D / 32; ++j) {
-                            uint32_t o[32];
-                            tmem_ld32(o_addr + 32 * j, o);
+                        for (int j = 0; j < D / 16; j += 2) {
+                            uint32_t o[16];
+                            tmem_ld16(o_addr + 8 * j, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tmem_st32(o_addr + 32 * j, o);
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st16(o_addr + 8 * j, o);
                         }
                     }
                     m = mn;
@@ -415,12 +462,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 uint64_t sum[2] = {0, 0};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    // 32 probabilities: 16 words (and 16 of low parts)
-                    uint32_t w[16], low[16];
+                    // 16 probabilities: 8 words (and 8 of low parts)
+                    uint32_t w[8], low[8];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
+                    for (int e = 0; e < 8; ++e) {
+                        const int at = 16 * (j & 1) + 2 * e;
                         const uint64_t x = fma_f32x2(
-                            pack_f32x2(__uint_as_float(s[j][2 * e]), __uint_as_float(s[j][2 * e + 1])), c2, shift2);
+                            pack_f32x2(__uint_as_float(s[j >> 1][at]), __uint_as_float(s[j >> 1][at + 1])), c2, shift2);
                         float p0, p1;
                         unpack_f32x2(x, p0, p1);
                         p0 = exp2_fast(p0);
@@ -431,8 +479,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         else
                             w[e] = pack2<K>(p0, p1);
                     }
-                    tmem_st16(s_addr + L::kPStep * j, w);
-                    if constexpr (K == Kind::kF32) tmem_st16(s_addr + L::kPStep * j + 16, low);
+                    const uint32_t col = s_addr + L::kPStep * (2 * h + (j >> 1)) + 8 * (j & 1);
+                    tmem_st8(col, w);
+                    if constexpr (K == Kind::kF32) tmem_st8(col + 16, low);
                 }
                 float sum0, sum1;
                 unpack_f32x2(add_f32x2(sum[0], sum[1]), sum0, sum1);
@@ -440,37 +489,76 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bar.p_full[t]);
+                if (lane == 0) mbar_arrive(&bar.p_full[t][h]);
             }
-            if (!ok) break;
-            ok = wait_or_dead(&bar.o_full[t], items & 1, dead);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            wait_or_dead(&bar.o_full[t], items & 1, dead);
+            __syncwarp();
             tc_fence_after();
             ++items;
+            // the row's sum, from both halves
+            if (h == 1) *run = __float_as_int(l);
+            named_barrier(pair_barrier, 64);
+            if (h == 0) {
+                l += __int_as_float(*run);
+                *run = __float_as_int(l);
+            }
+            named_barrier(pair_barrier, 64);
+            l = __int_as_float(*run);
             const bool whole = pc.whole();
-            const size_t slot = ((size_t)blockIdx.x * 2 + (pc.index > 0)) * kTileRows + tile_row;
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const size_t slot = ((size_t)blockIdx.x * 2 + (pc.index > 0)) * kTileRows + 128 * t;
+            const float inv = whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f;
+            const bool none = whole && !(l != 0.0f);
+            Act* const out = static_cast<Act*>(a.out) + out_row * a.ld_out + (size_t)head * D + h * (D / 2);
 #pragma unroll 1
-            for (int j = 0; j < D / 32; ++j) {
+            for (int j = 0; j < D / 64; ++j) {
                 uint32_t o[32];
                 tmem_ld32(o_addr + 32 * j, o);
                 tmem_wait_ld();
-                if (!live) continue;
-                float x[32];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(o[e]);
-                if (whole) {
+                for (int e = 0; e < 32; ++e) o[e] = none ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+                // 32 columns of 32 rows, turned in shared memory so that rows are
+                // written whole
+                if (sizeof(Act) == 2 && whole) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[e] = l > 0.0f ? x[e] * inv : 0.0f;
-                    store_values<Act, 32>(static_cast<Act*>(a.out) + out_row * a.ld_out + (size_t)head * D + 32 * j, x);
+                    for (int x = 0; x < 4; ++x)
+                        *reinterpret_cast<uint4*>(out_stage + lane * 64 + ((x ^ (lane >> 1 & 3)) << 4)) = make_uint4(
+                            pack2<K>(__uint_as_float(o[8 * x]), __uint_as_float(o[8 * x + 1])),
+                            pack2<K>(__uint_as_float(o[8 * x + 2]), __uint_as_float(o[8 * x + 3])),
+                            pack2<K>(__uint_as_float(o[8 * x + 4]), __uint_as_float(o[8 * x + 5])),
+                            pack2<K>(__uint_as_float(o[8 * x + 6]), __uint_as_float(o[8 * x + 7])));
+                    __syncwarp();
+#pragma unroll
+                    for (int it = 0; it < 4; ++it) {
+                        const int rr = it * 8 + lane / 4, x = lane & 3;
+                        const unsigned long long to = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), rr);
+                        const uint4 v = *reinterpret_cast<const uint4*>(out_stage + rr * 64 + ((x ^ (rr >> 1 & 3)) << 4));
+                        if (128 * t + 32 * quad + rr < tl.rows) reinterpret_cast<uint4*>(to)[4 * j + x] = v;
+                    }
                 } else {
-                    store_values<float, 32>(part.o + slot * D + 32 * j, x);
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        *reinterpret_cast<uint4*>(out_stage + lane * 128 + ((x ^ (lane & 7)) << 4)) =
+                            make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int it = 0; it < 8; ++it) {
+                        const int rr = it * 4 + lane / 8, x = lane & 7;
+                        unsigned long long to = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), rr);
+                        if (!whole)
+                            to = reinterpret_cast<unsigned long long>(part.o + (slot + 32 * quad + rr) * D + h * (D / 2));
+                        const uint4 v = *reinterpret_cast<const uint4*>(out_stage + rr * 128 + ((x ^ (rr & 7)) << 4));
+                        if (128 * t + 32 * quad + rr < tl.rows) reinterpret_cast<uint4*>(to)[8 * j + x] = v;
+                    }
                 }
+                __syncwarp();
             }
-            if (live && whole && a.lse)
-                a.lse[out_row * a.heads + head] = l > 0.0f ? (m - kBias<K> + log2f(l)) * kLn2 : -CUDART_INF_F;
+            if (h == 0 && live) {
+                if (!whole)
+                    part.ml[slot + row] = make_float2(m - kBias<K>, l);
+                else if (a.lse)
+                    a.lse[out_row * a.heads + head] = none ? -CUDART_INF_F : (m - kBias<K> + log2f(l)) * kLn2;
+            }
             if (!whole) {
-                part.ml[slot] = make_float2(m - kBias<K>, l);
                 left[pc.index > 0] = true;
                 if (tid == 0)
                     part.notes[blockIdx.x * 2 + (pc.index > 0)] = {pc.s, pc.h, pc.r, pc.b, pc.count, tl.blocks};
@@ -485,7 +573,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     pdl_launch_dependents();
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -505,6 +593,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // ---------------------------------------------------------------------------
 constexpr int kDecodeKeys = 64;
 constexpr int kDecodeMinUnits = 4;
+constexpr int kDecodeCost = 1;
 
 template <Kind K, int D, int ROWS>
 struct DecodeLayout {
@@ -596,11 +685,11 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
         bar.dead = 0;
         mbar_fence_init();
     }
-    plan_share<ROWS, kDecodeKeys>(a.batch, group, a.cache.kv_heads, a.window, held, kDecodeMinUnits,
+    plan_share<ROWS, kDecodeKeys, kDecodeCost>(a.batch, group, a.cache.kv_heads, a.window, held, kDecodeMinUnits,
                                   reinterpret_cast<unsigned long long*>(smem), &bar.share);
     fence_proxy_async();  // the plan's words, before the ring's copies land on them
     __syncthreads();
-    Pieces<ROWS, kDecodeKeys> pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
+    Pieces<ROWS, kDecodeKeys, kDecodeCost> pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
 
     if (warp == kWarps) {
         // ---------------- TMA: a lane per (K or V, page, half)

@@ -5,10 +5,11 @@
 // A tile is kRows query rows (new token x query head of one KV head) of one
 // sequence and KV head; its keys are cut into blocks of kBlock positions. The
 // blocks of all tiles, in the order sequence, KV head, tile, block, are dealt
-// out in equal contiguous shares, one per CTA: lengths of any raggedness keep
-// every CTA busy, long contexts with few rows are split over many CTAs, and
-// a CTA has at most two tiles that it shares with others (its first and its
-// last). Those leave partial sums in the workspace, which a second kernel
+// out in contiguous shares of equal cost, one per CTA, a tile costing kCost
+// blocks on top of its own (its queries and outputs): lengths of any
+// raggedness keep every CTA busy, long contexts with few rows are split over
+// many CTAs, and a CTA has at most two tiles that it shares with others (its
+// first and its last). Those leave partial sums in the workspace, which a second kernel
 // joins in the order of the CTAs.
 #pragma once
 #include "paged_device.cuh"
@@ -45,14 +46,14 @@ __device__ __forceinline__ int tiles_of(const Sequence& q, int group) {
 
 // Where a CTA's share begins, and how many blocks it is.
 struct Share {
-    int s, h, r, b;
+    int s, h, r;
+    int at;     // in the tile's units: kCost, then its blocks
     int units;
-    int ctas;  // that have a share
 };
 
 // Worked out by all threads; per_seq ([sequences] words of shared memory) and
 // out are free to use and reuse once it returns. Ends with a barrier.
-template <int kRows, int kBlock>
+template <int kRows, int kBlock, int kCost>
 __device__ __forceinline__ void plan_share(const PagedBatch& b, int group, int kv_heads, int window, int held,
                                            int min_units, unsigned long long* per_seq, Share* out) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
@@ -60,7 +61,7 @@ __device__ __forceinline__ void plan_share(const PagedBatch& b, int group, int k
         const Sequence q = sequence_of(b, s);
         const int n = tiles_of<kRows>(q, group);
         unsigned long long sum = 0;
-        for (int r = lane; r < n; r += 32) sum += tile_of<kRows, kBlock>(q, r, group, window, held).blocks;
+        for (int r = lane; r < n; r += 32) sum += tile_of<kRows, kBlock>(q, r, group, window, held).blocks + kCost;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) per_seq[s] = sum;
@@ -74,7 +75,7 @@ __device__ __forceinline__ void plan_share(const PagedBatch& b, int group, int k
         all *= kv_heads;
         const unsigned long long want = (all + min_units - 1) / min_units;
         const int ctas = want < gridDim.x ? (int)want : (int)gridDim.x;
-        Share v = {0, 0, 0, 0, 0, ctas};
+        Share v = {0, 0, 0, 0, 0};
         if ((int)blockIdx.x < ctas) {
             unsigned long long at = all * blockIdx.x / ctas;
             v.units = (int)(all * (blockIdx.x + 1) / ctas - at);
@@ -104,7 +105,7 @@ __device__ __forceinline__ void plan_share(const PagedBatch& b, int group, int k
             const int n = tiles_of<kRows>(q, group);
             for (int base = 0; base < n; base += 32) {
                 const unsigned long long mine =
-                    base + lane < n ? tile_of<kRows, kBlock>(q, base + lane, group, window, held).blocks : 0;
+                    base + lane < n ? tile_of<kRows, kBlock>(q, base + lane, group, window, held).blocks + kCost : 0;
                 unsigned long long run = mine;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -120,52 +121,61 @@ __device__ __forceinline__ void plan_share(const PagedBatch& b, int group, int k
                 }
                 at -= __shfl_sync(0xffffffffu, run, 31);
             }
-            v.b = (int)at;
+            v.at = (int)at;
         }
         if (lane == 0) *out = v;
     }
     __syncthreads();
 }
 
-// A share's pieces in turn: piece [b, b + count) of the blocks of `tile`.
-template <int kRows, int kBlock>
+// A share's pieces in turn: blocks [b, b + count) of `tile`, the index-th piece.
+template <int kRows, int kBlock, int kCost>
 struct Pieces {
     const PagedBatch& batch;
     int group, kv_heads, window, held;
-    int s, h, r, b, left, count, index;
+    int s, h, r, at, left, b, count, index;
     Sequence seq;
     Tile tile;
 
     __device__ __forceinline__ Pieces(const PagedBatch& batch, int group, int kv_heads, int window, int held,
                                       const Share& share)
         : batch(batch), group(group), kv_heads(kv_heads), window(window), held(held), s(share.s), h(share.h),
-          r(share.r), b(share.b), left(share.units), count(0), index(0) {
-        if (left > 0) enter();
-    }
-    __device__ __forceinline__ void enter() {
+          r(share.r), at(share.at), left(share.units), b(0), count(0), index(0) {
+        if (left <= 0) return;
         seq = sequence_of(batch, s);
         take();
+        if (count == 0) step();
     }
     __device__ __forceinline__ void take() {
         tile = tile_of<kRows, kBlock>(seq, r, group, window, held);
-        count = min(tile.blocks - b, left);
+        const int units = min(tile.blocks + kCost - at, left);
+        b = max(at - kCost, 0);
+        count = max(at + units - kCost, 0) - b;
+        left -= units;
     }
-    __device__ __forceinline__ bool valid() const { return left > 0; }
+    // to the next tile that has blocks in this share
+    __device__ __forceinline__ void step() {
+        count = 0;
+        while (left > 0 && count == 0) {
+            at = 0;
+            if (++r >= tiles_of<kRows>(seq, group)) {
+                r = 0;
+                if (++h == kv_heads) {
+                    h = 0;
+                    do {  // a sequence with work follows, as units are left
+                        ++s;
+                        seq = sequence_of(batch, s);
+                    } while (seq.rows == 0 && s + 1 < batch.sequences);
+                }
+            }
+            take();
+        }
+    }
+    __device__ __forceinline__ bool valid() const { return count > 0; }
     __device__ __forceinline__ bool whole() const { return b == 0 && count == tile.blocks; }
     __device__ __forceinline__ void next() {
-        left -= count;
         ++index;
-        if (left <= 0) return;
-        b = 0;
-        if (++r < tiles_of<kRows>(seq, group)) return take();
-        r = 0;
-        if (++h < kv_heads) return take();
-        h = 0;
-        do {  // a sequence with work follows, as blocks are left
-            ++s;
-            seq = sequence_of(batch, s);
-        } while (seq.rows == 0 && s + 1 < batch.sequences);
-        take();
+        step();
     }
 };
 
