@@ -23,7 +23,7 @@ enum class Kind { kF32, kF16, kBf16 };
 constexpr int kTileRows = 256;  // two MMA tiles of 128 query rows
 constexpr int kBlockKeys = 128;
 constexpr int kSoftmaxWarps = 16;  // two warpgroups per MMA tile, a thread per row and half of its keys
-constexpr int kTcThreads = (kSoftmaxWarps + 2) * 32;  // and a TMA and an MMA warp
+constexpr int kTcThreads = (kSoftmaxWarps + 3) * 32;  // and a TMA, an MMA and a piece-walking warp
 constexpr int kTileCost = 2;
 constexpr int kMinUnits = 4;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -50,15 +50,28 @@ struct Types<Kind::kBf16> {
     using Act = __nv_bfloat16;
 };
 
+// A piece as the softmax warps need it, written by a warp that walks ahead of
+// them: the walk's state and divisions take none of their registers and time.
+struct PieceInfo {
+    int count;  // blocks; 0: no more pieces
+    int first_row, position, row0, rows;  // the tile's query rows: of the batch, of the sequence
+    int h;
+    int begin, key_first, key_end;  // first key of the piece; keys that any row sees
+    int whole, slot;                // slot: which of the CTA's two partial sums
+    PieceNote note;
+};
+
 struct TcBars {
     uint64_t full[6], empty[6];
     uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], done;
+    uint64_t piece_full[2][2], piece_empty[2][2];
     uint32_t tmem;
     int dead;
     Share share;
     int run[2][128];  // per row of each tile: what its two threads tell each other
+    PieceInfo piece[2][2];  // per tile, in turn
 };
-constexpr int kBarBytes = 1024 + 256;
+constexpr int kBarBytes = 1024 + 768;
 static_assert(sizeof(TcBars) <= kBarBytes, "barrier area");
 
 // Shared memory: Q (per MMA tile: the fp16 high and, for fp32 activations,
@@ -118,11 +131,13 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 }
 
 // The power of two, as two factors, that brings a row of largest magnitude
-// `most` to below 2^8 (any fp32 row then fits fp16 parts).
-__device__ __forceinline__ void row_scale(float most, float& f1, float& f2) {
+// `most` to below 2^8 (any fp32 row then fits fp16 parts), and c divided by it.
+__device__ __forceinline__ void row_scale(float most, float c, float& f1, float& f2, float& c_out) {
     const int e = min(max((int)(__float_as_uint(most) >> 23) - 126, -100), 127);  // most < 2^e
-    f1 = __uint_as_float((uint32_t)(127 + (8 - e) / 2) << 23);
-    f2 = __uint_as_float((uint32_t)(127 + (8 - e) - (8 - e) / 2) << 23);
+    const int e1 = (8 - e) / 2, e2 = 8 - e - e1;
+    f1 = __uint_as_float((uint32_t)(127 + e1) << 23);
+    f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
+    c_out = c * __uint_as_float((uint32_t)(127 - e1) << 23) * __uint_as_float((uint32_t)(127 - e2) << 23);
 }
 
 // Signed whole numbers in the order of the floats.
@@ -155,7 +170,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     constexpr uint32_t kIdescO = idesc_f16(K == Kind::kBf16, 128, D, true);
     // TMEM columns: S (its probabilities written over it) and O of each MMA tile
     constexpr uint32_t kS = 0, kO = 256;
-    constexpr int kTmaWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1;
+    constexpr int kTmaWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1, kWalkWarp = kSoftmaxWarps + 2;
 
     extern __shared__ __align__(1024) uint8_t smem_dyn[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
@@ -176,6 +191,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             mbar_init(&bar.p_full[i][0], kSoftmaxWarps / 4);
             mbar_init(&bar.p_full[i][1], kSoftmaxWarps / 4);
             mbar_init(&bar.o_full[i], 1);
+            for (int j = 0; j < 2; ++j) {
+                mbar_init(&bar.piece_full[i][j], 1);
+                mbar_init(&bar.piece_empty[i][j], kSoftmaxWarps / 2);
+            }
         }
         mbar_init(&bar.done, 1);
         bar.dead = 0;
@@ -305,9 +324,40 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         }
         __syncwarp();
+    } else if (warp == kWalkWarp) {
+        if (lane == 0) {
+            // ---------------- the pieces, for the softmax warps of each tile; a count of 0 ends them
+            Walk pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
+            uint32_t turn[2] = {0, 0};
+            bool ok = true;
+            for (bool more = true; more && ok; pc.next()) {
+                more = pc.valid();
+                for (int t = 0; t < 2 && ok; ++t) {
+                    if (more && pc.tile.rows <= 128 * t) continue;
+                    const uint32_t slot = turn[t] & 1;
+                    ok = wait_or_dead(&bar.piece_empty[t][slot], (turn[t] >> 1 & 1) ^ 1, dead);
+                    if (!ok) break;
+                    ++turn[t];
+                    PieceInfo& pi = bar.piece[t][slot];
+                    pi.count = more ? pc.count : 0;
+                    pi.first_row = pc.seq.first_row;
+                    pi.position = pc.seq.position;
+                    pi.row0 = pc.tile.row0 + 128 * t;
+                    pi.rows = pc.tile.rows - 128 * t;
+                    pi.h = pc.h;
+                    pi.begin = pc.tile.key_begin + pc.b * kBlockKeys;
+                    pi.key_first = pc.tile.key_first;
+                    pi.key_end = pc.tile.key_end;
+                    pi.whole = pc.whole();
+                    pi.slot = pc.index > 0;
+                    pi.note = {pc.s, pc.h, pc.r, pc.b, pc.count, pc.tile.blocks};
+                    mbar_arrive(&bar.piece_full[t][slot]);
+                }
+            }
+        }
+        __syncwarp();
     } else {
         // ---------------- softmax: MMA tile t, half h of a block's keys, a thread per query row
-        Walk pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
         const int t = warp >> 3, h = warp >> 2 & 1, quad = warp & 3, row = 32 * quad + lane;
         const int pair_barrier = 1 + 4 * t + quad, tile_barrier = 9 + t;
         const uint32_t lanes = (uint32_t)(32 * quad) << 16;
@@ -317,43 +367,45 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         uint8_t* const out_stage =
             smem + (L::kOutInQ ? t * L::kParts * L::kMat : L::kOut + t * L::kOutTile) + (warp & 7) * 4096;
         int n = 1;  // ring number of the block's V
-        uint32_t items = 0, phase = 0;
-        bool left[2] = {false, false};
-        // (a wait that gives up is not acted on here: every warp goes through the
-        // same barriers, and once one wait has given up the others return at once)
-        for (; pc.valid(); pc.next()) {
-            const Tile& tl = pc.tile;
-            if (tl.rows <= 128 * t) {
-                n += 2 * pc.count;
-                continue;
-            }
-            const int r = tl.row0 + 128 * t + row;
-            const bool live = 128 * t + row < tl.rows;
-            const int token = r / group, head = pc.h * group + r % group;
-            const size_t out_row = (size_t)pc.seq.first_row + token;
+        uint32_t phase = 0;
+        int left = 0;  // bit i: partial sum i has been left
+        // (a wait that gives up is not acted on within a piece: every warp goes
+        // through the same barriers, and once one wait has given up the others
+        // return at once)
+        for (uint32_t items = 0;; ++items) {
+            const PieceInfo& pi = bar.piece[t][items & 1];
+            const bool there = wait_or_dead(&bar.piece_full[t][items & 1], items >> 1 & 1, dead);
+            // and the last piece's outputs have left the shared memory
+            if (named_barrier_or(tile_barrier, 256, !there)) break;
+            const int count = pi.count;
+            if (count == 0) break;
+            const int r = pi.row0 + row;
             float c = a.scale * kLog2e;
-            named_barrier(tile_barrier, 256);  // the last piece's outputs have left the shared memory
             {
                 // Q into shared memory, 16 rows a warp, whole rows at a time
                 constexpr int kChunks = D * (int)sizeof(Act) / 16;  // 16-byte words of a row
                 constexpr int kAtOnce = 32 / kChunks;               // rows of one load
                 constexpr int kBatch = 4;
                 const int chunk = lane % kChunks;
-#pragma unroll
-                for (int it = 0; it < 16 / kAtOnce; it += kBatch) {
+                // where the warp's rows are: lanes 0 .. 15 know theirs (null: past the tile)
+                const int r0 = 16 * (warp & 7), rq = pi.row0 + r0 + (lane & 15);
+                const Act* q = static_cast<const Act*>(a.q) + ((size_t)pi.first_row + rq / group) * a.ld_q +
+                               (size_t)(pi.h * group + rq % group) * D;
+                const unsigned long long mine =
+                    r0 + (lane & 15) < pi.rows ? reinterpret_cast<unsigned long long>(q) : 0ull;
+#pragma unroll 1
+                for (int it = 0; it < 16; it += kBatch * kAtOnce) {
                     uint4 x[kBatch];
 #pragma unroll
                     for (int j = 0; j < kBatch; ++j) {
-                        const int rr = 128 * t + 16 * (warp & 7) + (it + j) * kAtOnce + lane / kChunks;
-                        const int rq = tl.row0 + rr;
-                        const Act* q = static_cast<const Act*>(a.q) + ((size_t)pc.seq.first_row + rq / group) * a.ld_q +
-                                       (size_t)(pc.h * group + rq % group) * D;
+                        const unsigned long long from =
+                            __shfl_sync(0xffffffffu, mine, it + j * kAtOnce + lane / kChunks);
                         x[j] = make_uint4(0u, 0u, 0u, 0u);
-                        if (rr < tl.rows) x[j] = __ldg(reinterpret_cast<const uint4*>(q) + chunk);
+                        if (from) x[j] = __ldg(reinterpret_cast<const uint4*>(from) + chunk);
                     }
 #pragma unroll
                     for (int j = 0; j < kBatch; ++j) {
-                        const int rr = 16 * (warp & 7) + (it + j) * kAtOnce + lane / kChunks;
+                        const int rr = r0 + it + j * kAtOnce + lane / kChunks;
                         if constexpr (K == Kind::kF32) {
                             // scaled by a power of two to below 2^8, as high and low parts
                             float v[4] = {__uint_as_float(x[j].x), __uint_as_float(x[j].y), __uint_as_float(x[j].z),
@@ -362,15 +414,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                             for (int o = kChunks / 2; o > 0; o >>= 1)
                                 most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                            float f1, f2;
-                            row_scale(most, f1, f2);
+                            float f1, f2, row_c;
+                            row_scale(most, c, f1, f2, row_c);
                             uint2 hi, lo;
                             split2(v[0] * f1 * f2, v[1] * f1 * f2, hi.x, lo.x);
                             split2(v[2] * f1 * f2, v[3] * f1 * f2, hi.y, lo.y);
                             uint8_t* at = qs + (chunk >> 4) * L::kHalf + swz128(rr, chunk >> 1 & 7) + (chunk & 1) * 8;
                             *reinterpret_cast<uint2*>(at) = hi;
                             *reinterpret_cast<uint2*>(at + L::kMat) = lo;
-                            if (chunk == 0) bar.run[t][rr] = __float_as_int(c / f1 / f2);
+                            if (chunk == 0) bar.run[t][rr] = __float_as_int(row_c);
                         } else {
                             *reinterpret_cast<uint4*>(qs + (chunk >> 3) * L::kHalf + swz128(rr, chunk & 7)) = x[j];
                         }
@@ -388,35 +440,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 named_barrier(pair_barrier, 64);
             }
             // keys this row sees, from this thread's first key of the piece on
-            const int position = pc.seq.position + token;
-            const int begin = tl.key_begin + pc.b * kBlockKeys;
-            int hi = (live ? min(position, held - 1) : -1) - begin - 64 * h;
-            int lo = (a.window > 0 ? max(position - a.window + 1, 0) : 0) - begin - 64 * h;
+            const int position = pi.position + r / group;
+            int hi = (row < pi.rows ? min(position, held - 1) : -1) - pi.begin - 64 * h;
+            int lo = (a.window > 0 ? max(position - a.window + 1, 0) : 0) - pi.begin - 64 * h;
+            // blocks of this piece with keys that no row sees: the first, the last
+            const bool fix_first = t == 0 && h == 0 && pi.begin < pi.key_first;
+            const bool fix_last = t == 0 && h == 0 && pi.begin + count * kBlockKeys > pi.key_end;
             float m = -CUDART_INF_F, l = 0.0f;
-            for (int i = 0; i < pc.count; ++i, ++phase, n += 2, hi -= kBlockKeys, lo -= kBlockKeys) {
-                if (t == 0 && h == 0) {
-                    const int key0 = begin + i * kBlockKeys;
-                    if (key0 < tl.key_first || key0 + kBlockKeys > tl.key_end) {
-                        // rows of V that no query row sees may hold anything
-                        // (or were never loaded): zeros, since 0 times them is not 0
-                        wait_or_dead(&bar.full[n % kStages], (n / kStages) & 1, dead);
-                        const int key = key0 + row;
-                        if (key < tl.key_first || key >= tl.key_end) {
-                            uint8_t* v = smem + L::kRing + (n % kStages) * L::kMat;
+            for (int i = 0; i < count; ++i, ++phase, hi -= kBlockKeys, lo -= kBlockKeys) {
+                if ((i == 0 && fix_first) || (i == count - 1 && fix_last)) {
+                    // rows of V that no query row sees may hold anything (or
+                    // were never loaded): zeros, since 0 times them is not 0
+                    const int v_stage = n + 2 * i;
+                    wait_or_dead(&bar.full[v_stage % kStages], (v_stage / kStages) & 1, dead);
+                    const int key = pi.begin + i * kBlockKeys + row;
+                    if (key < pi.key_first || key >= pi.key_end) {
+                        uint8_t* v = smem + L::kRing + (v_stage % kStages) * L::kMat;
 #pragma unroll
-                            for (int j = 0; j < D / 8; ++j)
-                                *reinterpret_cast<uint4*>(v + (j >> 3) * L::kHalf + swz128(row, j & 7)) =
-                                    make_uint4(0u, 0u, 0u, 0u);
-                        }
-                        fence_proxy_async();
+                        for (int j = 0; j < D / 8; ++j)
+                            *reinterpret_cast<uint4*>(v + (j >> 3) * L::kHalf + swz128(row, j & 7)) =
+                                make_uint4(0u, 0u, 0u, 0u);
                     }
+                    fence_proxy_async();
                 }
                 wait_or_dead(&bar.s_full[t], phase & 1, dead);
                 __syncwarp();
                 tc_fence_after();
                 uint32_t s[2][32];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) tmem_ld32(s_addr + 64 * h + 32 * j, s[j]);
+                tmem_ld32(s_addr + 64 * h, s[0]);
+                tmem_ld32(s_addr + 64 * h + 32, s[1]);
                 tmem_wait_ld();
                 if (__any_sync(0xffffffffu, hi < 63 || lo > 0)) {
 #pragma unroll
@@ -494,7 +546,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             wait_or_dead(&bar.o_full[t], items & 1, dead);
             __syncwarp();
             tc_fence_after();
-            ++items;
+            n += 2 * count;
             // the row's sum, from both halves
             if (h == 1) *run = __float_as_int(l);
             named_barrier(pair_barrier, 64);
@@ -504,10 +556,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
             named_barrier(pair_barrier, 64);
             l = __int_as_float(*run);
-            const bool whole = pc.whole();
-            const size_t slot = ((size_t)blockIdx.x * 2 + (pc.index > 0)) * kTileRows + 128 * t;
+            const bool whole = pi.whole;
+            const size_t slot = ((size_t)blockIdx.x * 2 + pi.slot) * kTileRows + 128 * t;
             const float inv = whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f;
             const bool none = whole && !(l != 0.0f);
+            const int rows = pi.rows;
+            const int head = pi.h * group + r % group;
+            const size_t out_row = (size_t)pi.first_row + r / group;
             Act* const out = static_cast<Act*>(a.out) + out_row * a.ld_out + (size_t)head * D + h * (D / 2);
 #pragma unroll 1
             for (int j = 0; j < D / 64; ++j) {
@@ -532,7 +587,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         const int rr = it * 8 + lane / 4, x = lane & 3;
                         const unsigned long long to = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), rr);
                         const uint4 v = *reinterpret_cast<const uint4*>(out_stage + rr * 64 + ((x ^ (rr >> 1 & 3)) << 4));
-                        if (128 * t + 32 * quad + rr < tl.rows) reinterpret_cast<uint4*>(to)[4 * j + x] = v;
+                        if (32 * quad + rr < rows) reinterpret_cast<uint4*>(to)[4 * j + x] = v;
                     }
                 } else {
 #pragma unroll
@@ -547,28 +602,29 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         if (!whole)
                             to = reinterpret_cast<unsigned long long>(part.o + (slot + 32 * quad + rr) * D + h * (D / 2));
                         const uint4 v = *reinterpret_cast<const uint4*>(out_stage + rr * 128 + ((x ^ (rr & 7)) << 4));
-                        if (128 * t + 32 * quad + rr < tl.rows) reinterpret_cast<uint4*>(to)[8 * j + x] = v;
+                        if (32 * quad + rr < rows) reinterpret_cast<uint4*>(to)[8 * j + x] = v;
                     }
                 }
                 __syncwarp();
             }
-            if (h == 0 && live) {
+            if (h == 0 && row < rows) {
                 if (!whole)
                     part.ml[slot + row] = make_float2(m - kBias<K>, l);
                 else if (a.lse)
                     a.lse[out_row * a.heads + head] = none ? -CUDART_INF_F : (m - kBias<K> + log2f(l)) * kLn2;
             }
             if (!whole) {
-                left[pc.index > 0] = true;
-                if (tid == 0)
-                    part.notes[blockIdx.x * 2 + (pc.index > 0)] = {pc.s, pc.h, pc.r, pc.b, pc.count, tl.blocks};
+                left |= 1 << pi.slot;
+                if (tid == 0) part.notes[blockIdx.x * 2 + pi.slot] = pi.note;
             }
             // O has been read before the next piece's first value MMA
             tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.piece_empty[t][items & 1]);
         }
         if (tid == 0)
             for (int i = 0; i < 2; ++i)
-                if (!left[i]) part.notes[blockIdx.x * 2 + i] = {0, 0, 0, 0, 0, 0};
+                if (!(left >> i & 1)) part.notes[blockIdx.x * 2 + i] = {0, 0, 0, 0, 0, 0};
     }
     pdl_launch_dependents();
     tc_fence_before();
@@ -759,8 +815,7 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
                             most = fmaxf(most, fmaxf(fabsf(x[s][e].x), fabsf(x[s][e].y)));
                         }
                     float f1, f2;
-                    row_scale(quad_max(most), f1, f2);
-                    c[y] = c[y] / f1 / f2;
+                    row_scale(quad_max(most), c[y], f1, f2, c[y]);
 #pragma unroll
                     for (int s = 0; s < D / 16; ++s)
 #pragma unroll

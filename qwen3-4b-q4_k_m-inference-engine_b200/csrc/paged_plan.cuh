@@ -73,12 +73,17 @@ __device__ __forceinline__ void plan_share(const PagedBatch& b, int group, int k
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
         all *= kv_heads;
-        const unsigned long long want = (all + min_units - 1) / min_units;
-        const int ctas = want < gridDim.x ? (int)want : (int)gridDim.x;
+        const int ctas = all >= (unsigned long long)gridDim.x * min_units ? (int)gridDim.x
+                                                                          : ((int)all + min_units - 1) / min_units;
         Share v = {0, 0, 0, 0, 0};
         if ((int)blockIdx.x < ctas) {
-            unsigned long long at = all * blockIdx.x / ctas;
-            v.units = (int)(all * (blockIdx.x + 1) / ctas - at);
+            // (32-bit divisions where they do: the 64-bit ones take hundreds of cycles)
+            const bool small = all < (1ull << 32) / (gridDim.x + 1);
+            auto divide = [&](unsigned long long x, unsigned long long y) {
+                return small ? (unsigned long long)((uint32_t)x / (uint32_t)y) : x / y;
+            };
+            unsigned long long at = divide(all * blockIdx.x, ctas);
+            v.units = (int)(divide(all * (blockIdx.x + 1), ctas) - at);
             // the sequence, 32 at a time
             for (int base = 0; base < b.sequences; base += 32) {
                 const unsigned long long mine = base + lane < b.sequences ? per_seq[base + lane] * kv_heads : 0;
@@ -98,8 +103,8 @@ __device__ __forceinline__ void plan_share(const PagedBatch& b, int group, int k
                 at -= __shfl_sync(0xffffffffu, run, 31);
             }
             const unsigned long long head = per_seq[v.s];
-            v.h = (int)(at / head);
-            at %= head;
+            v.h = (int)divide(at, head);
+            at -= v.h * head;
             // the tile, 32 at a time
             const Sequence q = sequence_of(b, v.s);
             const int n = tiles_of<kRows>(q, group);
@@ -134,8 +139,8 @@ struct Pieces {
     const PagedBatch& batch;
     int group, kv_heads, window, held;
     int s, h, r, at, left, b, count, index;
-    Sequence seq;
-    Tile tile;
+    Sequence seq = {};
+    Tile tile = {};
 
     __device__ __forceinline__ Pieces(const PagedBatch& batch, int group, int kv_heads, int window, int held,
                                       const Share& share)
