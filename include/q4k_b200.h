@@ -241,7 +241,8 @@ typedef struct {
  * A token whose position is negative or past the page table, or whose page is
  * not one of the cache's (a negative entry marks a page to skip), is not
  * written to the cache; its query is still rotated. The paged form of
- * Engine.cpp:87-91. Buffers 16-byte aligned, ld_* whole 16-byte words. */
+ * Engine.cpp:87-91. Buffers and gammas 16-byte aligned, ld_* whole 16-byte
+ * words. */
 int q4k_paged_append(const q4k_paged_kv* cache, const q4k_paged_batch* batch, size_t tokens, int type, const void* q,
                      int64_t ld_q, int query_heads, const void* k, int64_t ld_k, const void* v, int64_t ld_v,
                      const float* q_gamma, const float* k_gamma, float epsilon, float rope_base, void* q_out,

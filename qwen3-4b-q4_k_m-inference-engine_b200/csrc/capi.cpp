@@ -473,6 +473,8 @@ Q4K_API int q4k_paged_append(const q4k_paged_kv* cache, const q4k_paged_batch* b
         if (!(rope_base > 0.0f) || std::isinf(rope_base)) invalid("RoPE requires a positive frequency base");
         if ((q_gamma || k_gamma) && !(epsilon > 0.0f)) invalid("RMSNorm requires a positive epsilon");
         if (!q != !q_out) invalid("q and q_out go together");
+        if (reinterpret_cast<uintptr_t>(q_gamma) % 16 || reinterpret_cast<uintptr_t>(k_gamma) % 16)
+            invalid("gammas must be 16-byte aligned");
         if (a.batch.sequences == 0 || a.batch.tokens == 0) return;
         a.f32 = type == Q4K_TYPE_F32;
         const int d = a.cache.head_dim;

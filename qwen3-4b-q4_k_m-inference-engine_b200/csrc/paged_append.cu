@@ -8,8 +8,10 @@
 // of each half of a row (4 fp32 or 8 16-bit values), so that a pair never
 // leaves its thread and every access is a whole 16-byte word (8-byte stores
 // where fp32 rows become fp16); a row takes 4 to 16 neighbouring lanes, whose
-// sum of squares is a few shuffles. A CTA works on rows of one token, which
-// share their angles.
+// sum of squares is a few shuffles. A CTA takes kTokens tokens: one with few
+// tokens (a decode step), so that its rows spread over several CTAs; with many
+// as many as give every thread one angle to work out, which also spreads the
+// search for the token's sequence and page over more bytes.
 //
 // Angles: far positions need more bits than fp32 has (position 1e5 has an
 // fp32 angle error of 4e-3 rad), so the turns position * (base^(-2j/d) / 2 pi)
@@ -33,60 +35,82 @@ struct Frequencies {
     double turns[kMaxHalf];  // base^(-2j/d) / (2 pi)
 };
 
-template <typename T, typename C, int HALF>
+template <typename T, typename C, int HALF, int kTokens>
 __global__ void __launch_bounds__(kAppendThreads)
     paged_append_kernel(const __grid_constant__ PagedAppendArgs a, const __grid_constant__ Frequencies f) {
     constexpr int kVec = 16 / sizeof(T);
     constexpr int kLanes = HALF / kVec;             // lanes of a row
     constexpr int kRows = kAppendThreads / kLanes;  // rows a CTA holds at a time
     constexpr int D = 2 * HALF;
-    __shared__ float cosines[HALF], sines[HALF];
-    const int t = blockIdx.x, tid = threadIdx.x;
+    constexpr int kWarps = kAppendThreads / 32;
+    static_assert(kTokens <= kWarps, "a warp finds a token's place");
+    __shared__ float cosines[kTokens][HALF], sines[kTokens][HALF];
+    __shared__ long long places[kTokens];  // cache offset of head 0's row; -1: none; -2: a row behind the last sequence
+    __shared__ int positions[kTokens];
+    const int t0 = blockIdx.x * kTokens, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int heads = a.heads, kv = a.cache.kv_heads, rows = heads + 2 * kv;
+    const int tokens = min(kTokens, a.batch.tokens - t0);
     const int j0 = tid % kLanes * kVec;
-    const int first = blockIdx.y * kRows + tid / kLanes, step = gridDim.y * kRows;
+    // work items: rows of token 0, of token 1, ...
+    const int items = tokens * rows, step = gridDim.y * kRows;
+    int item = blockIdx.y * kRows + tid / kLanes;
 
-    // row r of the token: its queries, then keys, then values
-    auto row = [&](int r) -> const T* {
-        if (r < heads) return static_cast<const T*>(a.q) + t * a.ld_q + (size_t)r * D;
-        if (r < heads + kv) return static_cast<const T*>(a.k) + t * a.ld_k + (size_t)(r - heads) * D;
-        return static_cast<const T*>(a.v) + t * a.ld_v + (size_t)(r - heads - kv) * D;
+    // row r of a token: its queries, then keys, then values
+    auto row = [&](int t, int r) -> const T* {
+        if (r < heads) return static_cast<const T*>(a.q) + (t0 + t) * a.ld_q + (size_t)r * D;
+        if (r < heads + kv) return static_cast<const T*>(a.k) + (t0 + t) * a.ld_k + (size_t)(r - heads) * D;
+        return static_cast<const T*>(a.v) + (t0 + t) * a.ld_v + (size_t)(r - heads - kv) * D;
     };
-    float x0[kVec], x1[kVec];
-    if (first < rows) {
-        load_values(row(first) + j0, x0);
-        load_values(row(first) + j0 + HALF, x1);
+    uint4 x[2];
+    auto fetch = [&](int i) {
+        if (i >= items) return;
+        const int t = kTokens == 1 ? 0 : i / rows;
+        const T* p = row(t, i - t * rows) + j0;
+        x[0] = __ldg(reinterpret_cast<const uint4*>(p));
+        x[1] = __ldg(reinterpret_cast<const uint4*>(p + HALF));
+    };
+    fetch(item);
+    if (warp < tokens) {
+        // the sequences that end at or before a token's row are those before its own
+        const int t = t0 + warp;
+        int s = 0;
+        for (int i = 0; i < a.batch.sequences; i += 32)
+            s += __popc(__ballot_sync(0xffffffffu, i + lane < a.batch.sequences && __ldg(a.batch.q_start + i + lane + 1) <= t));
+        if (lane == 0) {
+            long long place = -2;
+            int position = 0;
+            if (s < a.batch.sequences) {
+                position = __ldg(a.batch.kv_len + s) - __ldg(a.batch.q_start + s + 1) + t;
+                const int column = position >> a.cache.page_shift;
+                place = -1;  // a position that no page holds
+                if (position >= 0 && column < a.batch.table_width) {
+                    const int page = __ldg(a.batch.page_table + (size_t)s * a.batch.table_stride + column);
+                    if (page >= 0 && page < a.cache.pages)
+                        place = page * a.cache.page_stride + (position & (a.cache.page_size - 1)) * a.cache.row_stride;
+                }
+            }
+            places[warp] = place;
+            positions[warp] = position;
+        }
     }
-    // the sequences that end at or before row t are those before its own
-    int s = 0;
-    for (int i = 0; i < a.batch.sequences; i += kAppendThreads)
-        s += __syncthreads_count(i + tid < a.batch.sequences && __ldg(a.batch.q_start + i + tid + 1) <= t);
-    if (s >= a.batch.sequences) return;  // a row behind the last sequence
-    const int position = __ldg(a.batch.kv_len + s) - __ldg(a.batch.q_start + s + 1) + t;
-    const int column = position >> a.cache.page_shift;
-    // the token's page; -1 for a position that no page holds
-    int page = -1;
-    if (position >= 0 && column < a.batch.table_width)
-        page = __ldg(a.batch.page_table + (size_t)s * a.batch.table_stride + column);
-    if (page >= a.cache.pages) page = -1;
-    if (tid < HALF) {
-        const double turns = (double)position * f.turns[tid];
-        sincospif(2.0f * (float)(turns - rint(turns)), &sines[tid], &cosines[tid]);
+    __syncthreads();
+    for (int i = tid; i < tokens * HALF; i += kAppendThreads) {
+        const double turns = (double)positions[i / HALF] * f.turns[i % HALF];
+        sincospif(2.0f * (float)(turns - rint(turns)), &sines[i / HALF][i % HALF], &cosines[i / HALF][i % HALF]);
     }
     __syncthreads();
 
-    for (int r = first; r < rows; r += step) {
-        const bool is_v = r >= heads + kv;
+    for (; item < items; item += step) {
+        const int t = kTokens == 1 ? 0 : item / rows, r = item - t * rows;
         float y0[kVec], y1[kVec];
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
-            y0[i] = x0[i];
-            y1[i] = x1[i];
+            y0[i] = to_float<T>(reinterpret_cast<const T*>(&x[0])[i]);
+            y1[i] = to_float<T>(reinterpret_cast<const T*>(&x[1])[i]);
         }
-        if (r + step < rows) {
-            load_values(row(r + step) + j0, x0);
-            load_values(row(r + step) + j0 + HALF, x1);
-        }
+        fetch(item + step);
+        const long long place = places[t];
+        const bool is_v = r >= heads + kv;
         if (!is_v) {
             const float* gamma = r < heads ? a.q_gamma : a.k_gamma;
             if (gamma) {
@@ -94,43 +118,63 @@ __global__ void __launch_bounds__(kAppendThreads)
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) ss += y0[i] * y0[i] + y1[i] * y1[i];
                 // the row's lanes are neighbours, and all of them are here
-                const unsigned mask = (kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1u) << ((tid & 31) / kLanes * kLanes));
+                const unsigned mask = kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1u) << (lane / kLanes * kLanes);
 #pragma unroll
                 for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
                 const float inv = rsqrtf(ss / (float)D + a.eps);
+                float g0[kVec], g1[kVec];
+#pragma unroll
+                for (int i = 0; i < kVec; i += 4) {
+                    *reinterpret_cast<float4*>(g0 + i) = __ldg(reinterpret_cast<const float4*>(gamma + j0 + i));
+                    *reinterpret_cast<float4*>(g1 + i) = __ldg(reinterpret_cast<const float4*>(gamma + j0 + HALF + i));
+                }
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) {
-                    y0[i] = y0[i] * inv * __ldg(gamma + j0 + i);
-                    y1[i] = y1[i] * inv * __ldg(gamma + j0 + HALF + i);
+                    y0[i] = y0[i] * inv * g0[i];
+                    y1[i] = y1[i] * inv * g1[i];
                 }
             }
 #pragma unroll
             for (int i = 0; i < kVec; ++i) {
-                const float c = cosines[j0 + i], sn = sines[j0 + i], u = y0[i], w = y1[i];
+                const float c = cosines[t][j0 + i], sn = sines[t][j0 + i], u = y0[i], w = y1[i];
                 y0[i] = u * c - w * sn;
                 y1[i] = u * sn + w * c;
             }
         }
+        if (place == -2) continue;
         if (r < heads) {
-            T* o = static_cast<T*>(a.q_out) + t * a.ld_q_out + (size_t)r * D + j0;
+            T* o = static_cast<T*>(a.q_out) + (t0 + t) * a.ld_q_out + (size_t)r * D + j0;
             store_values(o, y0);
             store_values(o + HALF, y1);
-        } else if (page >= 0) {
+        } else if (place >= 0) {
             const int h = is_v ? r - heads - kv : r - heads;
-            C* o = reinterpret_cast<C*>(is_v ? a.cache.v : a.cache.k) + page * a.cache.page_stride +
-                   h * a.cache.head_stride + (position & (a.cache.page_size - 1)) * a.cache.row_stride + j0;
+            C* o = reinterpret_cast<C*>(is_v ? a.cache.v : a.cache.k) + place + h * a.cache.head_stride + j0;
             store_values(o, y0);
             store_values(o + HALF, y1);
         }
     }
 }
 
-template <typename T, typename C>
-void launch(const PagedAppendArgs& a, const Frequencies& f, dim3 grid, cudaStream_t s) {
-    if (a.cache.head_dim == 128)
-        paged_append_kernel<T, C, 64><<<grid, kAppendThreads, 0, s>>>(a, f);
+template <typename T, typename C, int HALF>
+void launch(const PagedAppendArgs& a, const Frequencies& f, cudaStream_t s) {
+    constexpr int kHeld = kAppendThreads / (HALF / (16 / (int)sizeof(T)));  // rows of a CTA at a time
+    constexpr int kMany = kAppendThreads / HALF;
+    const int rows = a.heads + 2 * a.cache.kv_heads;
+    // few tokens: a token's rows over several CTAs; measured equal near 2 tokens per SM
+    if (a.batch.tokens <= 2 * sm_count())
+        paged_append_kernel<T, C, HALF, 1>
+            <<<dim3(a.batch.tokens, (rows + kHeld - 1) / kHeld), kAppendThreads, 0, s>>>(a, f);
     else
-        paged_append_kernel<T, C, 32><<<grid, kAppendThreads, 0, s>>>(a, f);
+        paged_append_kernel<T, C, HALF, kMany>
+            <<<dim3((a.batch.tokens + kMany - 1) / kMany, 1), kAppendThreads, 0, s>>>(a, f);
+}
+
+template <typename T, typename C>
+void launch_dim(const PagedAppendArgs& a, const Frequencies& f, cudaStream_t s) {
+    if (a.cache.head_dim == 128)
+        launch<T, C, 64>(a, f, s);
+    else
+        launch<T, C, 32>(a, f, s);
 }
 
 }  // namespace
@@ -142,15 +186,12 @@ cudaError_t paged_append(const PagedAppendArgs& a, cudaStream_t s) {
     const double ratio = std::pow(a.rope_base, -2.0 / d);
     f.turns[0] = 1.0 / 6.283185307179586476925;
     for (int j = 1; j < half; ++j) f.turns[j] = f.turns[j - 1] * ratio;
-    const int rows = a.heads + 2 * a.cache.kv_heads;
-    const int held = kAppendThreads / (half / (a.f32 ? 4 : 8));
-    const dim3 grid(a.batch.tokens, (rows + held - 1) / held);
     if (a.f32)
-        launch<float, __half>(a, f, grid, s);
+        launch_dim<float, __half>(a, f, s);
     else if (a.cache.bf16)
-        launch<__nv_bfloat16, __nv_bfloat16>(a, f, grid, s);
+        launch_dim<__nv_bfloat16, __nv_bfloat16>(a, f, s);
     else
-        launch<__half, __half>(a, f, grid, s);
+        launch_dim<__half, __half>(a, f, s);
     return cudaGetLastError();
 }
 
