@@ -80,7 +80,8 @@ struct alignas(16) SampleShared {
     u64 total[kMaxCluster];  // one word from every CTA of the cluster
     float bound[2][kMaxCluster];
     Crossing crossing;
-    int place, listed;
+    u64 last;
+    int place, listed, members;
     uint64_t landed[kCopies];
 };
 
@@ -174,10 +175,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     };
     __syncthreads();
     mbar_wait_bounded(&sh.landed[warp / (kSampleWarps / kCopies)], 0, nullptr, 0);
-    float most = -CUDART_INF_F;
+    float most = -CUDART_INF_F, least_logit = CUDART_INF_F;
     for_each([&](const float(&l)[kVec], int) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) most = fmaxf(most, l[j]);
+        for (int j = 0; j < kVec; ++j) {
+            most = fmaxf(most, l[j]);
+            least_logit = fminf(least_logit, l[j] > -CUDART_INF_F ? l[j] : CUDART_INF_F);
+        }
     });
 
     // The largest and smallest of a value over the cluster.
@@ -203,7 +207,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         }
         return make_float2(high, low);
     };
-    const float top = cluster_bounds(most, most).x;
+    const float2 extent = cluster_bounds(most, least_logit);
+    const float top = extent.x;
 
     const float temperature = a.temperature ? a.temperature[row] : 1.0f;
     const bool greedy = !(temperature > 0.0f);
@@ -293,16 +298,21 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         cluster.sync();
         return sh.crossing;
     };
-    // Index of the first logit, in index order, at which the running sum of the
-    // values (value(logits, index of the first, values); 0 for -inf) over the
-    // row exceeds target(total); -1 if none does.
-    auto locate = [&](auto&& value, auto&& target, u64& total) {
+    // found(index, logit, total) for the first logit, in index order, at which
+    // the running sum of value(logit), over the row's logits with in(logit,
+    // index), exceeds target(total).
+    auto locate = [&](auto&& in, auto&& value, auto&& target, auto&& found) {
         u64 mine = 0;
         for_each([&](const float(&l)[kVec], int i) {
-            u64 v[kVec];
-            value(l, i, v);
+            bool is_in[kVec], any = false;
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) mine += v[j];
+            for (int j = 0; j < kVec; ++j) any |= is_in[j] = in(l[j], i + j);
+            if (!any) return;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) {
+                const u64 v = value(l[j]);
+                mine += is_in[j] ? v : 0;
+            }
         });
         mine = warp_total(mine);
         __syncthreads();
@@ -313,44 +323,50 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
             if (w < warp) before += sh.warp_sum[w];
             all += sh.warp_sum[w];
         }
-        if (tid == 0) sh.place = -1;
         if (tid < ranks) cluster.map_shared_rank(sh.total, tid)[rank] = all;
         cluster.sync();
-        total = 0;
+        u64 total = 0;
         for (int r = 0; r < ranks; ++r) {
             if (r < rank) before += sh.total[r];
             total += sh.total[r];
         }
         const u64 goal = target(total);
-        if (before <= goal && goal < before + mine) {
-            // this warp's stretch again, a step at a time
-            for (int s = 0; s < stretch; s += kStep) {
-                const int at = warp * stretch + s + lane * kVec;
-                const bool there = s + lane * kVec < stretch;
-                float l[kVec];
-                u64 v[kVec], sum = 0;
+        // `before` is the sum before this CTA from here on
+        for (int w = 0; w < warp; ++w) before -= sh.warp_sum[w];
+        if (before <= goal && goal < before + all) {
+            // the stretch, then all threads over it: a few consecutive logits each
+            u64 at = goal - before;
+            int owner = 0;
+            while (at >= sh.warp_sum[owner]) at -= sh.warp_sum[owner++];
+            __syncthreads();  // the sums are read: they are written again below
+            constexpr int kEach = (kMaxSlice<T> / kSampleWarps + kSampleThreads - 1) / kSampleThreads;
+            const int each = (stretch + kSampleThreads - 1) / kSampleThreads;
+            const int i0 = owner * stretch + tid * each;
+            u64 v[kEach], sum = 0;
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) l[j] = there ? to_float<T>(held[at + j]) : -CUDART_INF_F;
-                value(l, base + at, v);
+            for (int j = 0; j < kEach; ++j) {
+                const bool there = j < each && tid * each + j < stretch;
+                const float l = to_float<T>(held[there ? i0 + j : 0]);
+                v[j] = there && in(l, base + i0 + j) ? value(l) : 0;
+                sum += v[j];
+            }
+            u64 run = warp_scan(sum);
+            if (lane == 31) sh.warp_sum[warp] = run;
+            __syncthreads();
+            for (int w = 0; w < warp; ++w) run += sh.warp_sum[w];
+            run -= sum;
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) sum += v[j];
-                if (!__any_sync(0xffffffffu, sum != 0)) continue;
-                u64 run = warp_scan(sum);
-                const u64 step = __shfl_sync(0xffffffffu, run, 31);
-                if (goal >= before + step) {
-                    before += step;
-                    continue;
-                }
-                run += before - sum;
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) {
-                    if (run <= goal && goal < run + v[j])
-                        for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&sh.place, r) = base + at + j;
-                    run += v[j];
-                }
-                break;
+            for (int j = 0; j < kEach; ++j) {
+                if (run <= at && at < run + v[j]) found(base + i0 + j, to_float<T>(held[i0 + j]), total);
+                run += v[j];
             }
         }
+    };
+    // the same, its index known to every CTA of the cluster
+    auto locate_all = [&](auto&& in, auto&& value, auto&& target) {
+        locate(in, value, target, [&](int i, float, u64) {
+            for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&sh.place, r) = i;
+        });
         cluster.sync();
         return sh.place;
     };
@@ -365,22 +381,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         a.tokens[row] = token;
         if (a.logprob) {
             const double x = l == top ? 0.0 : ((double)l - (double)top) / (double)temperature;
-            a.logprob[row] = (float)(x - log((double)total / (double)(1ull << S)));
+            a.logprob[row] = token < 0 ? -CUDART_INF_F : (float)(x - log((double)total / (double)(1ull << S)));
         }
     };
 
     if (top == -CUDART_INF_F || greedy) {
-        u64 total;
-        const int i = locate(
-            [&](const float(&l)[kVec], int, u64(&v)[kVec]) {
-#pragma unroll
-                for (int j = 0; j < kVec; ++j) v[j] = l[j] == top && l[j] > -CUDART_INF_F;
-            },
-            [](u64) { return 0ull; }, total);
-        if (rank == 0 && tid == 0) {
-            a.tokens[row] = i;
-            if (a.logprob) a.logprob[row] = i < 0 ? -CUDART_INF_F : 0.0f;
-        }
+        if (rank == 0 && tid == 0 && top == -CUDART_INF_F) answer(-1, top, 0);
+        locate([&](float l, int) { return l == top && l > -CUDART_INF_F; }, [](float) { return 1ull; },
+               [](u64) { return 0ull; }, [&](int i, float l, u64) { answer(i, l, 1ull << S); });
         return;  // the last cluster.sync is behind every access of another CTA's memory
     }
     int top_k = a.top_k ? a.top_k[row] : 0;
@@ -393,9 +401,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         const double want = ceil((double)top_p * (double)all);
         return want >= 1.0 ? (u64)want : 1ull;
     };
-    // distances from the top that the first bins resolve: logits of language
-    // models lie within 64 of their largest; weights end 2^-(S+1) below theirs
-    const float count_range = 64.0f, weight_range = fminf(fmaxf(32.0f * temperature, 1e-30f), 1e30f);
+    // distances from the top that the first bins resolve: the row's extent (the
+    // more bins its logits fall into, the fewer atomics meet), but logits of
+    // language models lie within 64 of their largest, where masks need not;
+    // weights end 2^-(S+1) below theirs
+    const float span = fmaxf(top - extent.y, 1e-30f);
+    const float count_range = fminf(span, 64.0f), 
+                weight_range = fminf(fminf(span, fmaxf(32.0f * temperature, 1e-30f)), 1e30f);
 
     // the distance from the top in bins, 0 for the top itself (also where inf -
     // inf is NaN), and the nearest whole number of one below 2^22
@@ -406,6 +418,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     // The first bins: of counts where top_k cuts, else of weights
     const bool counting = top_k < a.vocab;
     Crossing first = {0, 0, 0, kBins - 1};
+    bool narrowed = false;  // the first filter's cut has been found
     const float first_scale = (float)kBins / (counting ? count_range : weight_range);
     if (counting || by_weight) {
         clear();
@@ -424,25 +437,37 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
                 for (int j = 0; j < kVec; ++j)
                     if (w[j]) add(bin_in(l[j], first_scale), w[j]);
             });
-        if (tid == 0) sh.listed = 0;
+        if (tid == 0) sh.listed = sh.members = 0;
         // fewer tokens than top_k: the last of them ends the prefix
         first = cross(0, [&](u64 all) { return counting ? min((u64)top_k, all) : share_of(all); });
-        // the candidates, to CTA 0 if they are few
+        // the candidates, and those of the last bin (in the histogram's place)
+        u64* const member = reinterpret_cast<u64*>(sh.lo);
         for_each([&](const float(&l)[kVec], int i) {
 #pragma unroll
-            for (int j = 0; j < kVec; ++j)
-                if (l[j] > -CUDART_INF_F && bin_in(l[j], first_scale) <= first.bin) {
+            for (int j = 0; j < kVec; ++j) {
+                const int bin = bin_in(l[j], first_scale);
+                if (bin <= first.bin && l[j] > -CUDART_INF_F) {
+                    const u64 key = (u64)key_of(l[j]) << 32 | (uint32_t)~(i + j);
                     const int n = atomicAdd(&sh.listed, 1);
-                    if (n < kList) sh.list_key[n] = (u64)key_of(l[j]) << 32 | (uint32_t)~(i + j);
+                    if (n < kList) sh.list_key[n] = key;
+                    if (bin == first.bin) {
+                        const int m = atomicAdd(&sh.members, 1);
+                        if (m < kList) member[m] = key;
+                    }
                 }
+            }
         });
         __syncthreads();
-        if (tid < ranks) cluster.map_shared_rank(sh.total, tid)[rank] = (u64)sh.listed;
+        if (tid < ranks) cluster.map_shared_rank(sh.total, tid)[rank] = (u64)sh.listed << 32 | (uint32_t)sh.members;
         cluster.sync();
-        int before = 0, n = 0;
+        int before = 0, n = 0, members_before = 0, members = 0;
         for (int r = 0; r < ranks; ++r) {
-            if (r < rank) before += (int)sh.total[r];
-            n += (int)sh.total[r];
+            if (r < rank) {
+                before += (int)(sh.total[r] >> 32);
+                members_before += (int)(uint32_t)sh.total[r];
+            }
+            n += (int)(sh.total[r] >> 32);
+            members += (int)(uint32_t)sh.total[r];
         }
         if (n <= kList) {
             const u64 mine = tid < sh.listed ? sh.list_key[tid] : 0;
@@ -479,6 +504,30 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
                 if (run <= goal && goal < run + w) answer(index, l, total);
             }
             return;
+        }
+        if (members <= kList) {
+            // the last one to keep, found in one CTA and told to all
+            const u64 mine = tid < sh.members ? member[tid] : 0;
+            cluster.sync();
+            if (tid < sh.members) cluster.map_shared_rank(sh.list_key, 0)[members_before + tid] = mine;
+            cluster.sync();
+            if (rank == 0) {
+                const u64 key = tid < members ? sh.list_key[tid] : 0;
+                const u64 w = tid >= members ? 0 : counting ? 1 : weight(logit_of((uint32_t)(key >> 32)));
+                sh.list_w[tid] = w;
+                __syncthreads();
+                u64 ahead = first.above;
+                if (tid < members)
+                    for (int j = 0; j < members; ++j)
+                        if (sh.list_key[j] > key) ahead += sh.list_w[j];
+                const u64 want = counting ? min((u64)top_k, first.all) : share_of(first.all);
+                if (ahead < want && want <= ahead + w)
+                    for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&sh.last, r) = key;
+            }
+            cluster.sync();
+            cut = logit_of((uint32_t)(sh.last >> 32));
+            cut_index = (int)~(uint32_t)sh.last;
+            narrowed = true;
         }
     }
 
@@ -538,20 +587,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         cut = key;
         cut_index = a.vocab;
         if (n * each < x.inside) {
-            u64 total;
-            cut_index = locate(
-                [&](const float(&l)[kVec], int i, u64(&v)[kVec]) {
-#pragma unroll
-                    for (int j = 0; j < kVec; ++j)
-                        v[j] = l[j] == key && (key > old || (key == old && i + j <= old_index));
-                },
-                [&](u64) { return n - 1; }, total);
+            cut_index = locate_all(
+                [&](float l, int i) { return l == key && (key > old || (key == old && i <= old_index)); },
+                [](float) { return 1ull; }, [&](u64) { return n - 1; });
         } else if (key == old) {
             cut_index = old_index;
         }
     };
     if (counting) {
-        narrow([](float) -> u64 { return 1; }, first, first_scale, min((u64)top_k, first.all));
+        if (!narrowed) narrow([](float) -> u64 { return 1; }, first, first_scale, min((u64)top_k, first.all));
         if (by_weight) {
             const float scale = (float)kBins / weight_range;
             clear();
@@ -563,29 +607,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
             first = cross(0, share_of);
             narrow(weight, first, scale, share_of(first.all));
         }
-    } else if (by_weight) {
+    } else if (by_weight && !narrowed) {
         narrow(weight, first, first_scale, share_of(first.all));
     }
-    u64 total;
-    const int token = locate(
-        [&](const float(&l)[kVec], int i, u64(&v)[kVec]) {
-            bool in[kVec], any = false;
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-                in[j] = kept(l[j], i + j);
-                any |= in[j];
-                v[j] = 0;
-            }
-            if (!any) return;
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-                const u64 w = weight(l[j]);
-                v[j] = in[j] && w >= least ? w : 0;
-            }
+    locate(
+        kept,
+        [&](float l) {
+            const u64 w = weight(l);
+            return w >= least ? w : 0ull;
         },
-        goal_of, total);
-    if (rank == 0 && tid == 0)
-        answer(token, to_float<T>(static_cast<const T*>(a.logits)[row * a.ld + token]), total);
+        goal_of, answer);
 }
 
 template <typename T>
