@@ -80,7 +80,7 @@ struct alignas(16) SampleShared {
     u64 total[kMaxCluster];  // one word from every CTA of the cluster
     float bound[2][kMaxCluster];
     Crossing crossing;
-    u64 last;
+    u64 last, chosen;
     int place, listed, members;
     uint64_t landed[kCopies];
 };
@@ -111,9 +111,8 @@ struct Weights {
         const double v = table[i & 63];
         const double w = p * __hiloint2double(__double2hiint(v) + (((i >> 6) + S) << 20), __double2loint(v));
         const u64 n = (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
-        // selects, not a branch: four of these run side by side. top itself
-        // where inf - inf or 0 inf is NaN
-        return (l - top) * c > cutoff ? n : l == top ? 1ull << S : 0;
+        // a select, not a branch: four of these run side by side
+        return (l - top) * c > cutoff ? n : 0;
     }
 };
 
@@ -208,11 +207,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         return make_float2(high, low);
     };
     const float2 extent = cluster_bounds(most, least_logit);
-    const float top = extent.x;
+    float top = extent.x;
+    if (top == CUDART_INF_F) {
+        // infinite logits share the row: as equal finite ones
+        for (int i = tid; i < slice; i += kSampleThreads)
+            held[i] = from_float<T>(to_float<T>(held[i]) == CUDART_INF_F ? 0.0f : -CUDART_INF_F);
+        top = 0.0f;
+        __syncthreads();
+    }
 
     const float temperature = a.temperature ? a.temperature[row] : 1.0f;
     const bool greedy = !(temperature > 0.0f);
-    const double c = 1.44269504088896340736 / (double)(greedy ? 1.0f : temperature);
+    // (a temperature below 1e-37 would make 0 / T of the top itself NaN)
+    const double c = 1.44269504088896340736 / (double)(greedy ? 1.0f : fmaxf(temperature, 1e-37f));
     const Weights weight = {top, (float)c, -(float)S - 1.0f, (double)top, 64.0 * c, S, sh.table};
 
     // kept: logits above cut, and those equal to it up to index cut_index
@@ -263,8 +270,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
             mine[j] = 0;
             if (j < q && tid * q + j < per) {
                 const int bin = rank * per + tid * q + j;
-                for (int r = 0; r < ranks; ++r)
-                    mine[j] += ((u64)cluster.map_shared_rank(sh.hi, r)[bin] << 32) + cluster.map_shared_rank(sh.lo, r)[bin];
+                // eight CTAs' loads at a time
+                for (int r0 = 0; r0 < ranks; r0 += 8) {
+                    uint32_t low[8], high[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        low[r] = r0 + r < ranks ? cluster.map_shared_rank(sh.lo, r0 + r)[bin] : 0;
+                        high[r] = r0 + r < ranks ? cluster.map_shared_rank(sh.hi, r0 + r)[bin] : 0;
+                    }
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) mine[j] += ((u64)high[r] << 32) + low[r];
+                }
                 sum += mine[j];
             }
         }
@@ -380,7 +396,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     auto answer = [&](int token, float l, u64 total) {
         a.tokens[row] = token;
         if (a.logprob) {
-            const double x = l == top ? 0.0 : ((double)l - (double)top) / (double)temperature;
+            const double x = ((double)l - (double)top) / (double)fmaxf(temperature, 1e-37f);
             a.logprob[row] = token < 0 ? -CUDART_INF_F : (float)(x - log((double)total / (double)(1ull << S)));
         }
     };
@@ -405,13 +421,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     // more bins its logits fall into, the fewer atomics meet), but logits of
     // language models lie within 64 of their largest, where masks need not;
     // weights end 2^-(S+1) below theirs
-    const float span = fmaxf(top - extent.y, 1e-30f);
+    const float span = fminf(fmaxf(top - extent.y, 1e-30f), 1e30f);
     const float count_range = fminf(span, 64.0f), 
-                weight_range = fminf(fminf(span, fmaxf(32.0f * temperature, 1e-30f)), 1e30f);
+                weight_range = fminf(span, fmaxf(32.0f * temperature, 1e-30f));
 
-    // the distance from the top in bins, 0 for the top itself (also where inf -
-    // inf is NaN), and the nearest whole number of one below 2^22
-    auto distance = [&](float l, float scale) { return fminf(fmaxf((top - l) * scale, 0.0f), (float)(kBins - 1)); };
+    // the distance from the top in bins, and the nearest whole number of one below 2^22
+    auto distance = [&](float l, float scale) { return fminf((top - l) * scale, (float)(kBins - 1)); };
     auto whole = [](float x) { return (int)(__float_as_uint(x + 8388608.0f) & 0x3fffffu); };
     auto bin_in = [&](float l, float scale) { return whole(distance(l, scale)); };
 
@@ -437,55 +452,69 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
                 for (int j = 0; j < kVec; ++j)
                     if (w[j]) add(bin_in(l[j], first_scale), w[j]);
             });
-        if (tid == 0) sh.listed = sh.members = 0;
+        if (tid == 0) sh.listed = sh.members = sh.place = 0;
         // fewer tokens than top_k: the last of them ends the prefix
         first = cross(0, [&](u64 all) { return counting ? min((u64)top_k, all) : share_of(all); });
-        // the candidates, and those of the last bin (in the histogram's place)
-        u64* const member = reinterpret_cast<u64*>(sh.lo);
-        for_each([&](const float(&l)[kVec], int i) {
+        // To CTA 0: the candidates if they are few, else those of the last bin.
+        // How many there are the counts have told; under weights it takes a pass,
+        // which brings the last bin's on the way.
+        auto send = [&](u64* list, int* counter, float l, int i) {
+            const int n = atomicAdd(cluster.map_shared_rank(counter, 0), 1);
+            if (n < kList) cluster.map_shared_rank(list, 0)[n] = (u64)key_of(l) << 32 | (uint32_t)~i;
+        };
+        u64* const member = reinterpret_cast<u64*>(sh.lo);  // the histogram's place
+        u64 n = first.above + first.inside;
+        if (!counting) {
+            u64 mine = 0;
+            for_each([&](const float(&l)[kVec], int i) {
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-                const int bin = bin_in(l[j], first_scale);
-                if (bin <= first.bin && l[j] > -CUDART_INF_F) {
-                    const u64 key = (u64)key_of(l[j]) << 32 | (uint32_t)~(i + j);
-                    const int n = atomicAdd(&sh.listed, 1);
-                    if (n < kList) sh.list_key[n] = key;
-                    if (bin == first.bin) {
-                        const int m = atomicAdd(&sh.members, 1);
-                        if (m < kList) member[m] = key;
+                for (int j = 0; j < kVec; ++j) {
+                    const int bin = bin_in(l[j], first_scale);
+                    const bool in = bin <= first.bin && l[j] > -CUDART_INF_F;
+                    mine += in;
+                    // (one too many tells of an overflow as well as all of them)
+                    if (in && bin == first.bin && *reinterpret_cast<volatile int*>(&sh.place) <= kList &&
+                        atomicAdd(&sh.place, 1) <= kList)
+                        send(member, &sh.members, l[j], i + j);
+                }
+            });
+            mine = block_total(mine);
+            if (tid < ranks) cluster.map_shared_rank(sh.total, tid)[rank] = mine;
+            cluster.sync();
+            n = 0;
+            for (int r = 0; r < ranks; ++r) n += sh.total[r];
+        }
+        if (n <= kList || (counting && first.inside <= kList)) {
+            const bool all = n <= kList;
+            for_each([&](const float(&l)[kVec], int i) {
+#pragma unroll
+                for (int j = 0; j < kVec; ++j) {
+                    const int bin = bin_in(l[j], first_scale);
+                    if ((all ? bin <= first.bin : bin == first.bin) && l[j] > -CUDART_INF_F) {
+                        if (all)
+                            send(sh.list_key, &sh.listed, l[j], i + j);
+                        else
+                            send(member, &sh.members, l[j], i + j);
                     }
                 }
-            }
-        });
-        __syncthreads();
-        if (tid < ranks) cluster.map_shared_rank(sh.total, tid)[rank] = (u64)sh.listed << 32 | (uint32_t)sh.members;
-        cluster.sync();
-        int before = 0, n = 0, members_before = 0, members = 0;
-        for (int r = 0; r < ranks; ++r) {
-            if (r < rank) {
-                before += (int)(sh.total[r] >> 32);
-                members_before += (int)(uint32_t)sh.total[r];
-            }
-            n += (int)(sh.total[r] >> 32);
-            members += (int)(uint32_t)sh.total[r];
+            });
+            cluster.sync();
         }
         if (n <= kList) {
-            const u64 mine = tid < sh.listed ? sh.list_key[tid] : 0;
-            cluster.sync();
-            if (tid < sh.listed) cluster.map_shared_rank(sh.list_key, 0)[before + tid] = mine;
-            cluster.sync();
             if (rank != 0) return;
-            const u64 key = tid < n ? sh.list_key[tid] : 0;
+            const u64 key = tid < (int)n ? sh.list_key[tid] : 0;
             const float l = logit_of((uint32_t)(key >> 32));
             const int index = (int)~(uint32_t)key;
-            u64 w = tid < n ? weight(l) : 0;
+            u64 w = tid < (int)n ? weight(l) : 0;
             sh.list_w[tid] = w;
             __syncthreads();
             // rank and weight of those before it
             int ahead = 0;
             u64 ahead_w = 0;
-            if (tid < n)
-                for (int j = 0; j < n; ++j)
+            const int listed = (int)n;
+            if (tid < listed)
+#pragma unroll 4
+                for (int j = 0; j < listed; ++j)
                     if (sh.list_key[j] > key) {
                         ++ahead;
                         ahead_w += sh.list_w[j];
@@ -499,34 +528,59 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
             const u64 goal = goal_of(total);
             if (w) {
                 u64 run = 0;
-                for (int j = 0; j < n; ++j)
+#pragma unroll 4
+                for (int j = 0; j < listed; ++j)
                     if ((uint32_t)sh.list_key[j] > (uint32_t)key) run += sh.list_w[j];  // lower indexes
                 if (run <= goal && goal < run + w) answer(index, l, total);
             }
             return;
         }
+        const int members = counting ? (int)min(first.inside, (u64)kList + 1) : *cluster.map_shared_rank(&sh.members, 0);
         if (members <= kList) {
             // the last one to keep, found in one CTA and told to all
-            const u64 mine = tid < sh.members ? member[tid] : 0;
-            cluster.sync();
-            if (tid < sh.members) cluster.map_shared_rank(sh.list_key, 0)[members_before + tid] = mine;
-            cluster.sync();
             if (rank == 0) {
-                const u64 key = tid < members ? sh.list_key[tid] : 0;
-                const u64 w = tid >= members ? 0 : counting ? 1 : weight(logit_of((uint32_t)(key >> 32)));
-                sh.list_w[tid] = w;
+                const u64 key = tid < members ? member[tid] : 0;
+                const float l = logit_of((uint32_t)(key >> 32));
+                const u64 w = tid >= members ? 0 : counting ? 1 : weight(l);
+                // kSampleThreads parts of the bin, then all with all within the part
+                // where the total passes
+                const float edge = (float)first.bin - 0.5f;
+                const int part = whole(fminf(fmaxf((distance(l, first_scale) - edge) * (float)kSampleThreads, 0.0f),
+                                             (float)(kSampleThreads - 1)));
                 __syncthreads();
-                u64 ahead = first.above;
-                if (tid < members)
-                    for (int j = 0; j < members; ++j)
-                        if (sh.list_key[j] > key) ahead += sh.list_w[j];
+                clear();
+                if (w) add(part, w);
+                if (tid == 0) sh.listed = 0;
+                __syncthreads();
+                const u64 mine_w = ((u64)sh.hi[tid] << 32) + sh.lo[tid];
+                u64 run = warp_scan(mine_w);
+                if (lane == 31) sh.warp_sum[warp] = run;
+                __syncthreads();
+                for (int i = 0; i < warp; ++i) run += sh.warp_sum[i];
+                run += first.above - mine_w;
                 const u64 want = counting ? min((u64)top_k, first.all) : share_of(first.all);
-                if (ahead < want && want <= ahead + w)
-                    for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&sh.last, r) = key;
+                if (run < want && want <= run + mine_w) {
+                    sh.place = tid;
+                    sh.last = run;
+                }
+                __syncthreads();
+                const bool passing = w && part == sh.place;
+                u64 ahead = sh.last;
+                if (passing) {
+                    const int n = atomicAdd(&sh.listed, 1);
+                    sh.list_key[n] = key;
+                    sh.list_w[n] = w;
+                }
+                __syncthreads();
+                if (passing)
+                    for (int j = 0; j < sh.listed; ++j)
+                        if (sh.list_key[j] > key) ahead += sh.list_w[j];
+                if (passing && ahead < want && want <= ahead + w)
+                    for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&sh.chosen, r) = key;
             }
             cluster.sync();
-            cut = logit_of((uint32_t)(sh.last >> 32));
-            cut_index = (int)~(uint32_t)sh.last;
+            cut = logit_of((uint32_t)(sh.chosen >> 32));
+            cut_index = (int)~(uint32_t)sh.chosen;
             narrowed = true;
         }
     }
@@ -540,24 +594,32 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
             return whole(fminf(fmaxf((distance(l, scale) - low_edge) * (float)kBins, 0.0f), (float)(kBins - 1)));
         };
         auto level = [&](u64) { return want; };
-        clear();
-        for_each([&](const float(&l)[kVec], int i) {
+        // the bin's ends (sub < 0), or those of its finer bin `sub`
+        int sub = -1;
+        auto among = [&](float l, int i) { return bin_in(l, scale) == bin && (sub < 0 || fine(l) == sub) && kept(l, i); };
+        auto ends_of = [&] {
+            float high = -CUDART_INF_F, low = CUDART_INF_F;
+            for_each([&](const float(&l)[kVec], int i) {
 #pragma unroll
-            for (int j = 0; j < kVec; ++j)
-                if (bin_in(l[j], scale) == bin && kept(l[j], i + j)) add(fine(l[j]), value(l[j]));
-        });
-        x = cross(x.above, level);
-        const int sub = x.bin;
-        float high = -CUDART_INF_F, low = CUDART_INF_F;
-        for_each([&](const float(&l)[kVec], int i) {
+                for (int j = 0; j < kVec; ++j)
+                    if (among(l[j], i + j)) high = fmaxf(high, l[j]), low = fminf(low, l[j]);
+            });
+            __syncthreads();
+            cluster.sync();  // the last bounds have been read
+            return cluster_bounds(high, low);
+        };
+        float2 ends = ends_of();
+        if (ends.x != ends.y) {
+            clear();
+            for_each([&](const float(&l)[kVec], int i) {
 #pragma unroll
-            for (int j = 0; j < kVec; ++j)
-                if (bin_in(l[j], scale) == bin && fine(l[j]) == sub && kept(l[j], i + j)) {
-                    high = fmaxf(high, l[j]);
-                    low = fminf(low, l[j]);
-                }
-        });
-        const float2 ends = cluster_bounds(high, low);
+                for (int j = 0; j < kVec; ++j)
+                    if (among(l[j], i + j)) add(fine(l[j]), value(l[j]));
+            });
+            x = cross(x.above, level);
+            sub = x.bin;
+            ends = ends_of();
+        }
         float key = ends.x;
         if (ends.x != ends.y) {
             uint32_t prefix = 0;
@@ -569,7 +631,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
                 for_each([&](const float(&l)[kVec], int i) {
 #pragma unroll 1
                     for (int j = 0; j < kVec; ++j) {
-                        if (!(bin_in(l[j], scale) == bin && fine(l[j]) == sub && kept(l[j], i + j))) continue;
+                        if (!among(l[j], i + j)) continue;
                         const uint32_t k = key_of(l[j]);
                         if (step == 0 || k >> (down + bits) == prefix)
                             add((int)(mask - (k >> down & mask)), value(l[j]));
