@@ -58,7 +58,7 @@ struct PieceInfo {
     int h;
     int begin, key_first, key_end;  // first key of the piece; keys that any row sees
     int whole, slot;                // slot: which of the CTA's two partial sums
-    PieceNote note;
+    JoinNote note;
 };
 
 struct TcBars {
@@ -99,7 +99,7 @@ struct Layout {
 // The workspace: a note per CTA and piece, then per CTA and piece the rows'
 // (m, l) and unnormalised outputs.
 struct Partials {
-    PieceNote* notes;  // [ctas][2]
+    JoinNote* notes;  // [ctas][2]
     float2* ml;        // [ctas][2][kTileRows]
     float* o;          // [ctas][2][kTileRows][D]
 };
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     pi.key_end = pc.tile.key_end;
                     pi.whole = pc.whole();
                     pi.slot = pc.index > 0;
-                    pi.note = {pc.s, pc.h, pc.r, pc.b, pc.count, pc.tile.blocks};
+                    pi.note = note_of(pc);
                     mbar_arrive(&bar.piece_full[t][slot]);
                 }
             }
@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         if (tid == 0)
             for (int i = 0; i < 2; ++i)
-                if (!(left >> i & 1)) part.notes[blockIdx.x * 2 + i] = {0, 0, 0, 0, 0, 0};
+                if (!(left >> i & 1)) part.notes[blockIdx.x * 2 + i] = {0, 0, 0, 0, 0};
     }
     pdl_launch_dependents();
     tc_fence_before();
@@ -1032,61 +1032,81 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
             if (!whole) {
                 left[pc.index > 0] = true;
                 if (tid == 0)
-                    part.notes[blockIdx.x * 2 + (pc.index > 0)] = {pc.s, pc.h, pc.r, pc.b, pc.count, tl.blocks};
+                    part.notes[blockIdx.x * 2 + (pc.index > 0)] = note_of(pc);
             }
             named_barrier(1, kWarps * 32);  // the join area may be written again
         }
         if (tid == 0)
             for (int i = 0; i < 2; ++i)
-                if (!left[i]) part.notes[blockIdx.x * 2 + i] = {0, 0, 0, 0, 0, 0};
+                if (!left[i]) part.notes[blockIdx.x * 2 + i] = {0, 0, 0, 0, 0};
     }
     pdl_launch_dependents();
 }
 
-// The tiles that several CTAs share: CTA c's block of this grid joins the
-// tile that begins in c's share and ends in a later one's, in the order of
-// the CTAs. One warp per query row.
+// The tiles that several CTAs share: block c of this grid joins the tile that
+// begins in CTA c's share and ends in a later one's, in the order of the CTAs.
+// A row's pieces are spread over as many warps as the block's rows leave (a
+// decode step over a long context: a few rows of dozens of pieces).
+constexpr int kJoinWarps = 8;
+constexpr int kJoinRows = 16;  // of a tile of 256, per block
 template <typename Act, int D, int kRows>
-__global__ void __launch_bounds__(128) paged_attention_join_kernel(const __grid_constant__ PagedAttentionArgs a,
-                                                                   const Partials part, int rows_per_block) {
+__global__ void __launch_bounds__(kJoinWarps * 32)
+    paged_attention_join_kernel(const __grid_constant__ PagedAttentionArgs a, const Partials part, int rows_per_block) {
     constexpr int V = D / 32;
+    __shared__ float sums[kJoinWarps][D + 1];
     pdl_wait();
     const int c0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int own = 1;
-    PieceNote n = part.notes[2 * c0 + 1];
-    if (n.count == 0) {
-        own = 0;
-        n = part.notes[2 * c0];
-    }
-    if (n.count == 0 || n.b != 0) return;
-    int pieces = 1;
-    for (int end = n.count; end < n.blocks && c0 + pieces < (int)gridDim.x; ++pieces)
-        end += part.notes[2 * (c0 + pieces)].count;
+    const JoinNote first = part.notes[2 * c0], second = part.notes[2 * c0 + 1];
+    const int own = second.pieces > 0;
+    const JoinNote n = own ? second : first;
+    const int begin = blockIdx.y * rows_per_block, end = min(begin + rows_per_block, n.rows);
+    if (n.pieces == 0 || begin >= end) return;
+    int spread = 1;  // warps of a row
+    while (2 * spread * (end - begin) <= kJoinWarps && 2 * spread <= n.pieces) spread *= 2;
     const int group = a.heads / a.cache.kv_heads;
-    const Sequence q = sequence_of(a.batch, n.s);
-    const int rows = min(q.rows * group - n.r * kRows, kRows);
-    const int begin = blockIdx.y * rows_per_block;
-    auto slot = [&](int i) { return (size_t)2 * (c0 + i) + (i == 0 ? own : 0); };
-    for (int row = begin + warp; row < min(begin + rows_per_block, rows); row += 4) {
-        float m = -CUDART_INF_F;
-        for (int i = lane; i < pieces; i += 32) m = fmaxf(m, part.ml[slot(i) * kRows + row].x);
-        m = warp_max(m);
-        float l = 0.0f, o[V];
+    // where (piece, row) is in the workspace
+    auto at = [&](int i, int row) { return ((size_t)2 * (c0 + i) + (i == 0 ? own : 0)) * kRows + row; };
+    for (int row0 = begin; row0 < end; row0 += kJoinWarps / spread) {
+        const int row = row0 + warp / spread, part_of = warp % spread;
+        const bool live = row < end;
+        float m = -CUDART_INF_F, l = 0.0f, o[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = 0.0f;
-        for (int i = 0; i < pieces; ++i) {
-            const size_t at = slot(i) * kRows + row;
-            const float2 ml = part.ml[at];
-            if (!(ml.y != 0.0f)) continue;
-            const float f = exp2_fast(ml.x - m);
-            l += f * ml.y;
-            const float* src = part.o + at * D + lane * V;
+        if (live) {
+            for (int i = lane; i < n.pieces; i += 32) m = fmaxf(m, part.ml[at(i, row)].x);
+            m = warp_max(m);
+#pragma unroll 4
+            for (int i = part_of; i < n.pieces; i += spread) {
+                const float2 ml = part.ml[at(i, row)];
+                const float* src = part.o + at(i, row) * D + lane * V;
+                float v[V];
+                if constexpr (V == 4)
+                    *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+                else
+                    *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+                const float f = ml.y != 0.0f ? exp2_fast(ml.x - m) : 0.0f;
+                l += f * ml.y;
 #pragma unroll
-            for (int j = 0; j < V; ++j) o[j] += f * src[j];
+                for (int j = 0; j < V; ++j) o[j] += f != 0.0f ? f * v[j] : 0.0f;
+            }
         }
-        const int r = n.r * kRows + row;
-        const int head = n.h * group + r % group;
-        const size_t out_row = (size_t)q.first_row + r / group;
+        if (spread > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < V; ++j) sums[warp][lane * V + j] = o[j];
+            if (lane == 0) sums[warp][D] = l;
+            __syncthreads();
+            if (part_of == 0)
+                for (int w = 1; w < spread; ++w) {
+                    l += sums[warp + w][D];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) o[j] += sums[warp + w][lane * V + j];
+                }
+        }
+        if (!live || part_of) continue;
+        const int r = n.row0 + row;
+        const int head = n.head + r % group;
+        const size_t out_row = (size_t)n.first_row + r / group;
         Act* out = static_cast<Act*>(a.out) + out_row * a.ld_out + (size_t)head * D + lane * V;
 #pragma unroll
         for (int j = 0; j < V; ++j) out[j] = from_float<Act>(l != 0.0f ? o[j] / l : 0.0f);
@@ -1121,10 +1141,10 @@ size_t partial_bytes(int ctas, int rows, int head_dim) {
 }
 
 Partials partials(void* workspace, int ctas, int rows) {
-    static_assert(sizeof(PieceNote) <= 32, "notes");
+    static_assert(sizeof(JoinNote) <= 32, "notes");
     Partials p;
     uint8_t* w = static_cast<uint8_t*>(workspace);
-    p.notes = reinterpret_cast<PieceNote*>(w);
+    p.notes = reinterpret_cast<JoinNote*>(w);
     p.ml = reinterpret_cast<float2*>(w + (size_t)ctas * 2 * 32);
     p.o = reinterpret_cast<float*>(w + (size_t)ctas * 2 * (32 + (size_t)rows * sizeof(float2)));
     return p;
@@ -1148,8 +1168,8 @@ cudaError_t launch_tc(const PagedAttentionArgs& a, cudaStream_t s) {
     kernel<<<ctas, kTcThreads, L::kBytes, s>>>(a, km, vm, part);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_pdl(paged_attention_join_kernel<typename Types<K>::Act, D, kTileRows>, dim3(ctas, kTileRows / 32),
-                      dim3(128), 0, s, a, part, 32);
+    return launch_pdl(paged_attention_join_kernel<typename Types<K>::Act, D, kTileRows>, dim3(ctas, kTileRows / kJoinRows),
+                      dim3(kJoinWarps * 32), 0, s, a, part, kJoinRows);
 }
 
 template <Kind K, int D, int ROWS>
@@ -1170,8 +1190,8 @@ cudaError_t launch_decode(const PagedAttentionArgs& a, cudaStream_t s) {
     kernel<<<ctas, L::kThreads, L::kBytes, s>>>(a, km, vm, part);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_pdl(paged_attention_join_kernel<typename Types<K>::Act, D, ROWS>, dim3(ctas, 1), dim3(128), 0, s, a,
-                      part, ROWS);
+    return launch_pdl(paged_attention_join_kernel<typename Types<K>::Act, D, ROWS>, dim3(ctas, 1),
+                      dim3(kJoinWarps * 32), 0, s, a, part, ROWS);
 }
 
 // Query rows per sequence and KV head up to which the decode kernel is used:

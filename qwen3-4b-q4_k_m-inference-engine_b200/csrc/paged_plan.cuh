@@ -49,6 +49,8 @@ struct Share {
     int s, h, r;
     int at;     // in the tile's units: kCost, then its blocks
     int units;
+    unsigned long long start, all;  // among all units
+    int ctas;                       // that have a share
 };
 
 // Worked out by all threads; per_seq ([sequences] words of shared memory) and
@@ -57,14 +59,29 @@ template <int kRows, int kBlock, int kCost>
 __device__ __forceinline__ void plan_share(const PagedBatch& b, int group, int kv_heads, int window, int held,
                                            int min_units, unsigned long long* per_seq, Share* out) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-    for (int s = warp; s < b.sequences; s += warps) {
-        const Sequence q = sequence_of(b, s);
+    // a thread per sequence; the tiles of a sequence of many, a lane each
+    for (int base = 32 * warp; base < b.sequences; base += 32 * warps) {
+        const int s = base + lane;
+        Sequence q = {};
+        if (s < b.sequences) q = sequence_of(b, s);
         const int n = tiles_of<kRows>(q, group);
         unsigned long long sum = 0;
-        for (int r = lane; r < n; r += 32) sum += tile_of<kRows, kBlock>(q, r, group, window, held).blocks + kCost;
+        constexpr int kFew = 2;
+        if (n <= kFew)
+            for (int r = 0; r < n; ++r) sum += tile_of<kRows, kBlock>(q, r, group, window, held).blocks + kCost;
+        for (unsigned many = __ballot_sync(0xffffffffu, n > kFew); many; many &= many - 1) {
+            const int from = __ffs(many) - 1;
+            const Sequence one = {__shfl_sync(0xffffffffu, q.first_row, from), __shfl_sync(0xffffffffu, q.rows, from),
+                                  __shfl_sync(0xffffffffu, q.position, from)};
+            const int tiles = __shfl_sync(0xffffffffu, n, from);
+            unsigned long long part = 0;
+            for (int r = lane; r < tiles; r += 32)
+                part += tile_of<kRows, kBlock>(one, r, group, window, held).blocks + kCost;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) per_seq[s] = sum;
+            for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+            if (lane == from) sum = part;
+        }
+        if (s < b.sequences) per_seq[s] = sum;
     }
     __syncthreads();
     if (warp == 0) {
@@ -75,7 +92,7 @@ __device__ __forceinline__ void plan_share(const PagedBatch& b, int group, int k
         all *= kv_heads;
         const int ctas = all >= (unsigned long long)gridDim.x * min_units ? (int)gridDim.x
                                                                           : ((int)all + min_units - 1) / min_units;
-        Share v = {0, 0, 0, 0, 0};
+        Share v = {0, 0, 0, 0, 0, 0, all, ctas};
         if ((int)blockIdx.x < ctas) {
             // (32-bit divisions where they do: the 64-bit ones take hundreds of cycles)
             const bool small = all < (1ull << 32) / (gridDim.x + 1);
@@ -83,6 +100,7 @@ __device__ __forceinline__ void plan_share(const PagedBatch& b, int group, int k
                 return small ? (unsigned long long)((uint32_t)x / (uint32_t)y) : x / y;
             };
             unsigned long long at = divide(all * blockIdx.x, ctas);
+            v.start = at;
             v.units = (int)(divide(all * (blockIdx.x + 1), ctas) - at);
             // the sequence, 32 at a time
             for (int base = 0; base < b.sequences; base += 32) {
@@ -141,11 +159,14 @@ struct Pieces {
     int s, h, r, at, left, b, count, index;
     Sequence seq = {};
     Tile tile = {};
+    unsigned long long start, all;
+    int ctas, units;
 
     __device__ __forceinline__ Pieces(const PagedBatch& batch, int group, int kv_heads, int window, int held,
                                       const Share& share)
         : batch(batch), group(group), kv_heads(kv_heads), window(window), held(held), s(share.s), h(share.h),
-          r(share.r), at(share.at), left(share.units), b(0), count(0), index(0) {
+          r(share.r), at(share.at), left(share.units), b(0), count(0), index(0), start(share.start), all(share.all),
+          ctas(share.ctas), units(share.units) {
         if (left <= 0) return;
         seq = sequence_of(batch, s);
         take();
@@ -184,12 +205,23 @@ struct Pieces {
     }
 };
 
-// What a CTA leaves for the joining kernel: of its first and last piece, where
-// they belong. Pieces 0 and 1 are different ones, or only 0 is there.
-struct PieceNote {
-    int s, h, r;
-    int b, count, blocks;  // count 0: nothing left here
+// What the joining kernel has to know of a tile that several CTAs share, left
+// by the one where it begins (pieces 0: nothing begins here). CTA c shares
+// units [all c / ctas, all (c + 1) / ctas), so unit x is CTA
+// ((x + 1) ctas - 1) / all's.
+struct JoinNote {
+    int pieces;               // of consecutive CTAs, this one's first
+    int first_row, row0, rows;  // of the batch, of the sequence, in the tile
+    int head;                 // the KV head's first query head
 };
+
+template <int kRows, int kBlock, int kCost>
+__device__ __forceinline__ JoinNote note_of(const Pieces<kRows, kBlock, kCost>& p) {
+    if (p.whole() || p.b != 0) return {0, 0, 0, 0, 0};
+    const unsigned long long end = p.start + (p.units - p.left) + (p.tile.blocks - p.count);
+    const int last = (int)((end * p.ctas - 1) / p.all);
+    return {last - (int)blockIdx.x + 1, p.seq.first_row, p.tile.row0, p.tile.rows, p.h * p.group};
+}
 
 }  // namespace paged_dev
 }  // namespace q4k
