@@ -219,13 +219,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int n = 0;
         bool ok = true;
         for (; pc.valid() && ok; pc.next()) {
+            const int* const table = a.batch.page_table + (size_t)pc.s * a.batch.table_stride;
+            auto page_of = [&](int key) {  // of this lane's box of the block
+                key += page_in_block * box;
+                return page_in_block < boxes && key < pc.tile.key_end ? __ldg(table + (key >> a.cache.page_shift)) : -1;
+            };
+            int next_page = page_of(pc.tile.key_begin + pc.b * kBlockKeys);
             for (int i = 0; i < pc.count && ok; ++i) {
                 const int key0 = pc.tile.key_begin + (pc.b + i) * kBlockKeys;
                 const int live = min(max((pc.tile.key_end - key0 + box - 1) / box, 0), boxes);
-                int page = -1;
-                if (page_in_block < live)
-                    page = __ldg(a.batch.page_table + (size_t)pc.s * a.batch.table_stride +
-                                 ((key0 + page_in_block * box) >> a.cache.page_shift));
+                const int page = next_page;
+                if (i + 1 < pc.count) next_page = page_of(key0 + kBlockKeys);  // a block ahead
                 for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
                     const int st = n % kStages;
                     ok = wait_or_dead(&bar.empty[st], ((n / kStages) & 1) ^ 1, dead);
@@ -756,13 +760,18 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
         int n = 0;
         bool ok = true;
         for (; pc.valid() && ok; pc.next()) {
+            const int* const table = a.batch.page_table + (size_t)pc.s * a.batch.table_stride;
+            auto page_of = [&](int key) {  // of this lane's box of the block
+                key += page_in_block * box;
+                return page_in_block < boxes && key < pc.tile.key_end ? __ldg(table + (key >> a.cache.page_shift)) : -1;
+            };
+            // two blocks ahead
+            int page = page_of(pc.tile.key_begin + pc.b * kDecodeKeys);
+            int next_page = page_of(pc.tile.key_begin + (pc.b + 1) * kDecodeKeys);
             for (int i = 0; i < pc.count; ++i, ++n) {
                 const int key0 = pc.tile.key_begin + (pc.b + i) * kDecodeKeys;
                 const int live = min(max((pc.tile.key_end - key0 + box - 1) / box, 0), boxes);
-                int page = -1;
-                if (page_in_block < live)
-                    page = __ldg(a.batch.page_table + (size_t)pc.s * a.batch.table_stride +
-                                 ((key0 + page_in_block * box) >> a.cache.page_shift));
+                const int far_page = page_of(key0 + 2 * kDecodeKeys);
                 const int st = n % kStages;
                 ok = wait_or_dead(&bar.empty[st], ((n / kStages) & 1) ^ 1, dead);
                 if (!__all_sync(0xffffffffu, ok)) {
@@ -775,6 +784,8 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
                     tma_load_4d(smem + st * L::kStage + kv * L::kMat + half * L::kHalf + page_in_block * box * 128,
                                 kv ? &vmap : &kmap, half * 64, key0 & (a.cache.page_size - 1), pc.h, page,
                                 &bar.full[st]);
+                page = next_page;
+                next_page = far_page;
             }
         }
         for (int i = max(n - kStages, 0); i < n; ++i)
