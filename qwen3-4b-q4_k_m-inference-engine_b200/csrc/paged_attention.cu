@@ -1201,8 +1201,8 @@ cudaError_t launch_decode(const PagedAttentionArgs& a, cudaStream_t s) {
     kernel<<<ctas, L::kThreads, L::kBytes, s>>>(a, km, vm, part);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_pdl(paged_attention_join_kernel<typename Types<K>::Act, D, ROWS>, dim3(ctas, 1),
-                      dim3(kJoinWarps * 32), 0, s, a, part, ROWS);
+    return launch_pdl(paged_attention_join_kernel<typename Types<K>::Act, D, ROWS>, dim3(ctas, ROWS / 2),
+                      dim3(kJoinWarps * 32), 0, s, a, part, 2);
 }
 
 // Query rows per sequence and KV head up to which the decode kernel is used:
