@@ -24,7 +24,7 @@ constexpr int kTileRows = 256;  // two MMA tiles of 128 query rows
 constexpr int kBlockKeys = 128;
 constexpr int kSoftmaxWarps = 16;  // two warpgroups per MMA tile, a thread per row and half of its keys
 constexpr int kTcThreads = (kSoftmaxWarps + 3) * 32;  // and a TMA, an MMA and a piece-walking warp
-constexpr int kTileCost = 2;
+constexpr int kTileCost = 4;
 constexpr int kMinUnits = 4;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -652,7 +652,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // tile when 8 rows suffice, else in two MMAs.
 // ---------------------------------------------------------------------------
 constexpr int kDecodeKeys = 64;
-constexpr int kDecodeMinUnits = 4;
+constexpr int kDecodeMinUnits = 1;
 constexpr int kDecodeCost = 1;
 
 template <Kind K, int D, int ROWS>
