@@ -37,6 +37,14 @@ constexpr float kLazy = 8.0f;
 // 2^-24, so that one of 2^-32 of the row's largest still has its low part.
 template <Kind K>
 constexpr float kBias = K == Kind::kBf16 ? 0.0f : 7.0f;
+// The tensor cores truncate their fp32 sums: each MMA takes on average half a
+// last place, kTruncation of the sum so far (2^-24 of the mean of 1 / mantissa),
+// off O. fp32 activations cannot leave it at that (1.5e-6 after 512 keys, 7e-6
+// after 4500, measured): O leaves TMEM every kFlush blocks for a sum in the
+// workspace, and what its 16 MMAs a block have taken is given back.
+constexpr float kTruncation = 0.7213f / 16777216.0f;
+constexpr int kFlush = 8;
+
 template <Kind K>
 struct Types {
     using Act = __half;
@@ -102,6 +110,7 @@ struct Partials {
     JoinNote* notes;  // [ctas][2]
     float2* ml;        // [ctas][2][kTileRows]
     float* o;          // [ctas][2][kTileRows][D]
+    float4* flushed;   // [ctas][D / 4][kTileRows]: fp32 activations' sums over a long piece
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -263,14 +272,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             auto wait_stage = [&](int i) { return wait_or_dead(&bar.full[i % kStages], (i / kStages) & 1, dead); };
             auto score = [&](int t, int stage) {
                 const uint64_t k = k_desc + (stage % kStages) * (L::kMat >> 4);
-                uint64_t q = q_desc + t * L::kParts * (L::kMat >> 4);
+                // the low parts first, while the sum is small: each MMA truncates it
+                uint64_t q = q_desc + (t + 1) * L::kParts * (L::kMat >> 4);
 #pragma unroll
-                for (int pt = 0; pt < L::kParts; ++pt, q += L::kMat >> 4)
+                for (int pt = 0; pt < L::kParts; ++pt) {
+                    q -= L::kMat >> 4;
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
                         const uint32_t off = ((kk / 4) * L::kHalf + (kk % 4) * 32) >> 4;
                         mma_ss(tmem + kS + 128 * t, q + off, k + off, kIdescS, (pt | kk) != 0);
                     }
+                }
                 tc_commit(&bar.s_full[t]);
             };
             // O += P V over one half of the block's keys
@@ -306,7 +318,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             ok = wait_or_dead(&bar.p_full[t][half], phase, dead);
                             if (!ok) break;
                             tc_fence_after();
-                            value(t, v_stage, half, i > 0 || half > 0);
+                            value(t, v_stage, half, (K == Kind::kF32 ? i % kFlush : i) > 0 || half > 0);
                         }
                         if (!ok) break;
                         if (more) {
@@ -451,6 +463,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const bool fix_first = t == 0 && h == 0 && pi.begin < pi.key_first;
             const bool fix_last = t == 0 && h == 0 && pi.begin + count * kBlockKeys > pi.key_end;
             float m = -CUDART_INF_F, l = 0.0f;
+            // fp32 activations: sums since the last flush of O are l and steps, those
+            // before it l_flushed, its reference point m_flushed
+            float steps = 0.0f, l_flushed = 0.0f, m_flushed = -CUDART_INF_F;
+            float4* const flushed = part.flushed + ((size_t)blockIdx.x * (D / 4) + h * (D / 8)) * kTileRows + 128 * t + row;
+            // The sums so far being O l' / l, with l' the row's sum then, the 16 MMAs
+            // of a block have taken 16 kTruncation sum(l') / l of O.
+            auto give_back = [&] { return l > 0.0f ? 1.0f + 16.0f * kTruncation * steps / l : 1.0f; };
+            auto flushed_factor = [&] { return m_flushed == m ? 1.0f : exp2_fast(m_flushed - m); };
             for (int i = 0; i < count; ++i, ++phase, hi -= kBlockKeys, lo -= kBlockKeys) {
                 if ((i == 0 && fix_first) || (i == count - 1 && fix_last)) {
                     // rows of V that no query row sees may hold anything (or
@@ -470,6 +490,33 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 wait_or_dead(&bar.s_full[t], phase & 1, dead);
                 __syncwarp();
                 tc_fence_after();
+                bool fresh = i == 0;  // O begins anew with this block
+                if (K == Kind::kF32 && i > 0 && i % kFlush == 0) {
+                    // the score MMAs of this block were committed after the last
+                    // block's value MMAs: O is at rest
+                    const float back = give_back(), f = i == kFlush ? 0.0f : flushed_factor();
+#pragma unroll 1
+                    for (int j = 0; j < D / 2; j += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o_addr + j, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            float4* const at = flushed + (size_t)((j + e) / 4) * kTileRows;
+                            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (i > kFlush) v = *at;
+                            v.x = fmaf(v.x, f, back * __uint_as_float(o[e]));
+                            v.y = fmaf(v.y, f, back * __uint_as_float(o[e + 1]));
+                            v.z = fmaf(v.z, f, back * __uint_as_float(o[e + 2]));
+                            v.w = fmaf(v.w, f, back * __uint_as_float(o[e + 3]));
+                            *at = v;
+                        }
+                    }
+                    m_flushed = m;
+                    l_flushed += l;
+                    l = steps = 0.0f;
+                    fresh = true;
+                }
                 uint32_t s[2][32];
                 tmem_ld32(s_addr + 64 * h, s[0]);
                 tmem_ld32(s_addr + 64 * h + 32, s[1]);
@@ -496,11 +543,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const float top = from_ordered(*reinterpret_cast<volatile int*>(run));
                 if (__any_sync(0xffffffffu, top > m + kLazy)) {
                     const float mn = top > m + kLazy ? top : m;
-                    if (i > 0) {
-                        const float f = mn == m ? 1.0f : exp2_fast(m - mn);
+                    const float f = mn == m ? 1.0f : exp2_fast(m - mn);
+                    if (K == Kind::kF32) l_flushed *= f;
+                    if (!fresh) {
                         l *= f;
-                        // the score MMAs of this block were committed after the
-                        // last block's value MMAs: O is at rest
+                        if (K == Kind::kF32) steps *= f;
+                        // (at rest, as above)
 #pragma unroll 1
                         for (int j = 0; j < D / 16; j += 2) {
                             uint32_t o[16];
@@ -541,6 +589,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 float sum0, sum1;
                 unpack_f32x2(add_f32x2(sum[0], sum[1]), sum0, sum1);
+                if (K == Kind::kF32) steps += fmaf(0.5f, sum0 + sum1, l);
                 l += sum0 + sum1;
                 tmem_wait_st();
                 tc_fence_before();
@@ -551,6 +600,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
             tc_fence_after();
             n += 2 * count;
+            const float back = K == Kind::kF32 ? give_back() : 1.0f;
+            const bool was_flushed = K == Kind::kF32 && count > kFlush;
+            const float before = was_flushed ? flushed_factor() : 0.0f;
+            if (K == Kind::kF32) l += l_flushed;
             // the row's sum, from both halves
             if (h == 1) *run = __float_as_int(l);
             named_barrier(pair_barrier, 64);
@@ -573,6 +626,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 uint32_t o[32];
                 tmem_ld32(o_addr + 32 * j, o);
                 tmem_wait_ld();
+                if constexpr (K == Kind::kF32) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) {
+                        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (was_flushed) v = flushed[(size_t)(8 * j + e / 4) * kTileRows];
+                        o[e] = __float_as_uint(fmaf(v.x, before, back * __uint_as_float(o[e])));
+                        o[e + 1] = __float_as_uint(fmaf(v.y, before, back * __uint_as_float(o[e + 1])));
+                        o[e + 2] = __float_as_uint(fmaf(v.z, before, back * __uint_as_float(o[e + 2])));
+                        o[e + 3] = __float_as_uint(fmaf(v.w, before, back * __uint_as_float(o[e + 3])));
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = none ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
                 // 32 columns of 32 rows, turned in shared memory so that rows are
@@ -1148,16 +1212,19 @@ bool page_map(const PagedCache& c, const uint16_t* base, int rows, CUtensorMap* 
 }
 
 size_t partial_bytes(int ctas, int rows, int head_dim) {
-    return (size_t)ctas * 2 * (32 + (size_t)rows * (sizeof(float2) + sizeof(float) * head_dim));
+    const size_t partial = 32 + (size_t)rows * (sizeof(float2) + sizeof(float) * head_dim);
+    const size_t flushed = rows == kTileRows ? (size_t)rows * sizeof(float) * head_dim : 0;
+    return (size_t)ctas * (2 * partial + flushed);
 }
 
-Partials partials(void* workspace, int ctas, int rows) {
+Partials partials(void* workspace, int ctas, int rows, int head_dim) {
     static_assert(sizeof(JoinNote) <= 32, "notes");
     Partials p;
     uint8_t* w = static_cast<uint8_t*>(workspace);
     p.notes = reinterpret_cast<JoinNote*>(w);
     p.ml = reinterpret_cast<float2*>(w + (size_t)ctas * 2 * 32);
     p.o = reinterpret_cast<float*>(w + (size_t)ctas * 2 * (32 + (size_t)rows * sizeof(float2)));
+    p.flushed = reinterpret_cast<float4*>(p.o + (size_t)ctas * 2 * rows * head_dim);
     return p;
 }
 
@@ -1175,7 +1242,7 @@ cudaError_t launch_tc(const PagedAttentionArgs& a, cudaStream_t s) {
     if (!page_map(a.cache, a.cache.k, kBlockKeys, &km) || !page_map(a.cache, a.cache.v, kBlockKeys, &vm))
         return cudaErrorInvalidValue;
     const int ctas = sm_count();
-    const Partials part = partials(a.workspace, ctas, kTileRows);
+    const Partials part = partials(a.workspace, ctas, kTileRows, D);
     kernel<<<ctas, kTcThreads, L::kBytes, s>>>(a, km, vm, part);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
@@ -1197,7 +1264,7 @@ cudaError_t launch_decode(const PagedAttentionArgs& a, cudaStream_t s) {
     if (!page_map(a.cache, a.cache.k, kDecodeKeys, &km) || !page_map(a.cache, a.cache.v, kDecodeKeys, &vm))
         return cudaErrorInvalidValue;
     const int ctas = sm_count();
-    const Partials part = partials(a.workspace, ctas, ROWS);
+    const Partials part = partials(a.workspace, ctas, ROWS, D);
     kernel<<<ctas, L::kThreads, L::kBytes, s>>>(a, km, vm, part);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
