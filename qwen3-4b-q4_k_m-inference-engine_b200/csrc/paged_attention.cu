@@ -65,6 +65,9 @@ struct PieceInfo {
     int first_row, position, row0, rows;  // the tile's query rows: of the batch, of the sequence
     int h;
     int begin, key_first, key_end;  // first key of the piece; keys that any row sees
+    int all_first, all_last;        // keys that every row sees
+    int poison_first, poison_last;  // keys with values that are not finite, of those that only some rows see
+    int twin;                       // tile 0: where tile 1's info is (-1: it has no rows)
     int whole, slot;                // slot: which of the CTA's two partial sums
     JoinNote note;
 };
@@ -79,7 +82,7 @@ struct TcBars {
     int run[2][128];  // per row of each tile: what its two threads tell each other
     PieceInfo piece[2][2];  // per tile, in turn
 };
-constexpr int kBarBytes = 1024 + 768;
+constexpr int kBarBytes = 1024 + 896;
 static_assert(sizeof(TcBars) <= kBarBytes, "barrier area");
 
 // Shared memory: Q (per MMA tile: the fp16 high and, for fp32 activations,
@@ -128,6 +131,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
         const __half2 v = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&v);
     }
+}
+
+// Whether 8 16-bit values are all finite: none has an exponent of ones.
+template <Kind K>
+__device__ __forceinline__ bool finite16(uint4 v) {
+    constexpr uint32_t kExp = K == Kind::kBf16 ? 0x7f807f80u : 0x7c007c00u;
+    // a half's exponent bits are all set where their complement is 0
+    auto hit = [](uint32_t w) { return __vcmpeq2(w & kExp, kExp); };
+    return (hit(v.x) | hit(v.y) | hit(v.z) | hit(v.w)) == 0;
 }
 
 // hi, lo: fp16 parts of (a, b); hi + lo is within 2^-22 of each.
@@ -348,7 +360,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             bool ok = true;
             for (bool more = true; more && ok; pc.next()) {
                 more = pc.valid();
-                for (int t = 0; t < 2 && ok; ++t) {
+                // (tile 1's first: tile 0's warps write into it)
+                for (int t = 1; t >= 0 && ok; --t) {
                     if (more && pc.tile.rows <= 128 * t) continue;
                     const uint32_t slot = turn[t] & 1;
                     ok = wait_or_dead(&bar.piece_empty[t][slot], (turn[t] >> 1 & 1) ^ 1, dead);
@@ -364,6 +377,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     pi.begin = pc.tile.key_begin + pc.b * kBlockKeys;
                     pi.key_first = pc.tile.key_first;
                     pi.key_end = pc.tile.key_end;
+                    pi.all_first = pc.tile.all_first;
+                    pi.all_last = pc.tile.all_last;
+                    pi.poison_first = 0x7fffffff;
+                    pi.poison_last = -1;
+                    pi.twin = pc.tile.rows > 128 ? (int)(turn[1] - 1 & 1) : -1;
                     pi.whole = pc.whole();
                     pi.slot = pc.index > 0;
                     pi.note = note_of(pc);
@@ -389,7 +407,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // through the same barriers, and once one wait has given up the others
         // return at once)
         for (uint32_t items = 0;; ++items) {
-            const PieceInfo& pi = bar.piece[t][items & 1];
+            PieceInfo& pi = bar.piece[t][items & 1];
             const bool there = wait_or_dead(&bar.piece_full[t][items & 1], items >> 1 & 1, dead);
             // and the last piece's outputs have left the shared memory
             if (named_barrier_or(tile_barrier, 256, !there)) break;
@@ -459,9 +477,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const int position = pi.position + r / group;
             int hi = (row < pi.rows ? min(position, held - 1) : -1) - pi.begin - 64 * h;
             int lo = (a.window > 0 ? max(position - a.window + 1, 0) : 0) - pi.begin - 64 * h;
-            // blocks of this piece with keys that no row sees: the first, the last
-            const bool fix_first = t == 0 && h == 0 && pi.begin < pi.key_first;
-            const bool fix_last = t == 0 && h == 0 && pi.begin + count * kBlockKeys > pi.key_end;
             float m = -CUDART_INF_F, l = 0.0f;
             // fp32 activations: sums since the last flush of O are l and steps, those
             // before it l_flushed, its reference point m_flushed
@@ -472,20 +487,40 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             auto give_back = [&] { return l > 0.0f ? 1.0f + 16.0f * kTruncation * steps / l : 1.0f; };
             auto flushed_factor = [&] { return m_flushed == m ? 1.0f : exp2_fast(m_flushed - m); };
             for (int i = 0; i < count; ++i, ++phase, hi -= kBlockKeys, lo -= kBlockKeys) {
-                if ((i == 0 && fix_first) || (i == count - 1 && fix_last)) {
-                    // rows of V that no query row sees may hold anything (or
-                    // were never loaded): zeros, since 0 times them is not 0
-                    const int v_stage = n + 2 * i;
-                    wait_or_dead(&bar.full[v_stage % kStages], (v_stage / kStages) & 1, dead);
-                    const int key = pi.begin + i * kBlockKeys + row;
-                    if (key < pi.key_first || key >= pi.key_end) {
+                if (t == 0 && h == 0) {
+                    const int key0 = pi.begin + i * kBlockKeys;
+                    if (key0 < pi.all_first || key0 + kBlockKeys - 1 > pi.all_last) {
+                        // V holds keys that some rows do not see, whose 0 times
+                        // what is not finite would not be 0. What no row sees (it may
+                        // never have been loaded) becomes zeros. A row of V that
+                        // is not finite becomes zeros too, and the rows that see it
+                        // NaN at the end.
+                        const int v_stage = n + 2 * i;
+                        wait_or_dead(&bar.full[v_stage % kStages], (v_stage / kStages) & 1, dead);
+                        const int key = key0 + row;
                         uint8_t* v = smem + L::kRing + (v_stage % kStages) * L::kMat;
-#pragma unroll
-                        for (int j = 0; j < D / 8; ++j)
-                            *reinterpret_cast<uint4*>(v + (j >> 3) * L::kHalf + swz128(row, j & 7)) =
-                                make_uint4(0u, 0u, 0u, 0u);
+                        bool clear = key < pi.key_first || key >= pi.key_end;
+                        if (!clear && (key < pi.all_first || key > pi.all_last)) {
+#pragma unroll 4
+                            for (int j = 0; j < D / 8; ++j)
+                                clear |= !finite16<K>(*reinterpret_cast<const uint4*>(v + (j >> 3) * L::kHalf +
+                                                                                      swz128(row, j & 7)));
+                            if (clear) {
+                                atomicMin(&pi.poison_first, key);
+                                atomicMax(&pi.poison_last, key);
+                                if (pi.twin >= 0) {
+                                    atomicMin(&bar.piece[1][pi.twin].poison_first, key);
+                                    atomicMax(&bar.piece[1][pi.twin].poison_last, key);
+                                }
+                            }
+                        }
+                        if (clear)
+#pragma unroll 4
+                            for (int j = 0; j < D / 8; ++j)
+                                *reinterpret_cast<uint4*>(v + (j >> 3) * L::kHalf + swz128(row, j & 7)) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                        fence_proxy_async();
                     }
-                    fence_proxy_async();
                 }
                 wait_or_dead(&bar.s_full[t], phase & 1, dead);
                 __syncwarp();
@@ -617,6 +652,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const size_t slot = ((size_t)blockIdx.x * 2 + pi.slot) * kTileRows + 128 * t;
             const float inv = whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f;
             const bool none = whole && !(l != 0.0f);
+            const bool poisoned = position >= pi.poison_first && (a.window == 0 || position - a.window < pi.poison_last);
             const int rows = pi.rows;
             const int head = pi.h * group + r % group;
             const size_t out_row = (size_t)pi.first_row + r / group;
@@ -639,6 +675,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
 #pragma unroll
                 for (int e = 0; e < 32; ++e) o[e] = none ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+                if (poisoned)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0x7fffffffu;
                 // 32 columns of 32 rows, turned in shared memory so that rows are
                 // written whole
                 if (sizeof(Act) == 2 && whole) {
@@ -927,17 +966,33 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
                 }
                 const int key0 = tl.key_begin + (pc.b + i) * kDecodeKeys;
                 const uint32_t kbase = smem_addr(smem + st * L::kStage), vbase = kbase + L::kMat;
-                const bool edge = key0 < tl.key_first || key0 + kDecodeKeys > tl.key_end;
+                // keys that some rows do not see: as in the other kernel, zeros for
+                // what no row sees and for what is not finite, and NaN for the
+                // rows that see the latter
+                const bool edge = key0 < tl.all_first || key0 + kDecodeKeys - 1 > tl.all_last;
+                bool nan[kR] = {};
                 if (edge) {
-                    // rows of V that no query row sees may hold anything (or
-                    // were never loaded): zeros, since 0 times them is not 0
                     uint8_t* v = smem + st * L::kStage + L::kMat;
-                    for (int row = lane; row < kDecodeKeys; row += 32)
-                        if (key0 + row < tl.key_first || key0 + row >= tl.key_end)
-#pragma unroll
+                    for (int row = lane; row < kDecodeKeys; row += 32) {
+                        const int key = key0 + row;
+                        const bool unseen = key < tl.key_first || key >= tl.key_end;
+                        bool poison = false;
+                        if (!unseen && (key < tl.all_first || key > tl.all_last))
+#pragma unroll 4
+                            for (int j = 0; j < D / 8; ++j)
+                                poison |= !finite16<K>(
+                                    *reinterpret_cast<const uint4*>(v + (j >> 3) * L::kHalf + swz128(row, j & 7)));
+                        if (unseen || poison)
+#pragma unroll 4
                             for (int j = 0; j < D / 8; ++j)
                                 *reinterpret_cast<uint4*>(v + (j >> 3) * L::kHalf + swz128(row, j & 7)) =
                                     make_uint4(0u, 0u, 0u, 0u);
+                        for (unsigned bad = __ballot_sync(0xffffffffu, poison); bad; bad &= bad - 1) {
+                            const int bad_key = key - lane + __ffs(bad) - 1;
+#pragma unroll
+                            for (int y = 0; y < kR; ++y) nan[y] |= bad_key >= first[y] && bad_key <= last[y];
+                        }
+                    }
                     __syncwarp();
                 }
                 // S = Q K^T: scores of 8 keys at a time
@@ -1043,7 +1098,14 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
                             mma16816<K>(o[j + 1], pf[kk][p], b[2], b[3]);
                         }
                     }
-                if (edge) fence_proxy_async();  // the zeros, before the next copy into this stage
+                if (edge) {
+                    fence_proxy_async();  // the zeros, before the next copy into this stage
+#pragma unroll
+                    for (int y = 0; y < kR; ++y)
+                        if (nan[y])
+#pragma unroll
+                            for (int j = 0; j < D / 8; ++j) o[j][2 * y] = o[j][2 * y + 1] = __uint_as_float(0x7fffffffu);
+                }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar.empty[st]);
             }

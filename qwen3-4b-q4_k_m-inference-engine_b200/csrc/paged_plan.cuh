@@ -23,6 +23,8 @@ struct Tile {
     int key_begin;         // first key any row sees, rounded down to a block
     int key_first;         // first key any row sees
     int key_end;           // past the last key any row sees
+    int all_first;         // keys that every row sees: all_first ..
+    int all_last;          // .. all_last
     int blocks;            // at least 1 (its outputs have to be written)
 };
 
@@ -34,6 +36,8 @@ __device__ __forceinline__ Tile tile_of(const Sequence& q, int r, int group, int
     const int first = q.position + t.row0 / group, last = q.position + (t.row0 + t.rows - 1) / group;
     t.key_end = max(min(last, held - 1) + 1, 0);
     t.key_first = window > 0 ? max(first - window + 1, 0) : 0;
+    t.all_first = window > 0 ? max(last - window + 1, 0) : 0;
+    t.all_last = min(first, held - 1);
     t.key_begin = t.key_first & ~(kBlock - 1);
     t.blocks = max((t.key_end - t.key_begin + kBlock - 1) / kBlock, 1);
     return t;

@@ -172,6 +172,46 @@ def test_attention_ignores_what_no_row_sees(kind, new, ctx):
     assert all(torch.equal(x, y) for x, y in zip(windowed, again))
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("new,ctx,heads,kv", [([5], [70], 4, 2), ([2, 3], [131, 64], 4, 1), ([150, 3], [400, 3], 8, 2), ([300], [300], 2, 2)])
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attention_new_tokens_do_not_see_later_ones(kind, new, ctx, heads, kv, window, bad):
+    """A new token whose key and value are not finite: those that do not attend to it keep their results to the bit,
+    those that do are not finite."""
+    c = Case(new, ctx, kind=kind, heads=heads, kv=kv)
+    clean, _ = c.attend(window=window)
+    n, length = new[0], ctx[0]
+    at = length - n + n // 2
+    page, slot = int(c.table[0, at // 16]), at % 16
+    c.v[page, :, slot] = bad
+    for poison_key in (False, True):
+        if poison_key:
+            c.k[page, :, slot] = bad
+        out, _ = c.attend(window=window)
+        position = torch.arange(length - n, length, device="cuda")
+        sees = (position >= at) & ((position - window < at) if window else torch.ones_like(position, dtype=torch.bool))
+        assert torch.equal(out[:n][~sees], clean[:n][~sees]) and torch.equal(out[n:], clean[n:])
+        assert not out[:n][sees].isfinite().any()
+
+
+@pytest.mark.parametrize("new,ctx,d", [([2100], [9000], 64), ([700, 1], [5000, 4000], 128)])
+def test_attention_fp32_over_many_blocks(new, ctx, d):
+    """Sums over hundreds of products keep fp32 accuracy: as accurate as fp32 sums of the same length (2^-24 times the
+    square root of the keys, 95 here) with the queries' and probabilities' 2^-22."""
+    c = Case(new, ctx, kind="f32", heads=32, kv=8, d=d, page=64)
+    out, _ = c.attend()
+    start = 0
+    for i, (n, length) in enumerate(zip(new, ctx)):
+        k, v = (ref.paged_rows(t, c.table[i], length) for t in (c.k, c.v))
+        for a in range(0, n, 700):
+            b = min(n, a + 700)
+            for h in range(0, 32, 8):
+                want, *_ = ref.attention(c.q[start + a:start + b, h:h + 8], k[h // 4:h // 4 + 2], v[h // 4:h // 4 + 2], length - n + a, d ** -0.5)
+                assert (out[start + a:start + b, h:h + 8].double() - want).norm() <= (95 * 2.0 ** -24 + 2.0 ** -21) * want.norm()
+        start += n
+
+
 @pytest.mark.parametrize("size", [1e-4, 30.0, 3000.0])
 @pytest.mark.parametrize("kind", TYPES)
 def test_attention_score_sizes(size, kind):
