@@ -258,7 +258,9 @@ int q4k_paged_append(const q4k_paged_kv* cache, const q4k_paged_batch* batch, si
  * outside the cache read as zero keys and values. fp32 activations keep fp32
  * accuracy (queries and probabilities enter the tensor cores as fp16 high and
  * low parts); 16-bit ones round their probabilities to 16 bits, sums are
- * fp32. workspace: q4k_paged_attention_workspace_bytes of the same call's
+ * fp32. Keys and values that are not finite only reach the tokens that attend
+ * to them (all of whose outputs may then be NaN); what stands in pages behind
+ * a sequence's end reaches none. workspace: q4k_paged_attention_workspace_bytes of the same call's
  * numbers, 16-byte aligned, contents irrelevant; calls that may overlap in
  * time need workspaces of their own. As in q4k_attention_decode_f16, waits on
  * copies are bounded (2 s); if one gives up, the output is undefined. */

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <nccl.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <limits>
@@ -526,7 +527,7 @@ Q4K_API int q4k_paged_attention(const q4k_paged_kv* cache, const q4k_paged_batch
         a.ld_q = ld_q, a.ld_out = ld_output;
         a.heads = query_heads;
         a.scale = scale > 0.0f ? scale : 1.0f / std::sqrt((float)a.cache.head_dim);
-        a.window = window;
+        a.window = std::min(window, 1 << 30);  // longer than any cache
         a.workspace = workspace;
         launched(q4k::paged_attention(a, as_stream(stream)));
     });

@@ -5,7 +5,24 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace q4k {
+
+// A kernel's shared-memory limit (and, for clusters of 16, leave to use them) on
+// the current device, set at its first launch there: attributes are a device's.
+template <typename Kernel>
+cudaError_t allow_shared(Kernel kernel, int bytes, std::atomic<unsigned long long>& done, bool big_clusters = false) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (e != cudaSuccess || (done.load() & bit)) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && big_clusters)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) done.fetch_or(bit);
+    return e;
+}
 
 // Element (page, head, row, dim) of K or V is at page * page_stride + head *
 // head_stride + row * row_stride + dim, in 2-byte elements.

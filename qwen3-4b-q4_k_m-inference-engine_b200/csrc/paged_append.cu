@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(kAppendThreads)
     constexpr int kWarps = kAppendThreads / 32;
     static_assert(kTokens <= kWarps, "a warp finds a token's place");
     __shared__ float cosines[kTokens][HALF], sines[kTokens][HALF];
-    __shared__ long long places[kTokens];  // cache offset of head 0's row; -1: none; -2: a row behind the last sequence
+    __shared__ long long places[kTokens];  // cache offset of head 0's row; -1: none; -2: a row of no sequence
     __shared__ int positions[kTokens];
     const int t0 = blockIdx.x * kTokens, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int heads = a.heads, kv = a.cache.kv_heads, rows = heads + 2 * kv;
@@ -79,8 +79,9 @@ __global__ void __launch_bounds__(kAppendThreads)
         if (lane == 0) {
             long long place = -2;
             int position = 0;
-            if (s < a.batch.sequences) {
-                position = __ldg(a.batch.kv_len + s) - __ldg(a.batch.q_start + s + 1) + t;
+            // (rows before the first sequence are nobody's either)
+            if (s < a.batch.sequences && t >= __ldg(a.batch.q_start + s)) {
+                position = max(__ldg(a.batch.kv_len + s), 0) - __ldg(a.batch.q_start + s + 1) + t;
                 const int column = position >> a.cache.page_shift;
                 place = -1;  // a position that no page holds
                 if (position >= 0 && column < a.batch.table_width) {

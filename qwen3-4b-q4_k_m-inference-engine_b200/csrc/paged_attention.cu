@@ -6,9 +6,6 @@
 // with a window of w also k > p - w. A row with no key gets o = 0, lse = -inf.
 #include <math_constants.h>
 
-#include <cstring>
-#include <mutex>
-
 #include "ops.h"
 #include "paged_plan.cuh"
 #include "paged_tc.cuh"
@@ -1294,19 +1291,16 @@ template <Kind K, int D>
 cudaError_t launch_tc(const PagedAttentionArgs& a, cudaStream_t s) {
     using L = Layout<K, D>;
     auto kernel = paged_attention_tc_kernel<K, D>;
-    static std::once_flag once;
-    static cudaError_t attr = cudaSuccess;
-    std::call_once(once, [&] {
-        attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
-    });
-    if (attr != cudaSuccess) return attr;
+    static std::atomic<unsigned long long> allowed{0};
+    cudaError_t e = allow_shared(kernel, L::kBytes, allowed);
+    if (e != cudaSuccess) return e;
     CUtensorMap km, vm;
     if (!page_map(a.cache, a.cache.k, kBlockKeys, &km) || !page_map(a.cache, a.cache.v, kBlockKeys, &vm))
         return cudaErrorInvalidValue;
     const int ctas = sm_count();
     const Partials part = partials(a.workspace, ctas, kTileRows, D);
     kernel<<<ctas, kTcThreads, L::kBytes, s>>>(a, km, vm, part);
-    cudaError_t e = cudaGetLastError();
+    e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     return launch_pdl(paged_attention_join_kernel<typename Types<K>::Act, D, kTileRows>, dim3(ctas, kTileRows / kJoinRows),
                       dim3(kJoinWarps * 32), 0, s, a, part, kJoinRows);
@@ -1316,19 +1310,16 @@ template <Kind K, int D, int ROWS>
 cudaError_t launch_decode(const PagedAttentionArgs& a, cudaStream_t s) {
     using L = DecodeLayout<K, D, ROWS>;
     auto kernel = paged_attention_decode_kernel<K, D, ROWS>;
-    static std::once_flag once;
-    static cudaError_t attr = cudaSuccess;
-    std::call_once(once, [&] {
-        attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
-    });
-    if (attr != cudaSuccess) return attr;
+    static std::atomic<unsigned long long> allowed{0};
+    cudaError_t e = allow_shared(kernel, L::kBytes, allowed);
+    if (e != cudaSuccess) return e;
     CUtensorMap km, vm;
     if (!page_map(a.cache, a.cache.k, kDecodeKeys, &km) || !page_map(a.cache, a.cache.v, kDecodeKeys, &vm))
         return cudaErrorInvalidValue;
     const int ctas = sm_count();
     const Partials part = partials(a.workspace, ctas, ROWS, D);
     kernel<<<ctas, L::kThreads, L::kBytes, s>>>(a, km, vm, part);
-    cudaError_t e = cudaGetLastError();
+    e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     return launch_pdl(paged_attention_join_kernel<typename Types<K>::Act, D, ROWS>, dim3(ctas, ROWS / 2),
                       dim3(kJoinWarps * 32), 0, s, a, part, 2);

@@ -21,7 +21,7 @@ struct Sequence {
 
 __device__ __forceinline__ Sequence sequence_of(const PagedBatch& b, int s) {
     Sequence r;
-    const int q0 = __ldg(b.q_start + s), q1 = __ldg(b.q_start + s + 1), len = __ldg(b.kv_len + s);
+    const int q0 = __ldg(b.q_start + s), q1 = __ldg(b.q_start + s + 1), len = max(__ldg(b.kv_len + s), 0);
     r.first_row = min(max(q0, 0), b.tokens);
     r.rows = max(min(q1, b.tokens) - r.first_row, 0);
     r.position = len - r.rows;

@@ -26,7 +26,6 @@
 #include <math_constants.h>
 
 #include <cmath>
-#include <mutex>
 
 #include "paged_device.cuh"
 
@@ -422,7 +421,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     // language models lie within 64 of their largest, where masks need not;
     // weights end 2^-(S+1) below theirs
     const float span = fminf(fmaxf(top - extent.y, 1e-30f), 1e30f);
-    const float count_range = fminf(span, 64.0f), 
+    const float count_range = fminf(span, 64.0f),
                 weight_range = fminf(span, fmaxf(32.0f * temperature, 1e-30f));
 
     // the distance from the top in bins, and the nearest whole number of one below 2^22
@@ -683,16 +682,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
 
 template <typename T>
 cudaError_t launch(const SampleArgs& a, cudaStream_t s) {
-    static std::once_flag once;
-    static cudaError_t attr = cudaSuccess;
     auto kernel = sample_kernel<T>;
     constexpr int kMost = (int)sizeof(SampleShared) + kMaxSlice<T> * (int)sizeof(T);
     static_assert(kMost <= 227 * 1024, "shared memory of one CTA");
-    std::call_once(once, [&] {
-        attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
-        if (attr == cudaSuccess) attr = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    });
-    if (attr != cudaSuccess) return attr;
+    static std::atomic<unsigned long long> allowed{0};
+    const cudaError_t e = allow_shared(kernel, kMost, allowed, true);
+    if (e != cudaSuccess) return e;
     // CTAs per row: as few as leave two CTAs to an SM, more while the rows
     // leave SMs idle and a CTA has 2048 logits of its own
     int ranks = 1;

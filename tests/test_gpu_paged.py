@@ -137,7 +137,7 @@ def test_attention_many_sequences(sequences):
     c.check(*c.attend())
 
 
-@pytest.mark.parametrize("max_new", [0, 50, 4096])
+@pytest.mark.parametrize("max_new", [0, 1, 2, 50, 4096])
 def test_attention_host_bound_of_new_tokens(max_new):
     """The bound chooses how the work is cut, not the result."""
     c = Case([1, 50, 7], [300, 60, 7], max_new=max_new)
@@ -372,6 +372,27 @@ def test_append_in_place_and_fused_rows():
     rest = qkv[:, 8:].clone()
     got = q.paged_append(c.cache(), c.batch(), key, value, q=query, q_out=query)
     assert torch.equal(got, want) and torch.equal(qkv[:, 8:], rest)
+
+
+def test_rows_before_the_first_sequence_and_odd_lengths():
+    """q_start need not begin at 0; negative lengths are empty caches; windows may be as long as an int."""
+    c = Case([2, 3, 1], [40, 3, 5], kind="f16", max_new=1)
+    base = c.attend(window=(1 << 31) - 1)
+    assert all(torch.equal(x, y) for x, y in zip(base, c.attend()))
+    k0, v0 = c.k.clone(), c.v.clone()
+    c.q_start[0] = 1  # the first row is nobody's: a new token less
+    c.kv_len[1] = -(1 << 31)
+    out, lse = c.attend()
+    assert (out[0] == LEFT).all() and (lse[0] == LEFT).all() and torch.equal(out[1], base[0][1]) and torch.equal(out[5], base[0][5])
+    assert (out[2:5] == 0).all() and (lse[2:5] == -math.inf).all()
+    key = torch.randn(6, c.kv, c.d, device="cuda").half()
+    turned = torch.full_like(c.q, LEFT)
+    q.paged_append(c.cache(), c.batch(), key, key, q=c.q, q_out=turned)
+    assert (turned[0] == LEFT).all() and (turned[1:] != LEFT).any(-1).all()
+    p, r = int(c.table[0, 2]), int(c.table[2, 0])
+    assert torch.equal(c.v[p, :, 7], key[1]) and torch.equal(c.v[r, :, 4], key[5])
+    c.k[p, :, 7], c.v[p, :, 7], c.k[r, :, 4], c.v[r, :, 4] = k0[p, :, 7], v0[p, :, 7], k0[r, :, 4], v0[r, :, 4]
+    assert torch.equal(c.k, k0) and torch.equal(c.v, v0)
 
 
 def test_empty_calls():
