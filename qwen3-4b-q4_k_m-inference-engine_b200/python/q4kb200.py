@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -71,6 +72,8 @@ class EngineConfig(C.Structure):
         return {f: getattr(self, f) for f, _ in self._fields_}
 
 
+# The two structures as ctypes types, and as the packers that the calls use (an
+# instance of a ctypes type costs a microsecond).
 class _PagedKV(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("type", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
                 ("page_size", C.c_int), ("pages", C.c_int64), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
@@ -80,6 +83,10 @@ class _PagedKV(C.Structure):
 class _PagedBatch(C.Structure):
     _fields_ = [("sequences", C.c_int), ("max_new", C.c_int), ("q_start", C.c_void_p), ("kv_len", C.c_void_p),
                 ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("table_width", C.c_int)]
+
+
+_pack_kv = struct.Struct("@PPiiiiqqqq").pack
+_pack_batch = struct.Struct("@iiPPPqi0q").pack
 
 
 _lib = None
@@ -116,9 +123,9 @@ def lib():
             "q4k_attention_decode_f16": ([P, P, P, P, P, I, P, I, I, I, C.c_float, C.c_float, P, P, P], I),
             "q4k_attention_decode_f16_static": ([P, P, P, P, P, I, P, I, I, I, C.c_float, C.c_float, P, P], I),
             "q4k_attention_decode_scratch_bytes": ([I, I], S),
-            "q4k_paged_append": ([C.POINTER(_PagedKV), C.POINTER(_PagedBatch), S, I, P, I64, I, P, I64, P, I64, P, P,
+            "q4k_paged_append": ([P, P, S, I, P, I64, I, P, I64, P, I64, P, P,
                                   C.c_float, C.c_float, P, I64, P], I),
-            "q4k_paged_attention": ([C.POINTER(_PagedKV), C.POINTER(_PagedBatch), S, I, P, I64, I, C.c_float, I, P, I64,
+            "q4k_paged_attention": ([P, P, S, I, P, I64, I, C.c_float, I, P, I64,
                                      P, P, S, P], I),
             "q4k_paged_attention_workspace_bytes": ([I, I, I, I], S),
             "q4k_sample": ([P, I, I64, S, S, P, P, P, P, P, P, P, P], I),
@@ -526,19 +533,18 @@ class PagedKV:
 
     def __init__(self, k, v):
         _load_torch()
-        s = k.stride()
-        if k.dim() != 4 or k.shape != v.shape or s != v.stride() or k.dtype != v.dtype or s[3] != 1:
+        s, shape = k.stride(), k.shape
+        if len(s) != 4 or shape != v.shape or s != v.stride() or k.dtype is not v.dtype or s[3] != 1:
             _refuse("k and v must be alike, [pages][kv_heads][page_size][head_dim]")
         self.index = k.get_device()
         if self.index < 0 or v.get_device() != self.index:
             _refuse("k and v must be on one CUDA device")
         self.k, self.v = k, v
-        pages, self.heads, rows, d = k.shape
+        pages, self.heads, rows, d = shape
         self.head_dim = d
         # a dimension of one element has no stride of its own
-        self.c = _PagedKV(k.data_ptr(), v.data_ptr(), _type_of(k.dtype), self.heads, d, rows, pages,
-                          s[0] if pages > 1 else max(s[0], d), s[1] if self.heads > 1 else max(s[1], d), s[2])
-        self.ref = C.byref(self.c)
+        self.packed = _pack_kv(k.data_ptr(), v.data_ptr(), _type_of(k.dtype), self.heads, d, rows, pages,
+                               s[0] if pages > 1 else max(s[0], d), s[1] if self.heads > 1 else max(s[1], d), s[2])
 
 
 class PagedBatch:
@@ -561,9 +567,8 @@ class PagedBatch:
             _refuse("page_table rows must be contiguous")
         self.tensors = (q_start, kv_len, page_table)
         self.max_new = max_new
-        self.c = _PagedBatch(n, max_new, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
-                             max(s[0], width) if n > 1 else width, width)
-        self.ref = C.byref(self.c)
+        self.packed = _pack_batch(n, max_new, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
+                                  max(s[0], width) if n > 1 else width, width)
 
 
 def _token_rows(t, what: str, head_dim: int, index: int, like=None, heads: int = 0) -> int:
@@ -612,7 +617,7 @@ def paged_append(cache: PagedKV, batch: PagedBatch, k, v, q=None, q_out=None, q_
         pq, po = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         _refuse("q and q_out go together")
-    _call(index, lib().q4k_paged_append, cache.ref, batch.ref, k.shape[0], _type_of(k.dtype), pq, lq, heads,
+    _call(index, (_lib or lib()).q4k_paged_append, cache.packed, batch.packed, k.shape[0], _type_of(k.dtype), pq, lq, heads,
           k.data_ptr(), lk, v.data_ptr(), lv, _values(q_gamma, "q_gamma", d, index, f32),
           _values(k_gamma, "k_gamma", d, index, f32), epsilon, rope_base, po, lo, _stream_of(stream, index))
     return q_out
@@ -653,7 +658,7 @@ def paged_attention(cache: PagedKV, batch: PagedBatch, q, out=None, lse=None, sc
         if workspace.get_device() != index or not workspace.is_contiguous():
             _refuse("the workspace must be contiguous, on the cache's device")
         size = workspace.numel() * workspace.element_size()
-    _call(index, lib().q4k_paged_attention, cache.ref, batch.ref, tokens, _type_of(q.dtype), q.data_ptr(), lq, heads,
+    _call(index, (_lib or lib()).q4k_paged_attention, cache.packed, batch.packed, tokens, _type_of(q.dtype), q.data_ptr(), lq, heads,
           scale, window, out.data_ptr(), lo, pl, workspace.data_ptr(), size, s)
     return out
 
@@ -676,7 +681,7 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
         tokens = torch.empty(rows, dtype=i32, device=logits.device)
     if logprob is None:
         logprob = torch.empty(rows, dtype=f32, device=logits.device)
-    _call(index, lib().q4k_sample, logits.data_ptr(), _type_of(logits.dtype), s[0] if rows > 1 else vocab, rows, vocab,
+    _call(index, (_lib or lib()).q4k_sample, logits.data_ptr(), _type_of(logits.dtype), s[0] if rows > 1 else vocab, rows, vocab,
           _values(temperature, "temperature", rows, index, f32), _values(top_k, "top_k", rows, index, i32),
           _values(top_p, "top_p", rows, index, f32), _values(min_p, "min_p", rows, index, f32),
           _values(uniform, "uniform", rows, index, f32), _values(tokens, "tokens", rows, index, i32),

@@ -103,3 +103,9 @@ def test_python_refusals():
         q.sample(torch.zeros(2, 5), torch.zeros(2))
     with pytest.raises(q.InvalidArgument):
         q.PagedBatch(torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32))
+
+
+def test_packed_structures_are_the_ctypes_ones():
+    kv, b = tuple(range(1, 11)), tuple(range(1, 8))
+    assert bytes(q._PagedKV(*kv)) == q._pack_kv(*kv)
+    assert len(q._pack_batch(*b)) == C.sizeof(q._PagedBatch) and bytes(q._PagedBatch(*b))[:44] == q._pack_batch(*b)[:44]
