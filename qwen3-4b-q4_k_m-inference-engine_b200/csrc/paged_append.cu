@@ -9,9 +9,11 @@
 // leaves its thread and every access is a whole 16-byte word (8-byte stores
 // where fp32 rows become fp16); a row takes 4 to 16 neighbouring lanes, whose
 // sum of squares is a few shuffles. A CTA takes kTokens tokens: one with few
-// tokens (a decode step), so that its rows spread over several CTAs; with many
-// as many as give every thread one angle to work out, which also spreads the
-// search for the token's sequence and page over more bytes.
+// tokens (a decode step), so that its rows spread over several CTAs; eight with
+// many, a warp finding each token's sequence and page, so that this chain of
+// loads (2 us) and the angles are spread over more bytes. Measured: 8252 bf16
+// tokens of 32 + 2 x 8 heads of 128 in 40.8 us, 4.7 TB/s (1 token a CTA: 107 us,
+// 2: 43.7, 4: 41.6); 64 fp32 tokens 3.7 us, which is the launch and that chain.
 //
 // Angles: far positions need more bits than fp32 has (position 1e5 has an
 // fp32 angle error of 4e-3 rad), so the turns position * (base^(-2j/d) / 2 pi)
@@ -44,44 +46,55 @@ __global__ void __launch_bounds__(kAppendThreads)
     constexpr int D = 2 * HALF;
     constexpr int kWarps = kAppendThreads / 32;
     static_assert(kTokens <= kWarps, "a warp finds a token's place");
-    __shared__ float cosines[kTokens][HALF], sines[kTokens][HALF];
+    __shared__ __align__(16) float cosines[kTokens][HALF], sines[kTokens][HALF], gammas[2][D];
     __shared__ long long places[kTokens];  // cache offset of head 0's row; -1: none; -2: a row of no sequence
     __shared__ int positions[kTokens];
     const int t0 = blockIdx.x * kTokens, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int heads = a.heads, kv = a.cache.kv_heads, rows = heads + 2 * kv;
     const int tokens = min(kTokens, a.batch.tokens - t0);
     const int j0 = tid % kLanes * kVec;
-    // work items: rows of token 0, of token 1, ...
-    const int items = tokens * rows, step = gridDim.y * kRows;
-    int item = blockIdx.y * kRows + tid / kLanes;
-
-    // row r of a token: its queries, then keys, then values
-    auto row = [&](int t, int r) -> const T* {
-        if (r < heads) return static_cast<const T*>(a.q) + (t0 + t) * a.ld_q + (size_t)r * D;
-        if (r < heads + kv) return static_cast<const T*>(a.k) + (t0 + t) * a.ld_k + (size_t)(r - heads) * D;
-        return static_cast<const T*>(a.v) + (t0 + t) * a.ld_v + (size_t)(r - heads - kv) * D;
+    // work items: rows of token 0, of token 1, ...; this thread's next is row r of token t
+    const int step = gridDim.y * kRows;
+    int t = 0, r = blockIdx.y * kRows + tid / kLanes;
+    auto settle = [&] {
+        while (r >= rows && t < tokens) {
+            r -= rows;
+            ++t;
+        }
     };
     uint4 x[2];
-    auto fetch = [&](int i) {
-        if (i >= items) return;
-        const int t = kTokens == 1 ? 0 : i / rows;
-        const T* p = row(t, i - t * rows) + j0;
-        x[0] = __ldg(reinterpret_cast<const uint4*>(p));
-        x[1] = __ldg(reinterpret_cast<const uint4*>(p + HALF));
+    // the item's halves: a query's, key's or value's
+    auto fetch = [&] {
+        if (t >= tokens) return;
+        const T* p;
+        if (r < heads)
+            p = static_cast<const T*>(a.q) + (t0 + t) * a.ld_q + (size_t)r * D;
+        else if (r < heads + kv)
+            p = static_cast<const T*>(a.k) + (t0 + t) * a.ld_k + (size_t)(r - heads) * D;
+        else
+            p = static_cast<const T*>(a.v) + (t0 + t) * a.ld_v + (size_t)(r - heads - kv) * D;
+        x[0] = __ldg(reinterpret_cast<const uint4*>(p + j0));
+        x[1] = __ldg(reinterpret_cast<const uint4*>(p + j0 + HALF));
     };
-    fetch(item);
+    settle();
+    fetch();
+    for (int i = tid; i < 2 * D; i += kAppendThreads) {
+        const float* g = i < D ? a.q_gamma : a.k_gamma;
+        gammas[i / D][i % D] = g ? __ldg(g + i % D) : 1.0f;
+    }
     if (warp < tokens) {
         // the sequences that end at or before a token's row are those before its own
-        const int t = t0 + warp;
+        const int at = t0 + warp;
         int s = 0;
         for (int i = 0; i < a.batch.sequences; i += 32)
-            s += __popc(__ballot_sync(0xffffffffu, i + lane < a.batch.sequences && __ldg(a.batch.q_start + i + lane + 1) <= t));
+            s += __popc(
+                __ballot_sync(0xffffffffu, i + lane < a.batch.sequences && __ldg(a.batch.q_start + i + lane + 1) <= at));
         if (lane == 0) {
             long long place = -2;
             int position = 0;
             // (rows before the first sequence are nobody's either)
-            if (s < a.batch.sequences && t >= __ldg(a.batch.q_start + s)) {
-                position = max(__ldg(a.batch.kv_len + s), 0) - __ldg(a.batch.q_start + s + 1) + t;
+            if (s < a.batch.sequences && at >= __ldg(a.batch.q_start + s)) {
+                position = max(__ldg(a.batch.kv_len + s), 0) - __ldg(a.batch.q_start + s + 1) + at;
                 const int column = position >> a.cache.page_shift;
                 place = -1;  // a position that no page holds
                 if (position >= 0 && column < a.batch.table_width) {
@@ -101,20 +114,21 @@ __global__ void __launch_bounds__(kAppendThreads)
     }
     __syncthreads();
 
-    for (; item < items; item += step) {
-        const int t = kTokens == 1 ? 0 : item / rows, r = item - t * rows;
+    while (t < tokens) {
+        const int token = t, row = r;
         float y0[kVec], y1[kVec];
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
             y0[i] = to_float<T>(reinterpret_cast<const T*>(&x[0])[i]);
             y1[i] = to_float<T>(reinterpret_cast<const T*>(&x[1])[i]);
         }
-        fetch(item + step);
-        const long long place = places[t];
-        const bool is_v = r >= heads + kv;
+        r += step;
+        settle();
+        fetch();
+        const long long place = places[token];
+        const bool is_q = row < heads, is_v = row >= heads + kv;
         if (!is_v) {
-            const float* gamma = r < heads ? a.q_gamma : a.k_gamma;
-            if (gamma) {
+            if (is_q ? a.q_gamma : a.k_gamma) {
                 float ss = 0.0f;
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) ss += y0[i] * y0[i] + y1[i] * y1[i];
@@ -122,33 +136,36 @@ __global__ void __launch_bounds__(kAppendThreads)
                 const unsigned mask = kLanes == 32 ? 0xffffffffu : ((1u << kLanes) - 1u) << (lane / kLanes * kLanes);
 #pragma unroll
                 for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-                const float inv = rsqrtf(ss / (float)D + a.eps);
-                float g0[kVec], g1[kVec];
+                const float inv = rsqrtf(ss * (1.0f / (float)D) + a.eps);
+                const float* g = gammas[is_q ? 0 : 1] + j0;
 #pragma unroll
                 for (int i = 0; i < kVec; i += 4) {
-                    *reinterpret_cast<float4*>(g0 + i) = __ldg(reinterpret_cast<const float4*>(gamma + j0 + i));
-                    *reinterpret_cast<float4*>(g1 + i) = __ldg(reinterpret_cast<const float4*>(gamma + j0 + HALF + i));
+                    const float4 g0 = *reinterpret_cast<const float4*>(g + i);
+                    const float4 g1 = *reinterpret_cast<const float4*>(g + HALF + i);
+                    y0[i] *= inv * g0.x, y0[i + 1] *= inv * g0.y, y0[i + 2] *= inv * g0.z, y0[i + 3] *= inv * g0.w;
+                    y1[i] *= inv * g1.x, y1[i + 1] *= inv * g1.y, y1[i + 2] *= inv * g1.z, y1[i + 3] *= inv * g1.w;
                 }
+            }
+            float c[kVec], sn[kVec];
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    y0[i] = y0[i] * inv * g0[i];
-                    y1[i] = y1[i] * inv * g1[i];
-                }
+            for (int i = 0; i < kVec; i += 4) {
+                *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(&cosines[token][j0 + i]);
+                *reinterpret_cast<float4*>(sn + i) = *reinterpret_cast<const float4*>(&sines[token][j0 + i]);
             }
 #pragma unroll
             for (int i = 0; i < kVec; ++i) {
-                const float c = cosines[t][j0 + i], sn = sines[t][j0 + i], u = y0[i], w = y1[i];
-                y0[i] = u * c - w * sn;
-                y1[i] = u * sn + w * c;
+                const float u = y0[i], w = y1[i];
+                y0[i] = u * c[i] - w * sn[i];
+                y1[i] = u * sn[i] + w * c[i];
             }
         }
         if (place == -2) continue;
-        if (r < heads) {
-            T* o = static_cast<T*>(a.q_out) + (t0 + t) * a.ld_q_out + (size_t)r * D + j0;
+        if (is_q) {
+            T* o = static_cast<T*>(a.q_out) + (t0 + token) * a.ld_q_out + (size_t)row * D + j0;
             store_values(o, y0);
             store_values(o + HALF, y1);
         } else if (place >= 0) {
-            const int h = is_v ? r - heads - kv : r - heads;
+            const int h = is_v ? row - heads - kv : row - heads;
             C* o = reinterpret_cast<C*>(is_v ? a.cache.v : a.cache.k) + place + h * a.cache.head_stride + j0;
             store_values(o, y0);
             store_values(o + HALF, y1);
@@ -159,7 +176,7 @@ __global__ void __launch_bounds__(kAppendThreads)
 template <typename T, typename C, int HALF>
 void launch(const PagedAppendArgs& a, const Frequencies& f, cudaStream_t s) {
     constexpr int kHeld = kAppendThreads / (HALF / (16 / (int)sizeof(T)));  // rows of a CTA at a time
-    constexpr int kMany = kAppendThreads / HALF;
+    constexpr int kMany = 8;
     const int rows = a.heads + 2 * a.cache.kv_heads;
     // few tokens: a token's rows over several CTAs; measured equal near 2 tokens per SM
     if (a.batch.tokens <= 2 * sm_count())
