@@ -139,13 +139,16 @@ __device__ __forceinline__ bool finite16(uint4 v) {
     return (hit(v.x) | hit(v.y) | hit(v.z) | hit(v.w)) == 0;
 }
 
-// hi, lo: fp16 parts of (a, b); hi + lo is within 2^-22 of each.
+// hi, lo: 16-bit parts of (a, b); hi + lo is within 2^-22 of each (bf16: 2^-16).
+template <Kind K>
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
+    hi = pack2<K>(a, b);
+    if constexpr (K == Kind::kBf16) {
+        lo = pack2<K>(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        lo = pack2<K>(a - f.x, b - f.y);
+    }
 }
 
 // The power of two, as two factors, that brings a row of largest magnitude
@@ -448,8 +451,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             float f1, f2, row_c;
                             row_scale(most, c, f1, f2, row_c);
                             uint2 hi, lo;
-                            split2(v[0] * f1 * f2, v[1] * f1 * f2, hi.x, lo.x);
-                            split2(v[2] * f1 * f2, v[3] * f1 * f2, hi.y, lo.y);
+                            split2<K>(v[0] * f1 * f2, v[1] * f1 * f2, hi.x, lo.x);
+                            split2<K>(v[2] * f1 * f2, v[3] * f1 * f2, hi.y, lo.y);
                             uint8_t* at = qs + (chunk >> 4) * L::kHalf + swz128(rr, chunk >> 1 & 7) + (chunk & 1) * 8;
                             *reinterpret_cast<uint2*>(at) = hi;
                             *reinterpret_cast<uint2*>(at + L::kMat) = lo;
@@ -611,7 +614,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         p1 = exp2_fast(p1);
                         sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(p0, p1));
                         if constexpr (K == Kind::kF32)
-                            split2(p0, p1, w[e], low[e]);
+                            split2<K>(p0, p1, w[e], low[e]);
                         else
                             w[e] = pack2<K>(p0, p1);
                     }
@@ -747,9 +750,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // its own running maximum, sum and output), so no barrier stands in the loop,
 // and the warps are joined once per piece. kWarps divides the ring's stages:
 // all uses of a stage are one warp's, which therefore never waits on a stage
-// whose phase before its own is still another's. fp32 activations: queries and
-// probabilities as fp16 high and low parts, in rows 0-7 and 8-15 of one MMA
-// tile when 8 rows suffice, else in two MMAs.
+// whose phase before its own is still another's. Probabilities enter the products as
+// 16-bit high and low parts, fp32 activations' queries too: in rows 0-7 and 8-15
+// of one MMA tile when those are fp32 and 8 rows suffice, else in two MMAs.
 // ---------------------------------------------------------------------------
 constexpr int kDecodeKeys = 64;
 constexpr int kDecodeMinUnits = 1;
@@ -932,7 +935,7 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             uint32_t hi, lo;
-                            split2(x[s][e].x * f1 * f2, x[s][e].y * f1 * f2, hi, lo);
+                            split2<K>(x[s][e].x * f1 * f2, x[s][e].y * f1 * f2, hi, lo);
                             if constexpr (kStacked) {
                                 qf[s][0][2 * e] = hi;
                                 qf[s][0][2 * e + 1] = lo;
@@ -1052,49 +1055,44 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
                         o[j][3] *= f[kR - 1];
                     }
                 }
-                // probabilities, straight into the A fragments of P V
-                uint32_t pf[kDecodeKeys / 16][kParts][4];
+                // O += P V, 16 keys at a time: their probabilities go straight into
+                // the A fragments, as 16-bit high and low parts (the products are
+                // cheap here: 16-bit activations then only round their outputs)
+                float shift[kR];
 #pragma unroll
-                for (int y = 0; y < kR; ++y) {
-                    const float shift = m[y] == -CUDART_INF_F ? 0.0f : m[y] - kBias<K>;
-                    float sum = 0.0f;
+                for (int y = 0; y < kR; ++y) shift[y] = m[y] == -CUDART_INF_F ? 0.0f : m[y] - kBias<K>;
 #pragma unroll
-                    for (int j = 0; j < kDecodeKeys / 8; ++j) {
-                        const float p0 = exp2_fast(fmaf(s[j][2 * y], c[y], -shift));
-                        const float p1 = exp2_fast(fmaf(s[j][2 * y + 1], c[y], -shift));
-                        sum += p0 + p1;
-                        // keys 8j .. of step j / 2: fragment words 0, 1 (low half of 16 keys) or 2, 3
-                        const int w = 2 * (j & 1);
-                        if constexpr (kSplit) {
+                for (int kk = 0; kk < kDecodeKeys / 16; ++kk) {
+                    uint32_t pf[kStacked ? 1 : 2][4];
+#pragma unroll
+                    for (int y = 0; y < kR; ++y)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {  // keys 0-7 of the 16, keys 8-15
+                            const float p0 = exp2_fast(fmaf(s[2 * kk + e][2 * y], c[y], -shift[y]));
+                            const float p1 = exp2_fast(fmaf(s[2 * kk + e][2 * y + 1], c[y], -shift[y]));
+                            l[y] += p0 + p1;  // this lane's keys; the quad's are added at the end
                             uint32_t hi, lo;
-                            split2(p0, p1, hi, lo);
+                            split2<K>(p0, p1, hi, lo);
                             if constexpr (kStacked) {
-                                pf[j / 2][0][w] = hi;
-                                pf[j / 2][0][w + 1] = lo;
+                                pf[0][2 * e] = hi;
+                                pf[0][2 * e + 1] = lo;
                             } else {
-                                pf[j / 2][0][w + y] = hi;
-                                pf[j / 2][1][w + y] = lo;
+                                pf[0][2 * e + y] = hi;
+                                pf[1][2 * e + y] = lo;
                             }
-                        } else {
-                            pf[j / 2][0][w + y] = pack2<K>(p0, p1);
                         }
-                    }
-                    l[y] += sum;  // this lane's keys; the quad's are added at the end
-                }
-                // O += P V, 16 keys at a time
-#pragma unroll
-                for (int kk = 0; kk < kDecodeKeys / 16; ++kk)
 #pragma unroll
                     for (int j = 0; j < D / 8; j += 2) {
                         uint32_t b[4];
                         const int row = 16 * kk + (lane & 15), chunk = j + (lane >> 4);
                         ldsm_x4_t(vbase + (chunk >> 3) * L::kHalf + swz128(row, chunk & 7), b);
 #pragma unroll
-                        for (int p = 0; p < kParts; ++p) {
-                            mma16816<K>(o[j], pf[kk][p], b[0], b[1]);
-                            mma16816<K>(o[j + 1], pf[kk][p], b[2], b[3]);
+                        for (int p = 0; p < (kStacked ? 1 : 2); ++p) {
+                            mma16816<K>(o[j], pf[p], b[0], b[1]);
+                            mma16816<K>(o[j + 1], pf[p], b[2], b[3]);
                         }
                     }
+                }
                 if (edge) {
                     fence_proxy_async();  // the zeros, before the next copy into this stage
 #pragma unroll
