@@ -9,8 +9,8 @@
 // leaves its thread and every access is a whole 16-byte word (8-byte stores
 // where fp32 rows become fp16); a row takes 4 to 16 neighbouring lanes, whose
 // sum of squares is a few shuffles. A CTA takes kTokens tokens: one with few
-// tokens (a decode step), so that its rows spread over several CTAs; eight with
-// many, a warp finding each token's sequence and page, so that this chain of
+// tokens (a decode step), so that its rows spread over several CTAs; up to eight
+// with many, a warp finding each token's sequence and page, so that this chain of
 // loads (2 us) and the angles are spread over more bytes. Measured: 8252 bf16
 // tokens of 32 + 2 x 8 heads of 128 in 40.8 us, 4.7 TB/s (1 token a CTA: 107 us,
 // 2: 43.7, 4: 41.6); 64 fp32 tokens 3.7 us, which is the launch and that chain.
@@ -176,15 +176,18 @@ __global__ void __launch_bounds__(kAppendThreads)
 template <typename T, typename C, int HALF>
 void launch(const PagedAppendArgs& a, const Frequencies& f, cudaStream_t s) {
     constexpr int kHeld = kAppendThreads / (HALF / (16 / (int)sizeof(T)));  // rows of a CTA at a time
-    constexpr int kMany = 8;
-    const int rows = a.heads + 2 * a.cache.kv_heads;
-    // few tokens: a token's rows over several CTAs; measured equal near 2 tokens per SM
-    if (a.batch.tokens <= 2 * sm_count())
-        paged_append_kernel<T, C, HALF, 1>
-            <<<dim3(a.batch.tokens, (rows + kHeld - 1) / kHeld), kAppendThreads, 0, s>>>(a, f);
+    const int rows = a.heads + 2 * a.cache.kv_heads, n = a.batch.tokens, per_sm = n / sm_count();
+    // Tokens a CTA, by how many there are (us with 1 / 2 / 4 / 8 of them, fp32 rows of 32 + 2 x 8 heads of 128):
+    //   300 tokens 6.9 / 7.4 / 9.7 / 15.5, 1000 20.2 / 15.5 / 18.1 / 24.9, 2000 41.3 / 29.3 / 27.3 / 33.0,
+    //   4000 90.3 / 51.2 / 54.9 / 49.8; bf16 the same way (1000: 14.3 / 10.0 / 10.6 / 13.0)
+    if (per_sm < 2)  // a token's rows over several CTAs
+        paged_append_kernel<T, C, HALF, 1><<<dim3(n, (rows + kHeld - 1) / kHeld), kAppendThreads, 0, s>>>(a, f);
+    else if (per_sm < 8)
+        paged_append_kernel<T, C, HALF, 2><<<(n + 1) / 2, kAppendThreads, 0, s>>>(a, f);
+    else if (per_sm < 16)
+        paged_append_kernel<T, C, HALF, 4><<<(n + 3) / 4, kAppendThreads, 0, s>>>(a, f);
     else
-        paged_append_kernel<T, C, HALF, kMany>
-            <<<dim3((a.batch.tokens + kMany - 1) / kMany, 1), kAppendThreads, 0, s>>>(a, f);
+        paged_append_kernel<T, C, HALF, 8><<<(n + 7) / 8, kAppendThreads, 0, s>>>(a, f);
 }
 
 template <typename T, typename C>

@@ -46,20 +46,7 @@ __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 
-// N consecutive values from or to 16-byte aligned memory (N * sizeof(T) a
-// multiple of 16).
-template <typename T, int N>
-__device__ __forceinline__ void load_values(const T* p, float (&x)[N]) {
-    constexpr int kVec = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < N / kVec; ++i) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        const T* t = reinterpret_cast<const T*>(&w);
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) x[i * kVec + j] = to_float<T>(t[j]);
-    }
-}
-
+// N consecutive values to memory aligned to their size, at most 16 bytes.
 template <typename T, int N>
 __device__ __forceinline__ void store_values(T* p, const float (&x)[N]) {
     constexpr int kBytes = N * (int)sizeof(T);
