@@ -21,6 +21,8 @@ constexpr int kTileRows = 256;  // two MMA tiles of 128 query rows
 constexpr int kBlockKeys = 128;
 constexpr int kSoftmaxWarps = 16;  // two warpgroups per MMA tile, a thread per row and half of its keys
 constexpr int kTcThreads = (kSoftmaxWarps + 3) * 32;  // and a TMA, an MMA and a piece-walking warp
+// A tile's queries and outputs take as long as 4 of its blocks (prefill of 8192:
+// 578 us if 2 are reckoned, 575 with 3, 555 with 4), and a share is at least that.
 constexpr int kTileCost = 4;
 constexpr int kMinUnits = 4;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -177,7 +179,10 @@ __device__ __forceinline__ float from_ordered(int k) { return __int_as_float(k ^
 // as 16-bit values, O += P V with P from TMEM. Two threads share a row, each
 // with half of a block's keys and half of the row's output: with one thread to
 // a row the two warps of an SM sub-partition could not hide their own latencies
-// (2300 cycles for a softmax of 1024 cycles of exponentials).
+// (2300 cycles for a softmax of 1024 cycles of exponentials). Measured: 8192
+// bf16 tokens of 32 / 8 heads of 128 in 565 us, 970 TFLOP/s; tensor and
+// exponential pipes each 49% busy, the latencies of the softmax's steps (loads
+// of S, exchange of the maximum, waits) in between.
 // ---------------------------------------------------------------------------
 template <Kind K, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -755,6 +760,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // of one MMA tile when those are fp32 and 8 rows suffice, else in two MMAs.
 // ---------------------------------------------------------------------------
 constexpr int kDecodeKeys = 64;
+// Shares of one block: 1 sequence of 500 in 10.4 us; of two 10.8, of four 13.5.
 constexpr int kDecodeMinUnits = 1;
 constexpr int kDecodeCost = 1;
 
@@ -1180,7 +1186,10 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
 // A row's pieces are spread over as many warps as the block's rows leave (a
 // decode step over a long context: a few rows of dozens of pieces).
 constexpr int kJoinWarps = 8;
-constexpr int kJoinRows = 16;  // of a tile of 256, per block
+// Rows of a block: 16 of a tile of 256 (chunk of 512 at 4096 87.6 us, with 64
+// 96.2), 2 of a decode tile (2 sequences of 131071 56.0 us, with 8 58.2).
+constexpr int kJoinRows = 16;
+constexpr int kJoinDecodeRows = 2;
 template <typename Act, int D, int kRows>
 __global__ void __launch_bounds__(kJoinWarps * 32)
     paged_attention_join_kernel(const __grid_constant__ PagedAttentionArgs a, const Partials part, int rows_per_block) {
@@ -1319,18 +1328,31 @@ cudaError_t launch_decode(const PagedAttentionArgs& a, cudaStream_t s) {
     kernel<<<ctas, L::kThreads, L::kBytes, s>>>(a, km, vm, part);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    return launch_pdl(paged_attention_join_kernel<typename Types<K>::Act, D, ROWS>, dim3(ctas, ROWS / 2),
-                      dim3(kJoinWarps * 32), 0, s, a, part, 2);
+    return launch_pdl(paged_attention_join_kernel<typename Types<K>::Act, D, ROWS>, dim3(ctas, ROWS / kJoinDecodeRows),
+                      dim3(kJoinWarps * 32), 0, s, a, part, kJoinDecodeRows);
 }
 
-// Query rows per sequence and KV head up to which the decode kernel is used:
-// its 16 MMA rows.
+// Which kernel, by the query rows per sequence and KV head. Up to the decode
+// kernel's 16 MMA rows it is ahead everywhere (us, decode / chunk kernel: 1
+// sequence of 500 with 4 rows 10.7 / 25.9, 32 of 2000 57.9 / 130, with 16 rows
+// 75.8 / 136; bf16 61.3 / 93.9 and 68.7 / 102). Up to 32 rows it reads the keys
+// twice, which it can afford with head_dim 64 (256 sequences of 1000 with 32
+// rows: 261 / 287) and where few tiles leave it latency-bound (1 sequence of
+// 500 with 32 rows 15.3 / 26.3, bf16 13.8 / 21.0; 16 of 4000, fp32, 120 / 130),
+// not with many (256 of 1000: 577 / 468; bf16 4 of 32000: 191 / 148).
 constexpr int kDecodeRows = 16;
+
+bool few_rows(const PagedAttentionArgs& a, long long rows) {
+    const long long tiles = (long long)a.batch.sequences * a.cache.kv_heads;
+    return rows <= kDecodeRows || (rows <= 2 * kDecodeRows &&
+                                   (a.cache.head_dim == 64 || tiles <= (a.f32 ? 2 * sm_count() : 16)));
+}
 
 template <Kind K, int D>
 cudaError_t launch_dim(const PagedAttentionArgs& a, cudaStream_t s) {
     const long long rows = (long long)a.batch.max_new * (a.heads / a.cache.kv_heads);
-    if (rows > kDecodeRows) return launch_tc<K, D>(a, s);
+    if (!few_rows(a, rows)) return launch_tc<K, D>(a, s);
+    // (fp32, 4 rows: 10.7 us against 12.5 with 16 rows at 1 sequence of 500, 57.9 against 68.1 at 32 of 2000)
     if constexpr (K == Kind::kF32)
         if (rows <= 8) return launch_decode<K, D, 8>(a, s);
     return launch_decode<K, D, 16>(a, s);

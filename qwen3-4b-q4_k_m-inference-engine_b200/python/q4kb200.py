@@ -525,6 +525,16 @@ def _stream_of(stream, index: int):
     return stream_ptr(stream) if stream is not None else _torch._C._cuda_getCurrentRawStream(index)
 
 
+def _new(shape, dtype, device, stream, index: int):
+    """An empty tensor of the call's stream: memory that another stream's work
+    may still use cannot come back to it, nor go from it to others too early."""
+    if stream is None:
+        return _torch.empty(shape, dtype=dtype, device=device)
+    s = stream_ptr(stream)
+    with _torch.cuda.stream(_torch.cuda.ExternalStream(s, device=index) if s else _torch.cuda.default_stream(index)):
+        return _torch.empty(shape, dtype=dtype, device=device)
+
+
 class PagedKV:
     """One layer's paged K and V (q4k_paged_kv): tensors (possibly views) of
     shape [pages][kv_heads][page_size][head_dim], fp16 or bf16, of one shape and
@@ -612,7 +622,7 @@ def paged_append(cache: PagedKV, batch: PagedBatch, k, v, q=None, q_out=None, q_
         lq = _token_rows(q, "q", d, index, k)
         heads = q.shape[1]
         if q_out is None:
-            q_out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = _new(q.shape, q.dtype, q.device, stream, index)
         lo = _token_rows(q_out, "q_out", d, index, k, heads)
         pq, po = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
@@ -631,14 +641,14 @@ def paged_attention(cache: PagedKV, batch: PagedBatch, q, out=None, lse=None, sc
     """Causal attention of q [tokens][heads][head_dim] over the batch's pages
     (q4k_paged_attention). Returns out (allocated like q if not given); lse
     ([tokens][heads] fp32) is filled if given. The workspace comes from torch's
-    allocator, on its current stream, unless given (uint8)."""
+    allocator unless given (uint8). What a call allocates is the call's stream's."""
     d, index = cache.head_dim, cache.index
     if batch.index != index:
         _refuse("the batch must be on the cache's device")
     lq = _token_rows(q, "q", d, index)
     tokens, heads = q.shape[0], q.shape[1]
     if out is None:
-        out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = _new(q.shape, q.dtype, q.device, stream, index)
     lo = _token_rows(out, "out", d, index, q, heads)
     pl = _values(lse, "lse", tokens * heads, index, _torch.float32)
     s = _stream_of(stream, index)
@@ -649,11 +659,7 @@ def paged_attention(cache: PagedKV, batch: PagedBatch, q, out=None, lse=None, sc
             with _torch.cuda.device(index):
                 size = _workspace_bytes[key] = lib().q4k_paged_attention_workspace_bytes(heads, cache.heads, d,
                                                                                          batch.max_new)
-        workspace = _torch.empty(size, dtype=_torch.uint8, device=q.device)
-        if stream is not None:
-            # memory of torch's current stream, used on the caller's
-            workspace.record_stream(_torch.cuda.ExternalStream(s, device=index) if s
-                                    else _torch.cuda.default_stream(index))
+        workspace = _new(size, _torch.uint8, q.device, stream, index)
     else:
         if workspace.get_device() != index or not workspace.is_contiguous():
             _refuse("the workspace must be contiguous, on the cache's device")
@@ -678,9 +684,9 @@ def sample(logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None
     rows, vocab = logits.shape
     f32, i32 = torch.float32, torch.int32
     if tokens is None:
-        tokens = torch.empty(rows, dtype=i32, device=logits.device)
+        tokens = _new(rows, i32, logits.device, stream, index)
     if logprob is None:
-        logprob = torch.empty(rows, dtype=f32, device=logits.device)
+        logprob = _new(rows, f32, logits.device, stream, index)
     _call(index, (_lib or lib()).q4k_sample, logits.data_ptr(), _type_of(logits.dtype), s[0] if rows > 1 else vocab, rows, vocab,
           _values(temperature, "temperature", rows, index, f32), _values(top_k, "top_k", rows, index, i32),
           _values(top_p, "top_p", rows, index, f32), _values(min_p, "min_p", rows, index, f32),

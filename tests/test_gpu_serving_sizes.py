@@ -1,0 +1,118 @@
+"""The paged operators where a rule on sizes chooses another kernel, and calls on streams of their own."""
+import random
+
+import pytest
+import torch
+
+import q4kb200 as q
+import serving_reference as ref
+from test_gpu_paged import TYPES, Case
+
+pytestmark = pytest.mark.gpu
+
+
+def sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("per_sm,more", [(2, -1), (2, 3), (8, 1), (16, -1), (16, 5)])
+def test_append_of_many_tokens(kind, d, per_sm, more):
+    """One to eight tokens a CTA: sequences that begin and end inside a CTA's tokens, empty ones, pages of nobody. The
+    tolerances are test_append's."""
+    rng = random.Random(per_sm * 10 + more)
+    left, new, ctx = per_sm * sms() + more, [], []
+    while left:
+        n = min(left, rng.choice([0, 1, 1, 2, 7, 33, 150]))
+        new.append(n)
+        ctx.append(n + rng.randint(0, 40))
+        left -= n
+    c = Case(new, ctx, kind=kind, d=d, heads=4, kv=1, pad=3)
+    key, value = (torch.randn(c.tokens, 1, d, generator=c.g, device="cuda").to(c.act) for _ in range(2))
+    gq, gk = (1 + 0.1 * torch.randn(d, generator=c.g, device="cuda") for _ in range(2))
+    # the longest sequence's last page is missing
+    worst = ctx.index(max(ctx))
+    c.table[worst, (ctx[worst] - 1) // 16] = -1
+    k0, v0 = c.k.clone(), c.v.clone()
+    out = torch.full_like(c.q, 7.0)
+    q.paged_append(c.cache(), c.batch(), key, value, q=c.q, q_out=out, q_gamma=gq, k_gamma=gk)
+    u = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+    u_act, u_kv = u[kind], 2.0 ** -8 if kind == "bf16" else 2.0 ** -11
+    start, seen = 0, torch.zeros(c.k.shape[0], 16, dtype=torch.bool, device="cuda")
+    pair = lambda x: torch.cat([x.abs()[..., :d // 2] + x.abs()[..., d // 2:]] * 2, -1)  # noqa: E731
+    for i, (n, length) in enumerate(zip(new, ctx)):
+        rows = slice(start, start + n)
+        start += n
+        if n == 0:
+            continue
+        at = torch.arange(length - n, length, device="cuda")
+        pages, slot = c.table[i, at // 16].long(), at % 16
+        held = pages >= 0
+        seen[pages[held], slot[held]] = True
+        want_q = ref.normed_rotated(c.q[rows], gq, length - n, 1e-6, 1e6)
+        assert ((out[rows].double() - want_q).abs() <= u_act * want_q.abs() + 1e-5 * pair(want_q) + 2.0 ** -25).all()
+        want_k = ref.normed_rotated(key[rows], gk, length - n, 1e-6, 1e6)[held]
+        got_k = c.k[pages[held], :, slot[held]]
+        assert ((got_k.double() - want_k).abs() <= u_kv * want_k.abs() + 1e-5 * pair(want_k) + 2.0 ** -25).all()
+        assert torch.equal(c.v[pages[held], :, slot[held]], value[rows][held].to(c.v.dtype))
+    assert (out[start:] == 7.0).all()
+    keep = ~seen
+    assert torch.equal(c.k.transpose(1, 2)[keep], k0.transpose(1, 2)[keep]) and torch.equal(c.v.transpose(1, 2)[keep], v0.transpose(1, 2)[keep])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sequences,kv", [(1, 2), (6, 3), (45, 8)])
+@pytest.mark.parametrize("window", [0, 50])
+def test_attention_of_a_few_more_rows(kind, d, sequences, kv, window):
+    """17 to 32 query rows per sequence and KV head, on either side of the rule that chooses their kernel."""
+    rng = random.Random(sequences)
+    new = [rng.randint(1, 8) for _ in range(sequences)]
+    new[0] = 8
+    c = Case(new, [n + rng.randint(0, 200) for n in new], kind=kind, heads=4 * kv, kv=kv, d=d, pad=1)
+    c.check(*c.attend(window=window), window=window)
+
+
+def busy_block(like, value, sleep):
+    """Frees memory of `like`'s size that torch's current stream writes `value` to much later."""
+    block = torch.empty_like(like)
+    torch.cuda._sleep(sleep)
+    block.fill_(value)
+    return block.data_ptr()
+
+
+def test_allocations_are_the_streams():
+    """A call on a stream of its own takes no memory that the current stream's work still writes."""
+    c = Case([1] * 64, [200] * 64, kind="f16")
+    want, turned = c.attend()[0], q.paged_append(c.cache(), c.batch(), c.q[:, :2], c.q[:, :2], q=c.q)
+    logits, u = torch.randn(64, 5000, device="cuda"), torch.rand(64, device="cuda")
+    drawn = q.sample(logits, u)
+    again = c.attend()[0]
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    size = q.lib().q4k_paged_attention_workspace_bytes(8, 2, 128, 1)
+    busy_block(c.q, 3.0, 50_000_000)
+    busy_block(drawn[0], 3, 1)
+    busy_block(torch.empty(size, dtype=torch.uint8, device="cuda"), 255, 1)
+    # (the append's rows are written again to the same values)
+    got_turned = q.paged_append(c.cache(), c.batch(), c.q[:, :2], c.q[:, :2], q=c.q, stream=s)
+    got = q.paged_attention(c.cache(), c.batch(), c.q, stream=s)
+    got_drawn = q.sample(logits, u, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(got_turned, turned) and torch.equal(got, again)
+    assert all(torch.equal(x, y) for x, y in zip(got_drawn, drawn))
+    assert want.shape == got.shape
+
+
+def test_calls_on_two_streams_at_once():
+    """Calls that may overlap, each with memory of its own, give what they give alone."""
+    cases = [Case([1] * 40, [1500] * 40, kind="bf16", seed=2), Case([130, 5], [900, 700], kind="f32", seed=3)]
+    alone = [c.attend()[0] for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = [q.paged_attention(c.cache(), c.batch(), c.q, stream=s) for c, s in zip(cases, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, alone))
