@@ -74,36 +74,30 @@ def test_attention_of_a_few_more_rows(kind, d, sequences, kv, window):
     c.check(*c.attend(window=window), window=window)
 
 
-def busy_block(like, value, sleep):
-    """Frees memory of `like`'s size that torch's current stream writes `value` to much later."""
-    block = torch.empty_like(like)
-    torch.cuda._sleep(sleep)
-    block.fill_(value)
-    return block.data_ptr()
+def stream_of(x):
+    """The stream that torch's allocator holds a tensor's memory for."""
+    for segment in torch.cuda.memory_snapshot():
+        if segment["address"] <= x.data_ptr() < segment["address"] + segment["total_size"]:
+            return segment["stream"]
+    raise AssertionError("no segment holds the tensor")
 
 
 def test_allocations_are_the_streams():
-    """A call on a stream of its own takes no memory that the current stream's work still writes."""
+    """A call on a stream of its own takes no memory that the current stream's work may still write."""
     c = Case([1] * 64, [200] * 64, kind="f16")
-    want, turned = c.attend()[0], q.paged_append(c.cache(), c.batch(), c.q[:, :2], c.q[:, :2], q=c.q)
     logits, u = torch.randn(64, 5000, device="cuda"), torch.rand(64, device="cuda")
-    drawn = q.sample(logits, u)
-    again = c.attend()[0]
+    turned, drawn = q.paged_append(c.cache(), c.batch(), c.q[:, :2], c.q[:, :2], q=c.q), q.sample(logits, u)
+    want = c.attend()[0]
     s = torch.cuda.Stream()
     torch.cuda.synchronize()
-    torch.cuda.empty_cache()
-    size = q.lib().q4k_paged_attention_workspace_bytes(8, 2, 128, 1)
-    busy_block(c.q, 3.0, 50_000_000)
-    busy_block(drawn[0], 3, 1)
-    busy_block(torch.empty(size, dtype=torch.uint8, device="cuda"), 255, 1)
-    # (the append's rows are written again to the same values)
     got_turned = q.paged_append(c.cache(), c.batch(), c.q[:, :2], c.q[:, :2], q=c.q, stream=s)
     got = q.paged_attention(c.cache(), c.batch(), c.q, stream=s)
-    got_drawn = q.sample(logits, u, stream=s)
+    got_drawn = q.sample(logits, u, stream=s.cuda_stream)
     torch.cuda.synchronize()
-    assert torch.equal(got_turned, turned) and torch.equal(got, again)
+    assert torch.equal(got_turned, turned) and torch.equal(got, want)
     assert all(torch.equal(x, y) for x, y in zip(got_drawn, drawn))
-    assert want.shape == got.shape
+    assert {stream_of(x) for x in (got_turned, got, *got_drawn)} == {s.cuda_stream}
+    assert stream_of(q.paged_attention(c.cache(), c.batch(), c.q)) != s.cuda_stream
 
 
 def test_calls_on_two_streams_at_once():
