@@ -220,7 +220,8 @@ typedef struct {
  * their outputs are left as they were. max_new is a bound on the new tokens
  * of any one sequence, known to the host: 1 for a decode step; 0 if unknown.
  * It only chooses how the work is cut; results do not depend on it beyond
- * rounding. */
+ * rounding. Up to 2^24 tokens and 2^20 sequences (attention: 8192, and 2^31 - 1
+ * tokens x query heads). */
 typedef struct {
     int sequences;
     int max_new;
@@ -260,10 +261,11 @@ int q4k_paged_append(const q4k_paged_kv* cache, const q4k_paged_batch* batch, si
  * low parts); 16-bit ones may round their probabilities to 16 bits, sums are
  * fp32. Keys and values that are not finite only reach the tokens that attend
  * to them (all of whose outputs may then be NaN); what stands in pages behind
- * a sequence's end reaches none. workspace: q4k_paged_attention_workspace_bytes of the same call's
- * numbers, 16-byte aligned, contents irrelevant; calls that may overlap in
- * time need workspaces of their own. As in q4k_attention_decode_f16, waits on
- * copies are bounded (2 s); if one gives up, the output is undefined. */
+ * a sequence's end reaches none. workspace: q4k_paged_attention_workspace_bytes
+ * of the same call's numbers, 16-byte aligned, contents irrelevant; calls that
+ * may overlap in time need workspaces of their own. As in
+ * q4k_attention_decode_f16, waits on copies are bounded (2 s); if one gives up,
+ * the output is undefined. */
 int q4k_paged_attention(const q4k_paged_kv* cache, const q4k_paged_batch* batch, size_t tokens, int type,
                         const void* q, int64_t ld_q, int query_heads, float scale, int window, void* output,
                         int64_t ld_output, float* lse, void* workspace, size_t workspace_bytes, void* stream);

@@ -74,6 +74,21 @@ def test_attention_of_a_few_more_rows(kind, d, sequences, kv, window):
     c.check(*c.attend(window=window), window=window)
 
 
+@pytest.mark.parametrize("kind,longest", [("f32", 1), ("f32", 70), ("bf16", 12)])
+def test_attention_of_the_most_sequences(kind, longest):
+    """8192 sequences, most of them without a new token."""
+    rng = random.Random(longest)
+    new = [0] * 8192
+    for i in rng.sample(range(8192), 150) + [0, 8191]:
+        new[i] = rng.randint(1, longest)
+    new[8191] = longest
+    c = Case(new, [n + rng.randint(0, 70) for n in new], kind=kind, heads=4, kv=2, d=64)
+    out, lse = c.attend()
+    keep = [i for i in range(8192) if new[i]]
+    c.new, c.ctx, c.table = [new[i] for i in keep], [c.ctx[i] for i in keep], c.table[keep]
+    c.check(out, lse)
+
+
 def stream_of(x):
     """The stream that torch's allocator holds a tensor's memory for."""
     for segment in torch.cuda.memory_snapshot():
