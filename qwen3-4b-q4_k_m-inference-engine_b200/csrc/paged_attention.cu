@@ -73,7 +73,7 @@ struct PieceInfo {
 
 struct TcBars {
     uint64_t full[6], empty[6];
-    uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], done;
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
     uint64_t piece_full[2][2], piece_empty[2][2];
     uint32_t tmem;
     int dead;
@@ -214,8 +214,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.q_full[i], kSoftmaxWarps / 2);
             mbar_init(&bar.s_full[i], 1);
-            mbar_init(&bar.p_full[i][0], kSoftmaxWarps / 4);
-            mbar_init(&bar.p_full[i][1], kSoftmaxWarps / 4);
+            mbar_init(&bar.p_full[i], kSoftmaxWarps / 2);
             mbar_init(&bar.o_full[i], 1);
             for (int j = 0; j < 2; ++j) {
                 mbar_init(&bar.piece_full[i][j], 1);
@@ -302,12 +301,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 tc_commit(&bar.s_full[t]);
             };
-            // O += P V over one half of the block's keys
-            auto value = [&](int t, int stage, int half, bool accumulate) {
-                const uint64_t v = v_desc + (stage % kStages) * (L::kMat >> 4) + half * 4 * (2048 >> 4);
-                const uint32_t p = tmem + kS + 128 * t + L::kPStep * 2 * half;
+            // O += P V
+            auto value = [&](int t, int stage, bool accumulate) {
+                const uint64_t v = v_desc + (stage % kStages) * (L::kMat >> 4);
+                const uint32_t p = tmem + kS + 128 * t;
 #pragma unroll
-                for (int kk = 0; kk < kBlockKeys / 32; ++kk)
+                for (int kk = 0; kk < kBlockKeys / 16; ++kk)
 #pragma unroll
                     for (int pt = 0; pt < L::kParts; ++pt)
                         mma_ts(tmem + kO + 128 * t, p + L::kPStep * (kk / 2) + 16 * pt + 8 * (kk & 1),
@@ -330,14 +329,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (more) k_stage = n++;
                     for (int t = 0; t < tiles && ok; ++t) {
                         const uint32_t phase = p_phase[t]++ & 1;
-                        ok = wait_stage(v_stage);
-                        for (int half = 0; half < 2 && ok; ++half) {
-                            ok = wait_or_dead(&bar.p_full[t][half], phase, dead);
-                            if (!ok) break;
-                            tc_fence_after();
-                            value(t, v_stage, half, (K == Kind::kF32 ? i % kFlush : i) > 0 || half > 0);
-                        }
+                        // Both threads of every row: each MMA reads and writes all of
+                        // O's columns, and either thread may have rescaled its half of
+                        // them with this block (with a wait for one half of the keys at
+                        // a time, the first products could meet the other's rescaling)
+                        ok = wait_stage(v_stage) && wait_or_dead(&bar.p_full[t], phase, dead);
                         if (!ok) break;
+                        tc_fence_after();
+                        value(t, v_stage, (K == Kind::kF32 ? i % kFlush : i) > 0);
                         if (more) {
                             ok = wait_stage(k_stage);
                             if (!ok) break;
@@ -635,7 +634,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bar.p_full[t][h]);
+                if (lane == 0) mbar_arrive(&bar.p_full[t]);
             }
             wait_or_dead(&bar.o_full[t], items & 1, dead);
             __syncwarp();

@@ -1,0 +1,39 @@
+"""Calls of the paged operators and the sampler that were answered wrongly, or only by luck rightly."""
+import math
+
+import pytest
+import torch
+
+import q4kb200 as q
+import serving_reference as ref
+from test_gpu_paged import TYPES, Case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_scores_that_rise_with_every_block(kind, d):
+    """Scores 6 higher in every block of 128 keys (8.7 in powers of two, so that the sums so far are scaled down at
+    nearly every block): each half of a row's outputs is scaled before any product adds to it, in every repetition.
+
+    A score is a sum of 8 x 96 and the rest of d products, at most 2 d / 16 steps that each lose up to 2^-23 of 112, with
+    4 more roundings: 20 x 2^-23 x 112 = 2.7e-4, twice that in a probability (its own and the sum's)."""
+    c = Case([300, 41], [2048, 1500], kind=kind, heads=32, kv=8, d=d, page=64, seed=11)
+    c.q[..., 0] = 8.0
+    for i, length in enumerate(c.ctx):
+        at = torch.arange(length, device="cuda")
+        c.k[c.table[i, at // 64].long(), :, at % 64, 0] = (6.0 * (at // 128)).to(c.k.dtype)[:, None]
+    first = c.attend(scale=0.125)
+    u, tiny = {"f32": (0.0, 0.0), "f16": (2.0 ** -11, 2.0 ** -25), "bf16": (2.0 ** -8, 0.0)}[kind]
+    start = 0
+    for i, (n, length) in enumerate(zip(c.new, c.ctx)):
+        rows = slice(start, start + n)
+        start += n
+        k, v = (ref.paged_rows(t, c.table[i], length) for t in (c.k, c.v))
+        want, want_lse, size, flat = ref.attention(c.q[rows], k, v, length - n, 0.125)
+        err = (first[0][rows].double() - want).abs()
+        assert (err <= u * (size + want.abs()) + tiny * (flat + 1) + 6e-4 * size).all(), (i, float((err / size).max()))
+        assert ((first[1][rows].double() - want_lse).abs() <= 3e-4).all()
+    for _ in range(40):
+        assert all(torch.equal(x, y) for x, y in zip(first, c.attend(scale=0.125)))
