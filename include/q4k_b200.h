@@ -256,10 +256,10 @@ int q4k_paged_append(const q4k_paged_kv* cache, const q4k_paged_batch* batch, si
  * in q4k_paged_append. lse (optional, [tokens][query_heads] floats) receives
  * the natural logarithm of each row's sum of exponentials. A token that
  * attends to nothing (position < 0) gets zeros and lse -inf. Table entries
- * outside the cache read as zero keys and values. fp32 activations keep fp32
- * accuracy (queries and probabilities enter the tensor cores as fp16 high and
- * low parts); 16-bit ones may round their probabilities to 16 bits, sums are
- * fp32. Keys and values that are not finite only reach the tokens that attend
+ * outside the cache read as zero keys and values. Probabilities enter the tensor
+ * cores as 16-bit high and low parts, fp32 activations' queries too, sums are
+ * fp32: fp32 activations keep fp32 accuracy, 16-bit ones only round their
+ * outputs. Keys and values that are not finite only reach the tokens that attend
  * to them (all of whose outputs may then be NaN); what stands in pages behind
  * a sequence's end reaches none. workspace: q4k_paged_attention_workspace_bytes
  * of the same call's numbers, 16-byte aligned, contents irrelevant; calls that

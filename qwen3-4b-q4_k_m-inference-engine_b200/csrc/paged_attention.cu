@@ -38,9 +38,9 @@ template <Kind K>
 constexpr float kBias = K == Kind::kBf16 ? 0.0f : 7.0f;
 // The tensor cores truncate their fp32 sums: each MMA takes on average half a
 // last place, kTruncation of the sum so far (2^-24 of the mean of 1 / mantissa),
-// off O. fp32 activations cannot leave it at that (1.5e-6 after 512 keys, 7e-6
-// after 4500, measured): O leaves TMEM every kFlush blocks for a sum in the
-// workspace, and what its 16 MMAs a block have taken is given back.
+// off O, which is given back. fp32 activations cannot leave it at that (1.5e-6
+// after 512 keys, 7e-6 after 4500, measured without either): their O also leaves
+// TMEM every kFlush blocks for a sum in the workspace.
 constexpr float kTruncation = 0.7213f / 16777216.0f;
 constexpr int kFlush = 8;
 
@@ -73,7 +73,7 @@ struct PieceInfo {
 
 struct TcBars {
     uint64_t full[6], empty[6];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
+    uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2], done;
     uint64_t piece_full[2][2], piece_empty[2][2];
     uint32_t tmem;
     int dead;
@@ -90,10 +90,7 @@ static_assert(sizeof(TcBars) <= kBarBytes, "barrier area");
 // their way out (4 KB a softmax warp).
 template <Kind K, int D>
 struct Layout {
-    static constexpr int kParts = K == Kind::kF32 ? 2 : 1;
-    // TMEM columns of 32 probabilities, written over their scores: 16 (two to a
-    // column), for fp32 the low parts 16 on
-    static constexpr int kPStep = 16 * kParts;
+    static constexpr int kParts = K == Kind::kF32 ? 2 : 1;  // of Q
     static constexpr int kHalf = 128 * 128;
     static constexpr int kMat = D / 64 * kHalf;  // 128 rows of D 16-bit values
     static constexpr int kStages = D == 64 ? 6 : K == Kind::kF32 ? 3 : 5;
@@ -171,18 +168,20 @@ __device__ __forceinline__ int ordered(float v) {
 __device__ __forceinline__ float from_ordered(int k) { return __int_as_float(k ^ ((k >> 31) & 0x7fffffff)); }
 
 // ---------------------------------------------------------------------------
-// Many query rows (prompt chunks): bound by the tensor cores (4 x 512 cycles per
-// block of 256 rows x 128 keys x 128 dims) and as much by the exponentials (2048
-// cycles at 16 per cycle and SM). One MMA-issuing thread alternates between two
-// tiles of 128 rows, so that one tile's products run under the other's
-// softmax: S = Q K^T from shared memory into TMEM, probabilities back over S
-// as 16-bit values, O += P V with P from TMEM. Two threads share a row, each
+// Many query rows (prompt chunks): bound by the tensor cores (6 x 512 cycles per
+// block of 256 rows x 128 keys x 128 dims; fp32 activations 8 x 512) and the
+// exponentials (2048 cycles at 16 per cycle and SM). One MMA-issuing thread
+// alternates between two tiles of 128 rows, so that one tile's products run under
+// the other's softmax: S = Q K^T from shared memory into TMEM, probabilities back
+// over S as 16-bit high and low parts, O += P V with P from TMEM, the first half
+// of the products under the second half of their own exponentials (prefill 739 us,
+// 766 with all after them). High parts alone would take 524 us, but leave 16-bit
+// outputs 1.4 times the error that their own rounding has. Two threads share a row, each
 // with half of a block's keys and half of the row's output: with one thread to
 // a row the two warps of an SM sub-partition could not hide their own latencies
 // (2300 cycles for a softmax of 1024 cycles of exponentials). Measured: 8192
-// bf16 tokens of 32 / 8 heads of 128 in 565 us, 970 TFLOP/s; tensor and
-// exponential pipes each 49% busy, the latencies of the softmax's steps (loads
-// of S, exchange of the maximum, waits) in between.
+// bf16 tokens of 32 / 8 heads of 128 in 739 us, 744 TFLOP/s (of 1.5 times as many
+// in the products).
 // ---------------------------------------------------------------------------
 template <Kind K, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -194,8 +193,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     constexpr int kStages = L::kStages;
     constexpr uint32_t kIdescS = idesc_f16(K == Kind::kBf16, 128, kBlockKeys, false);
     constexpr uint32_t kIdescO = idesc_f16(K == Kind::kBf16, 128, D, true);
-    // TMEM columns: S (its probabilities written over it) and O of each MMA tile
-    constexpr uint32_t kS = 0, kO = 256;
+    // TMEM columns: S (its probabilities written over it: of 32 of them 16 columns
+    // of high parts, two to a column, then 16 of low parts) and O of each MMA tile
+    constexpr uint32_t kS = 0, kO = 256, kPStep = 32;
     constexpr int kTmaWarp = kSoftmaxWarps, kMmaWarp = kSoftmaxWarps + 1, kWalkWarp = kSoftmaxWarps + 2;
 
     extern __shared__ __align__(1024) uint8_t smem_dyn[];
@@ -214,7 +214,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.q_full[i], kSoftmaxWarps / 2);
             mbar_init(&bar.s_full[i], 1);
-            mbar_init(&bar.p_full[i], kSoftmaxWarps / 2);
+            mbar_init(&bar.p_full[i][0], kSoftmaxWarps / 2);
+            mbar_init(&bar.p_full[i][1], kSoftmaxWarps / 2);
             mbar_init(&bar.o_full[i], 1);
             for (int j = 0; j < 2; ++j) {
                 mbar_init(&bar.piece_full[i][j], 1);
@@ -301,16 +302,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 tc_commit(&bar.s_full[t]);
             };
-            // O += P V
-            auto value = [&](int t, int stage, bool accumulate) {
-                const uint64_t v = v_desc + (stage % kStages) * (L::kMat >> 4);
-                const uint32_t p = tmem + kS + 128 * t;
+            // O += P V over the first or second 32 of each thread's 64 keys
+            auto value = [&](int t, int stage, int part, bool accumulate) {
+                const uint64_t v = v_desc + (stage % kStages) * (L::kMat >> 4) + 2 * part * (2048 >> 4);
+                const uint32_t p = tmem + kS + 128 * t + kPStep * part;
 #pragma unroll
-                for (int kk = 0; kk < kBlockKeys / 16; ++kk)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int pt = 0; pt < L::kParts; ++pt)
-                        mma_ts(tmem + kO + 128 * t, p + L::kPStep * (kk / 2) + 16 * pt + 8 * (kk & 1),
-                               v + kk * (2048 >> 4), kIdescO, accumulate || (pt | kk) != 0);
+                    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                        for (int pt = 0; pt < 2; ++pt)
+                            mma_ts(tmem + kO + 128 * t, p + 2 * kPStep * h + 16 * pt + 8 * kk,
+                                   v + (4 * h + kk) * (2048 >> 4), kIdescO, accumulate || (pt | kk | h) != 0);
             };
             for (; pc.valid() && ok; pc.next()) {
                 const int tiles = pc.tile.rows > 128 ? 2 : 1;
@@ -329,14 +332,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (more) k_stage = n++;
                     for (int t = 0; t < tiles && ok; ++t) {
                         const uint32_t phase = p_phase[t]++ & 1;
-                        // Both threads of every row: each MMA reads and writes all of
-                        // O's columns, and either thread may have rescaled its half of
-                        // them with this block (with a wait for one half of the keys at
-                        // a time, the first products could meet the other's rescaling)
-                        ok = wait_stage(v_stage) && wait_or_dead(&bar.p_full[t], phase, dead);
+                        // Either part waits for both threads of every row: each MMA
+                        // reads and writes all of O's columns, and either thread may
+                        // have rescaled its half of them before its first part
+                        ok = wait_stage(v_stage);
+                        for (int part = 0; part < 2 && ok; ++part) {
+                            ok = wait_or_dead(&bar.p_full[t][part], phase, dead);
+                            if (!ok) break;
+                            tc_fence_after();
+                            value(t, v_stage, part, (K == Kind::kF32 ? i % kFlush : i) > 0 || part > 0);
+                        }
                         if (!ok) break;
-                        tc_fence_after();
-                        value(t, v_stage, (K == Kind::kF32 ? i % kFlush : i) > 0);
                         if (more) {
                             ok = wait_stage(k_stage);
                             if (!ok) break;
@@ -587,7 +593,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (K == Kind::kF32) l_flushed *= f;
                     if (!fresh) {
                         l *= f;
-                        if (K == Kind::kF32) steps *= f;
+                        steps *= f;
                         // (at rest, as above)
 #pragma unroll 1
                         for (int j = 0; j < D / 16; j += 2) {
@@ -606,7 +612,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 uint64_t sum[2] = {0, 0};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    // 16 probabilities: 8 words (and 8 of low parts)
+                    // 16 probabilities: 8 words of high and 8 of low parts
                     uint32_t w[8], low[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -618,29 +624,32 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         p0 = exp2_fast(p0);
                         p1 = exp2_fast(p1);
                         sum[e & 1] = add_f32x2(sum[e & 1], pack_f32x2(p0, p1));
-                        if constexpr (K == Kind::kF32)
-                            split2<K>(p0, p1, w[e], low[e]);
-                        else
-                            w[e] = pack2<K>(p0, p1);
+                        split2<K>(p0, p1, w[e], low[e]);
                     }
-                    const uint32_t col = s_addr + L::kPStep * (2 * h + (j >> 1)) + 8 * (j & 1);
+                    const uint32_t col = s_addr + kPStep * (2 * h + (j >> 1)) + 8 * (j & 1);
                     tmem_st8(col, w);
-                    if constexpr (K == Kind::kF32) tmem_st8(col + 16, low);
+                    tmem_st8(col + 16, low);
+                    if (j == 1) {  // half of them: their products run under the other half's exponentials
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bar.p_full[t][0]);
+                    }
                 }
                 float sum0, sum1;
                 unpack_f32x2(add_f32x2(sum[0], sum[1]), sum0, sum1);
-                if (K == Kind::kF32) steps += fmaf(0.5f, sum0 + sum1, l);
+                steps += fmaf(0.5f, sum0 + sum1, l);
                 l += sum0 + sum1;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bar.p_full[t]);
+                if (lane == 0) mbar_arrive(&bar.p_full[t][1]);
             }
             wait_or_dead(&bar.o_full[t], items & 1, dead);
             __syncwarp();
             tc_fence_after();
             n += 2 * count;
-            const float back = K == Kind::kF32 ? give_back() : 1.0f;
+            const float back = give_back();
             const bool was_flushed = K == Kind::kF32 && count > kFlush;
             const float before = was_flushed ? flushed_factor() : 0.0f;
             if (K == Kind::kF32) l += l_flushed;
@@ -655,7 +664,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             l = __int_as_float(*run);
             const bool whole = pi.whole;
             const size_t slot = ((size_t)blockIdx.x * 2 + pi.slot) * kTileRows + 128 * t;
-            const float inv = whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f;
+            const float inv = (whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f) * (K == Kind::kF32 ? 1.0f : back);
             const bool none = whole && !(l != 0.0f);
             const bool poisoned = position >= pi.poison_first && (a.window == 0 || position - a.window < pi.poison_last);
             const int rows = pi.rows;

@@ -37,3 +37,24 @@ def test_attention_scores_that_rise_with_every_block(kind, d):
         assert ((first[1][rows].double() - want_lse).abs() <= 3e-4).all()
     for _ in range(40):
         assert all(torch.equal(x, y) for x, y in zip(first, c.attend(scale=0.125)))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,ctx", [([200, 33], [200, 1700]), ([700], [3000])])
+def test_attention_of_16_bit_chunks_only_rounds_its_outputs(kind, d, new, ctx):
+    """Probabilities reach the products as high and low parts, 2^-16 of each together in bf16 (a half step of a half step)
+    and 2^-22 in fp16 (or 2^-32 of the row's largest, where a low part would be smaller than fp16's last place): what is
+    left is the outputs' own rounding (2^-25 where those are small for fp16), and fp32's as in Case.check."""
+    c = Case(new, ctx, kind=kind, heads=8, kv=2, d=d, page=32, seed=21)
+    out, _ = c.attend()
+    unit, parts = {"f16": (2.0 ** -11, 2.0 ** -22), "bf16": (2.0 ** -8, 2.0 ** -16)}[kind]
+    start = 0
+    for i, (n, length) in enumerate(zip(new, ctx)):
+        rows = slice(start, start + n)
+        start += n
+        k, v = (ref.paged_rows(t, c.table[i], length) for t in (c.k, c.v))
+        want, _, size, flat = ref.attention(c.q[rows], k, v, length - n, d ** -0.5)
+        err = (out[rows].double() - want).abs()
+        bound = unit * want.abs() + (parts + 2e-5) * size + (2.0 ** -25 + 2.0 ** -32 * flat if kind == "f16" else 0.0)
+        assert (err <= bound).all(), (i, float((err / bound).max()))
