@@ -228,7 +228,7 @@ typedef struct {
     const int* q_start;    /* [sequences + 1], ascending */
     const int* kv_len;     /* [sequences] */
     const int* page_table; /* [sequences][table_stride] */
-    int64_t table_stride;
+    int64_t table_stride;  /* entries between rows: table_width or more, or 0: one row for all */
     int table_width; /* entries of a table row that exist (positions below table_width * page_size) */
 } q4k_paged_batch;
 
@@ -241,7 +241,9 @@ typedef struct {
  * may both be NULL (query_heads is then ignored), and may be the same buffer.
  * A token whose position is negative or past the page table, or whose page is
  * not one of the cache's (a negative entry marks a page to skip), is not
- * written to the cache; its query is still rotated. The paged form of
+ * written to the cache; its query is still rotated. Of tokens that have the same
+ * row of a page (sequences may share pages) any one's key and any one's value
+ * stays there. The paged form of
  * Engine.cpp:87-91. Buffers and gammas 16-byte aligned, ld_* whole 16-byte
  * words. */
 int q4k_paged_append(const q4k_paged_kv* cache, const q4k_paged_batch* batch, size_t tokens, int type, const void* q,

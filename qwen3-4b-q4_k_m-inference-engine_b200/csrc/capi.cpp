@@ -450,7 +450,8 @@ q4k::PagedBatch paged_batch(const q4k_paged_batch* b, size_t tokens, int page_si
     r.tokens = (int)tokens;
     if (r.sequences == 0 || r.tokens == 0) return r;
     if (!b->q_start || !b->kv_len || !b->page_table) invalid("a batch needs q_start, kv_len and a page table");
-    if (b->table_width < 1 || b->table_stride < b->table_width) invalid("page table rows must hold table_width entries");
+    if (b->table_width < 1 || (b->table_stride < b->table_width && b->table_stride != 0))
+        invalid("page table rows must hold table_width entries, or be one row (stride 0)");
     if (b->table_width > std::numeric_limits<int>::max() / page_size - 1) out_of_range("the page table is too wide");
     r.q_start = b->q_start;
     r.kv_len = b->kv_len;

@@ -559,8 +559,9 @@ class PagedKV:
 
 class PagedBatch:
     """The sequences of a call (q4k_paged_batch): q_start [n + 1], kv_len [n] and
-    page_table [n][width], int32 on the device. max_new: a bound on the new
-    tokens of any one sequence (1 for a decode step; 0: unknown)."""
+    page_table [n][width], int32 on the device (one row expanded to n: sequences
+    of the same pages). max_new: a bound on the new tokens of any one sequence (1
+    for a decode step; 0: unknown)."""
 
     def __init__(self, q_start, kv_len, page_table, max_new: int = 0):
         int32 = _load_torch().int32
@@ -578,7 +579,7 @@ class PagedBatch:
         self.tensors = (q_start, kv_len, page_table)
         self.max_new = max_new
         self.packed = _pack_batch(n, max_new, q_start.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(),
-                                  max(s[0], width) if n > 1 else width, width)
+                                  s[0] if n > 1 else width, width)
 
 
 def _token_rows(t, what: str, head_dim: int, index: int, like=None, heads: int = 0) -> int:

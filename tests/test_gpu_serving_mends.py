@@ -58,3 +58,35 @@ def test_attention_of_16_bit_chunks_only_rounds_its_outputs(kind, d, new, ctx):
         err = (out[rows].double() - want).abs()
         bound = unit * want.abs() + (parts + 2e-5) * size + (2.0 ** -25 + 2.0 ** -32 * flat if kind == "f16" else 0.0)
         assert (err <= bound).all(), (i, float((err / bound).max()))
+
+
+@pytest.mark.parametrize("new", [[1] * 5, [3, 40, 1, 0, 150]])
+def test_sequences_that_share_one_row_of_a_page_table(new):
+    """Samples of one prompt: a page table expanded from one row, as if that row were repeated."""
+    c = Case([200], [200], kind="f16", seed=4)
+    n = len(new)
+    c.new, c.ctx = new, [170 + i for i in range(n)]
+    c.q_start = torch.tensor([0] + new).cumsum(0).int().cuda()
+    c.kv_len = torch.tensor(c.ctx).int().cuda()
+    c.tokens, c.max_new = sum(new), max(new)
+    c.q = torch.randn(c.tokens, c.heads, c.d, device="cuda").half()
+    row = c.table
+    # what would be taken for the other rows
+    store = torch.full((n, row.shape[1]), c.spare[0], dtype=torch.int32, device="cuda")
+    store[:1] = row
+    c.table = store[:1].expand(n, -1)
+    out, lse = c.attend()
+    c.check(out, lse)
+    key = torch.randn(n, c.kv, c.d, device="cuda").half()
+    one_each = q.PagedBatch(torch.arange(n + 1).int().cuda(), c.kv_len, c.table, max_new=1)
+    k0, v0 = c.k.clone(), c.v.clone()
+    q.paged_append(c.cache(), one_each, key, key)
+    for i, length in enumerate(c.ctx):
+        page, slot = int(row[0, (length - 1) // 16]), (length - 1) % 16
+        assert torch.equal(c.v[page, :, slot], key[i])
+        c.k[page, :, slot], c.v[page, :, slot] = k0[page, :, slot], v0[page, :, slot]
+    assert torch.equal(c.k, k0) and torch.equal(c.v, v0)
+    # rows that overlap in any other way are refused
+    c.table = store.flatten()[: n + row.shape[1]].as_strided((n, row.shape[1]), (1, 1))
+    with pytest.raises(q.InvalidArgument):
+        c.attend()
