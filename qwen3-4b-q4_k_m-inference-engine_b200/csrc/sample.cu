@@ -122,6 +122,15 @@ struct Weights {
     }
 };
 
+// All CTAs of the cluster have started once each has arrived: only then may one
+// touch another's shared memory.
+__device__ __forceinline__ void cluster_started_arrive() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_started_wait() {
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kSampleThreads, 2)
     sample_kernel(const __grid_constant__ SampleArgs a, const __grid_constant__ ExpTable table, int S, int slice) {
@@ -136,6 +145,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
     const int count = min(slice, a.vocab - base);
     const T* src = static_cast<const T*>(a.logits) + row * a.ld + base;
 
+    cluster_started_arrive();
     // The slice into shared memory: bulk copies where rows start on 16-byte
     // words, all in flight at once.
     const int stretch = slice / kSampleWarps;  // a warp's logits, a multiple of 8
@@ -212,6 +222,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         }
         return make_float2(high, low);
     };
+    cluster_started_wait();
     const float2 extent = cluster_bounds(most, least_logit);
     float top = extent.x;
     if (top == CUDART_INF_F) {
