@@ -65,7 +65,11 @@ struct PieceInfo {
     int h;
     int begin, key_first, key_end;  // first key of the piece; keys that any row sees
     int all_first, all_last;        // keys that every row sees
-    int poison_first, poison_last;  // keys with values that are not finite, of those that only some rows see
+    // Keys with values that are not finite, of those that only some rows see: bit
+    // i of [0] is key_first + i (below all_first), of [1] all_last + 1 + i. A tile
+    // has kTileRows tokens at most, so that neither has as many bits.
+    uint32_t poison[2][kTileRows / 32];
+    int poisoned;                   // there are such keys
     int twin;                       // tile 0: where tile 1's info is (-1: it has no rows)
     int whole, slot;                // slot: which of the CTA's two partial sums
     JoinNote note;
@@ -389,8 +393,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     pi.key_end = pc.tile.key_end;
                     pi.all_first = pc.tile.all_first;
                     pi.all_last = pc.tile.all_last;
-                    pi.poison_first = 0x7fffffff;
-                    pi.poison_last = -1;
+                    for (int i = 0; i < 2 * kTileRows / 32; ++i) (&pi.poison[0][0])[i] = 0;
+                    pi.poisoned = 0;
                     pi.twin = pc.tile.rows > 128 ? (int)(turn[1] - 1 & 1) : -1;
                     pi.whole = pc.whole();
                     pi.slot = pc.index > 0;
@@ -517,12 +521,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                 clear |= !finite16<K>(*reinterpret_cast<const uint4*>(v + (j >> 3) * L::kHalf +
                                                                                       swz128(row, j & 7)));
                             if (clear) {
-                                atomicMin(&pi.poison_first, key);
-                                atomicMax(&pi.poison_last, key);
-                                if (pi.twin >= 0) {
-                                    atomicMin(&bar.piece[1][pi.twin].poison_first, key);
-                                    atomicMax(&bar.piece[1][pi.twin].poison_last, key);
-                                }
+                                const int side = key > pi.all_last;
+                                const int bit = key - (side ? pi.all_last + 1 : pi.key_first);
+                                auto note = [&](PieceInfo& info) {
+                                    atomicOr(&info.poison[side][bit >> 5], 1u << (bit & 31));
+                                    info.poisoned = 1;
+                                };
+                                note(pi);
+                                if (pi.twin >= 0) note(bar.piece[1][pi.twin]);
                             }
                         }
                         if (clear)
@@ -666,7 +672,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const size_t slot = ((size_t)blockIdx.x * 2 + pi.slot) * kTileRows + 128 * t;
             const float inv = (whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f) * (K == Kind::kF32 ? 1.0f : back);
             const bool none = whole && !(l != 0.0f);
-            const bool poisoned = position >= pi.poison_first && (a.window == 0 || position - a.window < pi.poison_last);
+            bool poisoned = false;
+            if (pi.poisoned) {
+                const int oldest = a.window > 0 ? max(position - a.window + 1, 0) : 0;
+#pragma unroll 1
+                for (int i = 0; i < 2 * kTileRows / 32; ++i) {
+                    const int word = i % (kTileRows / 32), side = i / (kTileRows / 32);
+                    const int key = (side ? pi.all_last + 1 : pi.key_first) + 32 * word;  // of the word's first bit
+                    const int from = max(oldest - key, 0), to = min(position - key, 31);
+                    if (from <= to) poisoned |= (pi.poison[side][word] >> from << from & 0xffffffffu >> (31 - to)) != 0;
+                }
+            }
             const int rows = pi.rows;
             const int head = pi.h * group + r % group;
             const size_t out_row = (size_t)pi.first_row + r / group;

@@ -106,3 +106,22 @@ def test_clusters_with_ctas_that_have_few_or_no_logits(vocab, rows):
         for kw in ({}, {"temperature": torch.zeros(rows, device="cuda")}, {"top_p": torch.full((rows,), 0.9, device="cuda")}):
             for _ in range(50):
                 assert (q.sample(x, u, **kw)[0] == at).all()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("new,ctx,heads,kv", [([300], [330], 2, 2), ([300, 70], [700, 70], 8, 2), ([64, 900], [64, 1000], 5, 1)])
+@pytest.mark.parametrize("window", [0, 1, 16, 40, 200])
+def test_attention_of_chunks_with_several_values_that_are_not_finite(kind, new, ctx, heads, kv, window):
+    """Keys whose values are not finite, further apart than a window and next to each other, in the first sequence: tokens
+    that attend to none of them keep their results to the bit, those between two of them too."""
+    c = Case(new, ctx, kind=kind, heads=heads, kv=kv)
+    clean, _ = c.attend(window=window)
+    n, length = new[0], ctx[0]
+    position = torch.arange(length - n, length, device="cuda")
+    sees = torch.zeros(n, dtype=torch.bool, device="cuda")
+    for at in (length - n + 1, length - n + n // 3, length - n + n // 3 + 1, length - n + 3 * n // 4, length - 2):
+        c.v[int(c.table[0, at // 16]), :, at % 16] = math.inf if at % 2 else math.nan
+        sees |= (position >= at) & ((position - window < at) if window else torch.ones_like(sees))
+        out, _ = c.attend(window=window)
+        assert torch.equal(out[:n][~sees], clean[:n][~sees]) and torch.equal(out[n:], clean[n:])
+        assert not out[:n][sees].isfinite().any()
