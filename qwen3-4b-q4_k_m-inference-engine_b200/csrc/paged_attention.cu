@@ -38,11 +38,14 @@ template <Kind K>
 constexpr float kBias = K == Kind::kBf16 ? 0.0f : 7.0f;
 // The tensor cores truncate their fp32 sums: each MMA takes on average half a
 // last place, kTruncation of the sum so far (2^-24 of the mean of 1 / mantissa),
-// off O, which is given back. fp32 activations cannot leave it at that (1.5e-6
-// after 512 keys, 7e-6 after 4500, measured without either): their O also leaves
-// TMEM every kFlush blocks for a sum in the workspace.
+// off O, and addends are truncated too (values of one sign lose 1.7 times as much):
+// 7e-6 after 4500 keys, 6e-4 after 131072. So O leaves TMEM every kFlush blocks for
+// a sum in the workspace: 128 MMAs for fp32 activations, who are also given back
+// kTruncation of it (2.5e-6 left for values of mean and spread 1, whatever the
+// context), 1024 for 16-bit ones, whose outputs' rounding hides the 3e-5 left.
 constexpr float kTruncation = 0.7213f / 16777216.0f;
-constexpr int kFlush = 8;
+template <Kind K>
+constexpr int kFlush = K == Kind::kF32 ? 8 : 64;
 
 template <Kind K>
 struct Types {
@@ -113,7 +116,7 @@ struct Partials {
     JoinNote* notes;  // [ctas][2]
     float2* ml;        // [ctas][2][kTileRows]
     float* o;          // [ctas][2][kTileRows][D]
-    float4* flushed;   // [ctas][D / 4][kTileRows]: fp32 activations' sums over a long piece
+    float4* flushed;   // [ctas][D / 4][kTileRows]: sums over a long piece
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -344,7 +347,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             ok = wait_or_dead(&bar.p_full[t][part], phase, dead);
                             if (!ok) break;
                             tc_fence_after();
-                            value(t, v_stage, part, (K == Kind::kF32 ? i % kFlush : i) > 0 || part > 0);
+                            value(t, v_stage, part, i % kFlush<K> > 0 || part > 0);
                         }
                         if (!ok) break;
                         if (more) {
@@ -493,13 +496,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             int hi = (row < pi.rows ? min(position, held - 1) : -1) - pi.begin - 64 * h;
             int lo = (a.window > 0 ? max(position - a.window + 1, 0) : 0) - pi.begin - 64 * h;
             float m = -CUDART_INF_F, l = 0.0f;
-            // fp32 activations: sums since the last flush of O are l and steps, those
-            // before it l_flushed, its reference point m_flushed
+            // sums since the last flush of O are l and steps, those before it
+            // l_flushed, its reference point m_flushed
+            // (16-bit: l is of all blocks)
+            constexpr bool kBack = K == Kind::kF32;
             float steps = 0.0f, l_flushed = 0.0f, m_flushed = -CUDART_INF_F;
             float4* const flushed = part.flushed + ((size_t)blockIdx.x * (D / 4) + h * (D / 8)) * kTileRows + 128 * t + row;
             // The sums so far being O l' / l, with l' the row's sum then, the 16 MMAs
             // of a block have taken 16 kTruncation sum(l') / l of O.
-            auto give_back = [&] { return l > 0.0f ? 1.0f + 16.0f * kTruncation * steps / l : 1.0f; };
+            auto give_back = [&] { return kBack && l > 0.0f ? 1.0f + 16.0f * kTruncation * steps / l : 1.0f; };
             auto flushed_factor = [&] { return m_flushed == m ? 1.0f : exp2_fast(m_flushed - m); };
             for (int i = 0; i < count; ++i, ++phase, hi -= kBlockKeys, lo -= kBlockKeys) {
                 if (t == 0 && h == 0) {
@@ -543,10 +548,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 __syncwarp();
                 tc_fence_after();
                 bool fresh = i == 0;  // O begins anew with this block
-                if (K == Kind::kF32 && i > 0 && i % kFlush == 0) {
+                if (i > 0 && i % kFlush<K> == 0) {
                     // the score MMAs of this block were committed after the last
                     // block's value MMAs: O is at rest
-                    const float back = give_back(), f = i == kFlush ? 0.0f : flushed_factor();
+                    const float back = give_back(), f = i == kFlush<K> ? 0.0f : flushed_factor();
 #pragma unroll 1
                     for (int j = 0; j < D / 2; j += 16) {
                         uint32_t o[16];
@@ -556,7 +561,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         for (int e = 0; e < 16; e += 4) {
                             float4* const at = flushed + (size_t)((j + e) / 4) * kTileRows;
                             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            if (i > kFlush) v = *at;
+                            if (i > kFlush<K>) v = *at;
                             v.x = fmaf(v.x, f, back * __uint_as_float(o[e]));
                             v.y = fmaf(v.y, f, back * __uint_as_float(o[e + 1]));
                             v.z = fmaf(v.z, f, back * __uint_as_float(o[e + 2]));
@@ -565,8 +570,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                     }
                     m_flushed = m;
-                    l_flushed += l;
-                    l = steps = 0.0f;
+                    if (kBack) {
+                        l_flushed += l;
+                        l = steps = 0.0f;
+                    }
                     fresh = true;
                 }
                 uint32_t s[2][32];
@@ -596,10 +603,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (__any_sync(0xffffffffu, top > m + kLazy)) {
                     const float mn = top > m + kLazy ? top : m;
                     const float f = mn == m ? 1.0f : exp2_fast(m - mn);
-                    if (K == Kind::kF32) l_flushed *= f;
+                    if (kBack) l_flushed *= f;
+                    if (!kBack || !fresh) l *= f;
                     if (!fresh) {
-                        l *= f;
-                        steps *= f;
+                        if (kBack) steps *= f;
                         // (at rest, as above)
 #pragma unroll 1
                         for (int j = 0; j < D / 16; j += 2) {
@@ -644,7 +651,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 }
                 float sum0, sum1;
                 unpack_f32x2(add_f32x2(sum[0], sum[1]), sum0, sum1);
-                steps += fmaf(0.5f, sum0 + sum1, l);
+                if (kBack) steps += fmaf(0.5f, sum0 + sum1, l);
                 l += sum0 + sum1;
                 tmem_wait_st();
                 tc_fence_before();
@@ -656,9 +663,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             tc_fence_after();
             n += 2 * count;
             const float back = give_back();
-            const bool was_flushed = K == Kind::kF32 && count > kFlush;
+            const bool was_flushed = count > kFlush<K>;
             const float before = was_flushed ? flushed_factor() : 0.0f;
-            if (K == Kind::kF32) l += l_flushed;
+            if (kBack) l += l_flushed;
             // the row's sum, from both halves
             if (h == 1) *run = __float_as_int(l);
             named_barrier(pair_barrier, 64);
@@ -670,7 +677,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             l = __int_as_float(*run);
             const bool whole = pi.whole;
             const size_t slot = ((size_t)blockIdx.x * 2 + pi.slot) * kTileRows + 128 * t;
-            const float inv = (whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f) * (K == Kind::kF32 ? 1.0f : back);
+            const float inv = whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f;
             const bool none = whole && !(l != 0.0f);
             bool poisoned = false;
             if (pi.poisoned) {
@@ -692,7 +699,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 uint32_t o[32];
                 tmem_ld32(o_addr + 32 * j, o);
                 tmem_wait_ld();
-                if constexpr (K == Kind::kF32) {
+                if (kBack || was_flushed) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -788,6 +795,12 @@ constexpr int kDecodeKeys = 64;
 // Shares of one block: 1 sequence of 500 in 10.4 us; of two 10.8, of four 13.5.
 constexpr int kDecodeMinUnits = 1;
 constexpr int kDecodeCost = 1;
+// A warp's blocks between two drains of its outputs from the MMA's sums, which are
+// truncated, to fp32 ones in shared memory (see kTruncation; 4 or 8 MMAs a block
+// here): without them fp32 activations would lose 3e-5 over 32768 keys of values
+// of mean and spread 1, and 1.3e-4 over 131072.
+template <Kind K>
+constexpr int kDrain = K == Kind::kF32 ? 8 : 64;
 
 template <Kind K, int D, int ROWS>
 struct DecodeLayout {
@@ -986,6 +999,37 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
             float o[D / 8][4];
 #pragma unroll
             for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+            // o to the join area, onto what is there of this piece (its reference
+            // point: m_drained)
+            int undrained = 0;
+            bool drained = false;
+            float m_drained[kR];
+            auto drain = [&] {
+#pragma unroll
+                for (int y = 0; y < kR; ++y) {
+                    float* dst = join_o + (warp * ROWS + g + 8 * y) * D + 2 * t;
+                    const float f = m_drained[y] == m[y] ? 1.0f : exp2_fast(m_drained[y] - m[y]);
+#pragma unroll
+                    for (int j = 0; j < D / 8; ++j) {
+                        float2 v;
+                        if constexpr (kStacked)
+                            v = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
+                        else
+                            v = make_float2(o[j][2 * y], o[j][2 * y + 1]);
+                        if (drained) {
+                            const float2 u = *reinterpret_cast<const float2*>(dst + 8 * j);
+                            v = make_float2(fmaf(u.x, f, v.x), fmaf(u.y, f, v.y));
+                        }
+                        *reinterpret_cast<float2*>(dst + 8 * j) = v;
+                    }
+                    m_drained[y] = m[y];
+                }
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+                drained = true;
+            };
+#pragma unroll
+            for (int y = 0; y < kR; ++y) m_drained[y] = 0.0f;
 
             // this warp's blocks of the piece
             for (int i = (warp - n0 % kWarps + kWarps) % kWarps; i < pc.count && ok; i += kWarps) {
@@ -1134,24 +1178,19 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar.empty[st]);
+                if (++undrained == kDrain<K>) {
+                    drain();
+                    undrained = 0;
+                }
             }
             n0 += pc.count;
 
             // join the warps
+            drain();
 #pragma unroll
             for (int y = 0; y < kR; ++y) {
                 const int row = g + 8 * y;
                 l[y] = quad_sum(l[y]);
-                float* dst = join_o + (warp * ROWS + row) * D + 2 * t;
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j) {
-                    float2 v;
-                    if constexpr (kStacked)
-                        v = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
-                    else
-                        v = make_float2(o[j][2 * y], o[j][2 * y + 1]);
-                    *reinterpret_cast<float2*>(dst + 8 * j) = v;
-                }
                 if (t == 0) join_ml[warp * ROWS + row] = make_float2(m[y], l[y]);
             }
             if (named_barrier_or(1, kWarps * 32, !ok)) {

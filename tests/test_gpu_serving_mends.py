@@ -125,3 +125,34 @@ def test_attention_of_chunks_with_several_values_that_are_not_finite(kind, new, 
         out, _ = c.attend(window=window)
         assert torch.equal(out[:n][~sees], clean[:n][~sees]) and torch.equal(out[n:], clean[n:])
         assert not out[:n][sees].isfinite().any()
+
+
+@pytest.mark.parametrize("kind,ctx,group,new", [("f32", 65536, 1, 1), ("f32", 65536, 4, 3), ("f32", 65536, 4, 12), ("f16", 131072, 4, 1), ("f16", 131072, 4, 12),
+                                                ("f16", 131072, 1, 40)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("mean", [0.0, 1.0])
+def test_attention_sums_over_long_contexts(kind, ctx, group, new, d, mean):
+    """Many sequences over a long context, each tile's in one CTA: the tensor cores' truncated sums do not add up.
+
+    A sum leaves them after 8 (fp32) or 64 (16-bit) blocks, 64 or 128 and 512 or 1024 MMAs, each of which may take its
+    last place, 2^-23, off it and as much off what it adds, and is half grown on the average; queries and probabilities
+    have 2^-21 as fp16 pairs. fp16 outputs are rounded without bias."""
+    n, kv, page = 40, 8, 128
+    act, cached = TYPES[kind]
+    g = torch.Generator(device="cuda").manual_seed(31)
+    k = torch.randn(ctx // page, kv, page, d, generator=g, device="cuda").to(cached)
+    v = (torch.randn(ctx // page, kv, page, d, generator=g, device="cuda") + mean).to(cached)
+    table = torch.randperm(ctx // page, generator=g, device="cuda").int()[None]
+    query = torch.randn(n * new, kv * group, d, generator=g, device="cuda").to(act)
+    q_start, kv_len = (torch.arange(n + 1) * new).int().cuda(), torch.full((n,), ctx, dtype=torch.int32, device="cuda")
+    out = q.paged_attention(q.PagedKV(k, v), q.PagedBatch(q_start, kv_len, table.expand(n, -1), max_new=new), query)
+    position = ctx - new + torch.arange(n * new, device="cuda") % new
+    hidden = torch.arange(ctx, device="cuda") > position[:, None]
+    mmas = (64 if new * group <= 16 else 128) * (1 if kind == "f32" else 8)
+    for h in (0, kv * group - 1):
+        keys, values = (t[table[0].long(), h // group].flatten(0, 1).double() for t in (k, v))
+        want = torch.softmax((query[:, h].double() @ keys.T * d ** -0.5).masked_fill(hidden, -math.inf), -1) @ values
+        err = out[:, h].double() - want
+        assert abs(float((err * want).sum() / (want * want).sum())) <= mmas * 2.0 ** -23 + 2.0 ** -21
+        if kind == "f32":
+            assert err.norm() <= (mmas * 2.0 ** -23 + 2.0 ** -21) * want.norm()
