@@ -265,7 +265,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 if (i + 1 < pc.count) next_page = page_of(key0 + kBlockKeys);  // a block ahead
                 for (int kv = 0; kv < 2 && ok; ++kv, ++n) {
                     const int st = n % kStages;
-                    ok = wait_or_dead(&bar.empty[st], ((n / kStages) & 1) ^ 1, dead);
+                    // (once a wait has given up no stage is filled again: one whose copy is
+                    // missing may have been given back in that copy's phase)
+                    ok = wait_or_dead(&bar.empty[st], ((n / kStages) & 1) ^ 1, dead) && !*dead;
                     if (!__all_sync(0xffffffffu, ok)) {
                         ok = false;
                         break;
@@ -362,10 +364,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     tc_commit(&bar.empty[v_stage % kStages]);
                     if (more) tc_commit(&bar.empty[k_stage % kStages]);
                 }
-            }
-            if (!ok) {  // the MMAs in flight end before the TMEM is freed
-                tc_commit(&bar.done);
-                mbar_wait_bounded(&bar.done, 0, nullptr, 0);
             }
         }
         __syncwarp();
@@ -774,6 +772,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tc_fence_before();
     __syncthreads();
     if (warp == kMmaWarp) {
+        if (*dead && lane == 0) {  // the MMAs in flight end before the TMEM is freed
+            tc_commit(&bar.done);
+            mbar_wait_bounded(&bar.done, 0, nullptr, 0);
+        }
+        __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
