@@ -265,9 +265,8 @@ int q4k_paged_append(const q4k_paged_kv* cache, const q4k_paged_batch* batch, si
  * to them (all of whose outputs may then be NaN); what stands in pages behind
  * a sequence's end reaches none. workspace: q4k_paged_attention_workspace_bytes
  * of the same call's numbers, 16-byte aligned, contents irrelevant; calls that
- * may overlap in time need workspaces of their own. As in
- * q4k_attention_decode_f16, waits on copies are bounded (2 s); if one gives up,
- * the output is undefined. */
+ * may overlap in time need workspaces of their own. Waits on copies are bounded
+ * (2 s); rows whose part of the work met one that gave up are NaN, lse too. */
 int q4k_paged_attention(const q4k_paged_kv* cache, const q4k_paged_batch* batch, size_t tokens, int type,
                         const void* q, int64_t ld_q, int query_heads, float scale, int window, void* output,
                         int64_t ld_output, float* lse, void* workspace, size_t workspace_bytes, void* stream);

@@ -242,6 +242,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     fence_proxy_async();  // the plan's words, before the ring's copies land on them
     __syncthreads();
 
+    // The walking and the softmax warps go through all pieces even after a wait has
+    // given up, as their rows have to be written: a piece then takes 2 s at most.
+    auto piece_wait = [&](uint64_t* b, uint32_t parity) {
+        bool ok = false;
+        for (int i = 0; i < 4 && !ok; ++i) ok = mbar_wait_bounded(b, parity, nullptr, 0);
+        return ok;
+    };
+
     if (warp == kTmaWarp) {
         // ---------------- TMA: K and V blocks, page by page, a lane per (page, half)
         Walk pc(a.batch, group, a.cache.kv_heads, a.window, held, bar.share);
@@ -379,7 +387,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int t = 1; t >= 0 && ok; --t) {
                     if (more && pc.tile.rows <= 128 * t) continue;
                     const uint32_t slot = turn[t] & 1;
-                    ok = wait_or_dead(&bar.piece_empty[t][slot], (turn[t] >> 1 & 1) ^ 1, dead);
+                    ok = piece_wait(&bar.piece_empty[t][slot], (turn[t] >> 1 & 1) ^ 1);
                     if (!ok) break;
                     ++turn[t];
                     PieceInfo& pi = bar.piece[t][slot];
@@ -420,10 +428,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int left = 0;  // bit i: partial sum i has been left
         // (a wait that gives up is not acted on within a piece: every warp goes
         // through the same barriers, and once one wait has given up the others
-        // return at once)
+        // return at once; the rows of that piece and of later ones become NaN)
         for (uint32_t items = 0;; ++items) {
             PieceInfo& pi = bar.piece[t][items & 1];
-            const bool there = wait_or_dead(&bar.piece_full[t][items & 1], items >> 1 & 1, dead);
+            const bool there = piece_wait(&bar.piece_full[t][items & 1], items >> 1 & 1);
             // and the last piece's outputs have left the shared memory
             if (named_barrier_or(tile_barrier, 256, !there)) break;
             const int count = pi.count;
@@ -672,12 +680,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 *run = __float_as_int(l);
             }
             named_barrier(pair_barrier, 64);
-            l = __int_as_float(*run);
+            const bool lost = *dead != 0;
+            l = lost ? CUDART_NAN_F : __int_as_float(*run);
             const bool whole = pi.whole;
             const size_t slot = ((size_t)blockIdx.x * 2 + pi.slot) * kTileRows + 128 * t;
             const float inv = whole ? (l > 0.0f ? 1.0f / l : 0.0f) : 1.0f;
             const bool none = whole && !(l != 0.0f);
-            bool poisoned = false;
+            bool poisoned = lost;
             if (pi.poisoned) {
                 const int oldest = a.window > 0 ? max(position - a.window + 1, 0) : 0;
 #pragma unroll 1
@@ -1196,10 +1205,8 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
                 l[y] = quad_sum(l[y]);
                 if (t == 0) join_ml[warp * ROWS + row] = make_float2(m[y], l[y]);
             }
-            if (named_barrier_or(1, kWarps * 32, !ok)) {
-                ok = false;
-                break;
-            }
+            // (once a wait has given up, this piece's rows and those of later ones are NaN)
+            ok = !named_barrier_or(1, kWarps * 32, !ok);
             const bool whole = pc.whole();
             const size_t slot = ((size_t)blockIdx.x * 2 + (pc.index > 0)) * ROWS;
             for (int x = tid; x < tl.rows * (D / 4); x += kWarps * 32) {
@@ -1220,6 +1227,7 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
                     v[2] += f * u.z;
                     v[3] += f * u.w;
                 }
+                if (!ok) sum = CUDART_NAN_F;
                 const int r = tl.row0 + row;
                 const int head = pc.h * group + r % group;
                 const size_t out_row = (size_t)pc.seq.first_row + r / group;
