@@ -286,7 +286,8 @@ size_t q4k_paged_attention_workspace_bytes(int query_heads, int kv_heads, int he
  * the row. tokens[r] is -1 (logprob -inf) for a row with no logit above -inf.
  * logprob (optional) receives the natural logarithm of the token's probability
  * among the kept. Sums are exact (whole numbers), so results do not depend on
- * how the work is split. vocab <= 400000. */
+ * how the work is split. A row that has not arrived on the chip after 2 s gets
+ * token -1 and logprob NaN. vocab <= 400000. */
 int q4k_sample(const void* logits, int type, int64_t ld, size_t rows, size_t vocab, const float* temperature,
                const int* top_k, const float* top_p, const float* min_p, const float* uniform, int32_t* tokens,
                float* logprob, void* stream);

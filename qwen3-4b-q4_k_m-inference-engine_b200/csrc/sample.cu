@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         }
     };
     __syncthreads();
-    mbar_wait_bounded(&sh.landed[warp / (kSampleWarps / kCopies)], 0, nullptr, 0);
+    const bool lost = !mbar_wait_bounded(&sh.landed[warp / (kSampleWarps / kCopies)], 0, nullptr, 0);
     float most = -CUDART_INF_F, least_logit = CUDART_INF_F;
     for_each([&](const float(&l)[kVec], int) {
 #pragma unroll
@@ -199,11 +199,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
         }
     });
 
-    // The largest and smallest of a value over the cluster.
-    auto cluster_bounds = [&](float high, float low) {
+    // The largest and smallest of a value over the cluster; NaN if any thread says `bad`.
+    auto cluster_bounds = [&](float high, float low, bool bad = false) {
         high = warp_max(high);
         low = -warp_max(-low);
-        __syncthreads();
+        bad = __syncthreads_or(bad);
         if (lane == 0) sh.warp_sum[warp] = (u64)__float_as_uint(low) << 32 | __float_as_uint(high);
         __syncthreads();
         if (tid < ranks) {
@@ -212,19 +212,28 @@ __global__ void __launch_bounds__(kSampleThreads, 2)
                 low = fminf(low, __uint_as_float((uint32_t)(sh.warp_sum[w] >> 32)));
             }
             float* to = cluster.map_shared_rank(&sh.bound[0][0], tid);
-            to[rank] = high;
+            to[rank] = bad ? CUDART_NAN_F : high;
             to[kMaxCluster + rank] = low;
         }
         cluster.sync();
         for (int r = 0; r < ranks; ++r) {
+            bad |= sh.bound[0][r] != sh.bound[0][r];
             high = fmaxf(high, sh.bound[0][r]);
             low = fminf(low, sh.bound[1][r]);
         }
-        return make_float2(high, low);
+        return make_float2(bad ? CUDART_NAN_F : high, low);
     };
     cluster_started_wait();
-    const float2 extent = cluster_bounds(most, least_logit);
+    const float2 extent = cluster_bounds(most, least_logit, lost);
     float top = extent.x;
+    if (top != top) {  // a part of the row has not arrived, here or in another CTA
+        for (int i = 0; i < kCopies; ++i) mbar_wait_bounded(&sh.landed[i], 0, nullptr, 0);
+        if (rank == 0 && tid == 0) {
+            a.tokens[row] = -1;
+            if (a.logprob) a.logprob[row] = CUDART_NAN_F;
+        }
+        return;
+    }
     if (top == CUDART_INF_F) {
         // infinite logits share the row: as equal finite ones
         for (int i = tid; i < slice; i += kSampleThreads)

@@ -1,8 +1,8 @@
-// Bounded waits of the paged attention kernels that run out: the kernels are
-// compiled here with copies that can be left out, so that what waits for them
-// gives up after its limit. Rows whose work met that are NaN, all others keep
-// their results to the bit, and the next call is right again. No other access
-// changes.
+// Bounded waits of the paged attention kernels and of the sampler that run out:
+// the kernels are compiled here with copies that can be left out, so that what
+// waits for them gives up after its limit. Rows whose work met that are NaN (a
+// sampled row: token -1, logprob NaN), all others keep their results to the bit,
+// and the next call is right again. No other access changes.
 #define kWaitLimitNs kLibraryWaitLimitNs
 #include "q4k_device.cuh"
 #undef kWaitLimitNs
@@ -13,6 +13,7 @@ constexpr uint64_t kWaitLimitNs = 20000000ull;  // of the attention kernels' wai
 
 namespace q4k {
 __device__ int lost_page = -1;                // of KV head 0
+__device__ unsigned long long lost_source = 0;  // address, of a bulk copy
 namespace paged_dev {
 __device__ __forceinline__ void tma_load_4d_or_not(void* dst, const CUtensorMap* map, int x, int y, int z, int w,
                                                    uint64_t* bar) {
@@ -20,10 +21,16 @@ __device__ __forceinline__ void tma_load_4d_or_not(void* dst, const CUtensorMap*
     tma_load_4d(dst, map, x, y, z, w, bar);
 }
 }  // namespace paged_dev
+__device__ __forceinline__ void bulk_g2s_or_not(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    if (reinterpret_cast<unsigned long long>(src) != lost_source) bulk_g2s(dst, src, bytes, bar);
+}
 }  // namespace q4k
 #define tma_load_4d tma_load_4d_or_not
 #include "paged_attention.cu"
 #undef tma_load_4d
+#define bulk_g2s bulk_g2s_or_not
+#include "sample.cu"
+#undef bulk_g2s
 
 #include <algorithm>
 #include <cstdio>
@@ -158,6 +165,35 @@ static int attention(const char* name, bool f32, bool bf16, int d, int sequences
     return wrong + (same == 0);
 }
 
+static int sampling() {
+    const int rows = 3, vocab = 40000;
+    std::mt19937 rng(9);
+    std::normal_distribution<float> normal;
+    std::vector<float> logits((size_t)rows * vocab), uniform(rows, 0.4f);
+    for (auto& x : logits) x = normal(rng);
+    q4k::SampleArgs a;
+    const float* l = device(logits);
+    a.logits = l, a.type = Q4K_TYPE_F32, a.ld = vocab, a.rows = rows, a.vocab = vocab;
+    a.uniform = device(uniform);
+    a.tokens = device(std::vector<int>(rows));
+    a.logprob = device(std::vector<float>(rows));
+    std::vector<int> tokens[3];
+    std::vector<float> logprob[3];
+    for (int i = 0; i < 3; ++i) {
+        const unsigned long long lost = i == 1 ? reinterpret_cast<unsigned long long>(l + vocab) : 0;  // the first stretch of row 1
+        must(cudaMemcpyToSymbol(q4k::lost_source, &lost, sizeof lost), "symbol");
+        must(q4k::sample(a, nullptr), "launch");
+        must(cudaDeviceSynchronize(), "run");
+        tokens[i] = host(a.tokens, rows), logprob[i] = host(a.logprob, rows);
+    }
+    int wrong = tokens[0] != tokens[2] || logprob[0] != logprob[2];
+    for (int r = 0; r < rows; ++r)
+        wrong += r == 1 ? tokens[1][r] != -1 || logprob[1][r] == logprob[1][r]
+                        : tokens[1][r] != tokens[0][r] || logprob[1][r] != logprob[0][r];
+    std::printf("sampling: tokens %d %d %d, %d wrong\n", tokens[1][0], tokens[1][1], tokens[1][2], wrong);
+    return wrong;
+}
+
 int main() {
     int wrong = 0;
     // tiles shared by many CTAs, then tiles of one CTA, of both kernels
@@ -167,6 +203,7 @@ int main() {
     wrong += attention("chunk, fp32", true, false, 128, 2, 200, 3000, 8, 2);
     wrong += attention("chunk, bf16", false, true, 128, 40, 70, 300, 16, 4);
     wrong += attention("chunk, fp16", false, false, 64, 3, 90, 700, 10, 2);
+    wrong += sampling();
     std::printf("%d wrong in all\n", wrong);
     return wrong != 0;
 }

@@ -1,6 +1,7 @@
-"""Bounded waits of the paged attention kernels that are made to run out: the checker, tests/cuda/lost_copy_test.cu,
-compiles the kernels with copies that can be left out, and is compiled here with nvcc. The call ends without a fault,
-rows whose work waited for one are NaN, the others are as before, and so is the next call."""
+"""Bounded waits of the paged attention kernels and of the sampler that are made to run out: the checker,
+tests/cuda/lost_copy_test.cu, compiles the kernels with copies that can be left out, and is compiled here with nvcc. The
+call ends without a fault, rows whose work waited for one are NaN (a sampled row: token -1), the others are as before, and
+so is the next call."""
 import os
 import subprocess
 
