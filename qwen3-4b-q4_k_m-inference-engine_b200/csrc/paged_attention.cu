@@ -158,13 +158,16 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
 }
 
 // The power of two, as two factors, that brings a row of largest magnitude
-// `most` to below 2^8 (any fp32 row then fits fp16 parts), and c divided by it.
+// `most` to below 2^8 (any fp32 row then fits fp16 parts), and c divided by it:
+// at least the smallest normal number, whose products with scores, below 2^31,
+// are 0 to the exponential as well, and which leaves masked scores at -infinity.
 __device__ __forceinline__ void row_scale(float most, float c, float& f1, float& f2, float& c_out) {
     const int e = min(max((int)(__float_as_uint(most) >> 23) - 126, -100), 127);  // most < 2^e
     const int e1 = (8 - e) / 2, e2 = 8 - e - e1;
     f1 = __uint_as_float((uint32_t)(127 + e1) << 23);
     f2 = __uint_as_float((uint32_t)(127 + e2) << 23);
-    c_out = c * __uint_as_float((uint32_t)(127 - e1) << 23) * __uint_as_float((uint32_t)(127 - e2) << 23);
+    c_out = fmaxf(c * __uint_as_float((uint32_t)(127 - e1) << 23) * __uint_as_float((uint32_t)(127 - e2) << 23),
+                  1.17549435e-38f);
 }
 
 // Signed whole numbers in the order of the floats.

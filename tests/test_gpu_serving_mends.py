@@ -156,3 +156,30 @@ def test_attention_sums_over_long_contexts(kind, ctx, group, new, d, mean):
         assert abs(float((err * want).sum() / (want * want).sum())) <= mmas * 2.0 ** -23 + 2.0 ** -21
         if kind == "f32":
             assert err.norm() <= (mmas * 2.0 ** -23 + 2.0 ** -21) * want.norm()
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("new,ctx", [([1, 3], [90, 200]), ([70, 5], [200, 5])])
+@pytest.mark.parametrize("scale", [1e-45, 1e-30, 1e-13])
+def test_attention_with_scales_that_leave_no_differences(kind, new, ctx, scale):
+    """Queries of zeros or small values under scales whose product with them is below fp32's range: every key that a token
+    sees weighs the same (to check()'s bounds: the scores are below 1e-10 and their differences round away)."""
+    c = Case(new, ctx, kind=kind, seed=8)
+    c.q[::2] = 0.0
+    c.q[1::2] *= 1e-3
+    c.check(*c.attend(scale=scale), scale=scale)
+    c.check(*c.attend(scale=scale, window=20), window=20, scale=scale)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("new,ctx", [([1, 3], [90, 200]), ([70, 5], [200, 5])])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_attention_of_queries_that_are_not_finite(kind, new, ctx, bad):
+    """They reach no output but their own token's and head's."""
+    c = Case(new, ctx, kind=kind, seed=9)
+    clean, clean_lse = c.attend()
+    c.q[1, 2, 5] = bad
+    out, lse = c.attend()
+    assert not out[1, 2].isfinite().any() and not lse[1, 2].isfinite()
+    out[1, 2], lse[1, 2] = clean[1, 2], clean_lse[1, 2]
+    assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
