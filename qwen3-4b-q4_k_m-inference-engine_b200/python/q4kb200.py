@@ -666,7 +666,7 @@ def paged_attention(cache: PagedKV, batch: PagedBatch, q, out=None, lse=None, sc
             _refuse("the workspace must be contiguous, on the cache's device")
         size = workspace.numel() * workspace.element_size()
     _call(index, (_lib or lib()).q4k_paged_attention, cache.packed, batch.packed, tokens, _type_of(q.dtype), q.data_ptr(), lq, heads,
-          scale, window, out.data_ptr(), lo, pl, workspace.data_ptr(), size, s)
+          scale, min(max(window, -1), 0x7fffffff), out.data_ptr(), lo, pl, workspace.data_ptr(), size, s)
     return out
 
 

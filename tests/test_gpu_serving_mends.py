@@ -183,3 +183,9 @@ def test_attention_of_queries_that_are_not_finite(kind, new, ctx, bad):
     assert not out[1, 2].isfinite().any() and not lse[1, 2].isfinite()
     out[1, 2], lse[1, 2] = clean[1, 2], clean_lse[1, 2]
     assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
+def test_attention_windows_beyond_an_int():
+    c = Case([1, 40], [300, 60], kind="f16")
+    for window in (1 << 31, (1 << 32) + 5, 1 << 63):
+        assert all(torch.equal(x, y) for x, y in zip(c.attend(window=window), c.attend()))
