@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 // Q into shared memory, 16 rows a warp, whole rows at a time
                 constexpr int kChunks = D * (int)sizeof(Act) / 16;  // 16-byte words of a row
                 constexpr int kAtOnce = 32 / kChunks;               // rows of one load
-                constexpr int kBatch = K != Kind::kF32 && D == 128 ? 8 : 4;  // loads in flight
+                constexpr int kBatch = 4;                           // loads in flight
                 static_assert(16 % (kBatch * kAtOnce) == 0, "whole passes");
                 const int chunk = lane % kChunks;
                 // where the warp's rows are: lanes 0 .. 15 know theirs (null: past the tile)
