@@ -1,4 +1,5 @@
-"""Calls of the paged operators and the sampler that were answered wrongly, or only by luck rightly."""
+"""Paged attention where it is easily wrong: scores that rise all the time, what 16-bit probabilities lose, sums over long
+contexts, values and queries that are not finite, tiny scales, windows beyond an int, page tables of one row."""
 import math
 
 import pytest
@@ -90,22 +91,6 @@ def test_sequences_that_share_one_row_of_a_page_table(new):
     c.table = store.flatten()[: n + row.shape[1]].as_strided((n, row.shape[1]), (1, 1))
     with pytest.raises(q.InvalidArgument):
         c.attend()
-
-
-@pytest.mark.parametrize("vocab", [16385, 16900, 17281, 33000])
-@pytest.mark.parametrize("rows", [1, 4])
-def test_clusters_with_ctas_that_have_few_or_no_logits(vocab, rows):
-    """The last CTAs of a row's cluster have little or nothing to load, and tell the others of their bounds at once; the
-    largest logit in the first or last place, drawn in every repetition."""
-    g = torch.Generator(device="cuda").manual_seed(vocab)
-    logits = torch.randn(rows, vocab, generator=g, device="cuda")
-    u = torch.rand(rows, generator=g, device="cuda")
-    for at in (0, vocab - 1):
-        x = logits.clone()
-        x[:, at] = 60.0  # e^-55 and less is left to the others
-        for kw in ({}, {"temperature": torch.zeros(rows, device="cuda")}, {"top_p": torch.full((rows,), 0.9, device="cuda")}):
-            for _ in range(50):
-                assert (q.sample(x, u, **kw)[0] == at).all()
 
 
 @pytest.mark.parametrize("kind", TYPES)
