@@ -21,8 +21,9 @@ constexpr int kTileRows = 256;  // two MMA tiles of 128 query rows
 constexpr int kBlockKeys = 128;
 constexpr int kSoftmaxWarps = 16;  // two warpgroups per MMA tile, a thread per row and half of its keys
 constexpr int kTcThreads = (kSoftmaxWarps + 3) * 32;  // and a TMA, an MMA and a piece-walking warp
-// A tile's queries and outputs take as long as 4 of its blocks (prefill of 8192:
-// 578 us if 2 are reckoned, 575 with 3, 555 with 4), and a share is at least that.
+// A tile's queries and outputs take about as long as 4 of its blocks (chunk of 512
+// at 4096: 87.0 us with 2 to 4, 89.6 with 6; longer prompts the same with 2 to 6),
+// and a share is at least that.
 constexpr int kTileCost = 4;
 constexpr int kMinUnits = 4;
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -184,14 +185,16 @@ __device__ __forceinline__ float from_ordered(int k) { return __int_as_float(k ^
 // alternates between two tiles of 128 rows, so that one tile's products run under
 // the other's softmax: S = Q K^T from shared memory into TMEM, probabilities back
 // over S as 16-bit high and low parts, O += P V with P from TMEM, the first half
-// of the products under the second half of their own exponentials (prefill 739 us,
-// 766 with all after them). High parts alone would take 524 us, but leave 16-bit
-// outputs 1.4 times the error that their own rounding has. Two threads share a row, each
+// of the products under the second half of their own exponentials (bf16 prompt of
+// 8192: 739 us, 766 with all after them). High parts alone would take 524 us, but
+// leave 16-bit outputs 1.4 times the error of their own rounding. Two threads share a row, each
 // with half of a block's keys and half of the row's output: with one thread to
 // a row the two warps of an SM sub-partition could not hide their own latencies
 // (2300 cycles for a softmax of 1024 cycles of exponentials). Measured: 8192
-// bf16 tokens of 32 / 8 heads of 128 in 739 us, 744 TFLOP/s (of 1.5 times as many
-// in the products).
+// bf16 tokens of 32 / 8 heads of 128 in 720 to 790 us by the clocks of the moment
+// (853 in sustained calls), 730 TFLOP/s of 1100 in the products; tensor pipe 54%,
+// exponentials 36%, issue 43% busy: the latencies of a tile's softmax between its
+// own products, and the power limit.
 // ---------------------------------------------------------------------------
 template <Kind K, int D>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -807,7 +810,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 // of one MMA tile when those are fp32 and 8 rows suffice, else in two MMAs.
 // ---------------------------------------------------------------------------
 constexpr int kDecodeKeys = 64;
-// Shares of one block: 1 sequence of 500 in 10.4 us; of two 10.8, of four 13.5.
+// Shares of one block: 1 sequence of 500 in 11.1 us; of two 11.5, of four 14.0.
 constexpr int kDecodeMinUnits = 1;
 constexpr int kDecodeCost = 1;
 // A warp's blocks between two drains of its outputs from the MMA's sums, which are
@@ -1264,8 +1267,8 @@ __global__ void __launch_bounds__((DecodeLayout<K, D, ROWS>::kThreads), 1)
 // A row's pieces are spread over as many warps as the block's rows leave (a
 // decode step over a long context: a few rows of dozens of pieces).
 constexpr int kJoinWarps = 8;
-// Rows of a block: 16 of a tile of 256 (chunk of 512 at 4096 87.6 us, with 64
-// 96.2), 2 of a decode tile (2 sequences of 131071 56.0 us, with 8 58.2).
+// Rows of a block: 16 of a tile of 256 (chunk of 512 at 4096 86.9 us, with 64
+// 94.6), 2 of a decode tile (2 sequences of 131071 56.7 us, with 8 59.0).
 constexpr int kJoinRows = 16;
 constexpr int kJoinDecodeRows = 2;
 template <typename Act, int D, int kRows>
@@ -1411,26 +1414,32 @@ cudaError_t launch_decode(const PagedAttentionArgs& a, cudaStream_t s) {
 }
 
 // Which kernel, by the query rows per sequence and KV head. Up to the decode
-// kernel's 16 MMA rows it is ahead everywhere (us, decode / chunk kernel: 1
-// sequence of 500 with 4 rows 10.7 / 25.9, 32 of 2000 57.9 / 130, with 16 rows
-// 75.8 / 136; bf16 61.3 / 93.9 and 68.7 / 102). Up to 32 rows it reads the keys
-// twice, which it can afford with head_dim 64 (256 sequences of 1000 with 32
-// rows: 261 / 287) and where few tiles leave it latency-bound (1 sequence of
-// 500 with 32 rows 15.3 / 26.3, bf16 13.8 / 21.0; 16 of 4000, fp32, 120 / 130),
-// not with many (256 of 1000: 577 / 468; bf16 4 of 32000: 191 / 148).
+// kernel's 16 MMA rows it is ahead everywhere (us, decode / chunk kernel, 32 and 8
+// heads of 128: 1 sequence of 500 with 4 rows 10.8 / 25.0, 32 of 2000 53.8 / 125,
+// with 16 rows 73.8 / 131, bf16 57.9 / 103 and 64.1 / 109, 2 of 131071 with 4 rows
+// 160 / 402, bf16 169 / 323). Up to 32 rows it reads the keys twice, which it can
+// afford with head_dim 64 (1 sequence of 131071 with 32 rows 93 / 176, 256 of 1000
+// 260 / 374; bf16 90 / 163 and 219 / 328) and up to two tiles an SM, whatever the
+// context. With 32 rows of 128 in bf16: 1 sequence of 500 14.0 / 21.8, of 32000 47 /
+// 70, of 131071 173 / 179; 4 of 4000 30 / 40, of 32000 168 / 166, of 131071 627 / 649;
+// 16 of 500 30.6 / 28.7, of 4000 100 / 104; 32 of 500 49 / 41, of 4000 181 / 181.
+// fp32: 1 of 500 15.5 / 25.9, of 131071 195 / 221; 8 of 32000 358 / 400; 32 of 500
+// 58 / 50, of 4000 211 / 223. With more tiles it is behind more often than ahead
+// (64 of 1000 143 / 140, of 4000 398 / 415, 256 of 1000 524 / 453; bf16 116 / 119 and
+// 419 / 385 at 1000).
 constexpr int kDecodeRows = 16;
 
 bool few_rows(const PagedAttentionArgs& a, long long rows) {
     const long long tiles = (long long)a.batch.sequences * a.cache.kv_heads;
     return rows <= kDecodeRows || (rows <= 2 * kDecodeRows &&
-                                   (a.cache.head_dim == 64 || tiles <= (a.f32 ? 2 * sm_count() : 16)));
+                                   (a.cache.head_dim == 64 || tiles <= 2 * sm_count()));
 }
 
 template <Kind K, int D>
 cudaError_t launch_dim(const PagedAttentionArgs& a, cudaStream_t s) {
     const long long rows = (long long)a.batch.max_new * (a.heads / a.cache.kv_heads);
     if (!few_rows(a, rows)) return launch_tc<K, D>(a, s);
-    // (fp32, 4 rows: 10.7 us against 12.5 with 16 rows at 1 sequence of 500, 57.9 against 68.1 at 32 of 2000)
+    // (fp32, 4 rows: 11.0 us against 13.0 with 16 rows at 1 sequence of 500, 58.6 against 69.0 at 32 of 2000)
     if constexpr (K == Kind::kF32)
         if (rows <= 8) return launch_decode<K, D, 8>(a, s);
     return launch_decode<K, D, 16>(a, s);
